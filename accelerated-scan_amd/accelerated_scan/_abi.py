@@ -13,7 +13,7 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 # ascan_gate codes of include/ascan.h
 GATE_IDENTITY, GATE_SIGMOID, GATE_SIGMOID_LERP, GATE_EXP, GATE_EXP_NORM = 0, 1, 2, 3, 4
@@ -108,6 +108,36 @@ _SIGNATURES = {
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
          ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ascan_delta_blocks": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "ascan_delta_workspace_bytes": (
+        ctypes.c_size_t,
+        [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+         ctypes.c_int, ctypes.c_int, ctypes.c_int],
+    ),
+    "ascan_delta_forward": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 11 + [ctypes.c_int64] * 6
+        + [ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ascan_delta_backward": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 16 + [ctypes.c_int64] * 6
+        + [ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p],
+    ),
+    "ascan_delta_step": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 8 + [ctypes.c_int64] * 6 + [ctypes.c_float, ctypes.c_int, ctypes.c_int, ctypes.c_void_p],
+    ),
+    "ascan_gated_norm": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_void_p],
+    ),
+    "ascan_gated_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
+    "ascan_gated_norm_backward": (
+        ctypes.c_int,
+        [ctypes.c_void_p] * 7 + [ctypes.c_int64, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_void_p,
+                                 ctypes.c_size_t, ctypes.c_void_p],
     ),
     "ascan_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "ascan_last_hip_error": (ctypes.c_int, []),
@@ -376,6 +406,95 @@ def backward_lerp(gate_inputs, values, states, grad_out, d_gate_inputs, d_values
             _ptr(initial), grad_out.data_ptr(), d_gate_inputs.data_ptr(), d_values.data_ptr(), _ptr(d_initial), rows,
             seqlen, code, _ptr(workspace), workspace.numel() if workspace is not None else 0)
     _after_split(workspace, "backward_lerp")
+
+
+# ascan_delta_flags of include/ascan.h
+DELTA_GATES_F32, DELTA_OFFSETS_I64 = 1, 2
+
+
+def delta_blocks(rows: int, sequences: int, packed: bool) -> int:
+    """Blocks of 64 tokens that the sequences of a delta rule call can have."""
+    return (_lib or load()).ascan_delta_blocks(rows, sequences, 1 if packed else 0)
+
+
+def _delta_sizes(q, v, log_gates, offsets):
+    """(rows, sequences, heads, key_heads, dk, dv), dtype and flags of a delta rule call."""
+    batch, tokens, key_heads, dk = q.shape
+    heads, dv = v.shape[2:]
+    flags = DELTA_GATES_F32 if log_gates.dtype == torch.float32 else 0
+    sequences = batch
+    if offsets is not None:
+        sequences = offsets.shape[0] - 1
+        if offsets.dtype == torch.int64:
+            flags |= DELTA_OFFSETS_I64
+    return (batch * tokens, sequences, heads, key_heads, dk, dv), DTYPE_CODES[q.dtype], flags
+
+
+@functools.lru_cache(maxsize=1024)
+def _delta_workspace_bytes(rows, sequences, heads, dk, dv, code, packed, backward) -> int:
+    return (_lib or load()).ascan_delta_workspace_bytes(rows, sequences, heads, dk, dv, code, packed, backward)
+
+
+def _delta_workspace(sizes, code, packed, backward, device):
+    """Scratch memory of a delta rule call; freed by the caching allocator in stream order after its kernels."""
+    rows, sequences, heads, _, dk, dv = sizes
+    nbytes = _delta_workspace_bytes(rows, sequences, heads, dk, dv, code, 1 if packed else 0, 1 if backward else 0)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def delta_forward(q, k, v, log_gates, beta, initial, offsets, scale, out, final, states=None, updates=None) -> None:
+    """Enqueue the gated delta rule over (B, T, heads, dim) tensors; ``states`` and ``updates`` receive what
+    ``delta_backward`` needs."""
+    lib = _lib or load()
+    sizes, code, flags = _delta_sizes(q, v, log_gates, offsets)
+    workspace = _delta_workspace(sizes, code, offsets is not None, False, q.device)
+    _launch(q.device, lib.ascan_delta_forward, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_gates.data_ptr(),
+            beta.data_ptr(), _ptr(initial), _ptr(offsets), out.data_ptr(), _ptr(final), _ptr(states), _ptr(updates),
+            *sizes, scale, code, flags, workspace.data_ptr(), workspace.numel())
+
+
+def delta_backward(q, k, v, log_gates, beta, states, updates, offsets, scale, d_out, d_final, d_q, d_k, d_v,
+                   d_log_gates, d_beta, d_initial) -> None:
+    """Enqueue the backward pass of ``delta_forward`` (``d_out``, ``d_final`` and ``d_initial`` may be None)."""
+    lib = _lib or load()
+    sizes, code, flags = _delta_sizes(q, v, log_gates, offsets)
+    workspace = _delta_workspace(sizes, code, offsets is not None, True, q.device)
+    _launch(q.device, lib.ascan_delta_backward, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_gates.data_ptr(),
+            beta.data_ptr(), states.data_ptr(), updates.data_ptr(), _ptr(offsets), _ptr(d_out), _ptr(d_final),
+            d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_log_gates.data_ptr(), d_beta.data_ptr(),
+            _ptr(d_initial), *sizes, scale, code, flags, workspace.data_ptr(), workspace.numel())
+
+
+def delta_step(q, k, v, log_gates, beta, states, slots, scale, out) -> None:
+    """Enqueue one token of the gated delta rule for a batch, ``states`` updated in place."""
+    lib = _lib or load()
+    batch, key_heads, dk = q.shape
+    heads, dv = v.shape[1:]
+    flags = DELTA_GATES_F32 if log_gates.dtype == torch.float32 else 0
+    if slots is not None and slots.dtype == torch.int64:
+        flags |= DELTA_OFFSETS_I64
+    _launch(q.device, lib.ascan_delta_step, q.data_ptr(), k.data_ptr(), v.data_ptr(), log_gates.data_ptr(),
+            beta.data_ptr(), states.data_ptr(), _ptr(slots), out.data_ptr(), batch, states.shape[0], heads, key_heads,
+            dk, dv, scale, DTYPE_CODES[q.dtype], flags)
+
+
+def gated_norm(x, gate, weight, eps, out) -> None:
+    """Enqueue the gated norm of the rows of ``x``."""
+    lib = _lib or load()
+    width = weight.shape[0]
+    _launch(x.device, lib.ascan_gated_norm, x.data_ptr(), gate.data_ptr(), weight.data_ptr(), out.data_ptr(),
+            x.numel() // width, width, eps, DTYPE_CODES[x.dtype])
+
+
+def gated_norm_backward(x, gate, weight, eps, d_out, d_x, d_gate, d_weight) -> None:
+    """Enqueue the gradients of ``gated_norm``."""
+    lib = _lib or load()
+    width = weight.shape[0]
+    rows = x.numel() // width
+    workspace = torch.empty(lib.ascan_gated_norm_workspace_bytes(rows, width), dtype=torch.uint8, device=x.device)
+    _launch(x.device, lib.ascan_gated_norm_backward, x.data_ptr(), gate.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
+            d_x.data_ptr(), d_gate.data_ptr(), d_weight.data_ptr(), rows, width, eps, DTYPE_CODES[x.dtype],
+            workspace.data_ptr(), workspace.numel())
 
 
 def workspace_timeouts(workspace) -> int:

@@ -15,7 +15,7 @@ under ``torch.compile``.  Every operator validates its arguments itself: they
 are public as ``torch.ops.accelerated_scan.*``.
 """
 
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -285,3 +285,194 @@ def _backward_scan_forward_gated(ctx, grad):
 
 torch.library.register_autograd(
     "accelerated_scan::scan_forward_gated", _backward_scan_forward_gated, setup_context=_setup_scan_forward_gated)
+
+
+# ---------------------------------------------------------------------------
+# Gated delta rule and gated norm (modules ``delta`` and ``norm``).  The ``*_run`` functions choose between the
+# custom operator, while a graph is being captured, and the direct call.
+# ---------------------------------------------------------------------------
+def _delta_outputs(queries, values, initial, offsets, keep):
+    """Empty (out, final, states, updates) of a delta rule call."""
+    batch, tokens, _, key_dim = queries.shape
+    heads, value_dim = values.shape[2:]
+    sequences = batch if offsets is None else offsets.shape[0] - 1
+    blocks = -(-tokens // 64) * batch if offsets is None else batch * tokens // 64 + sequences
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=queries.device)  # noqa: E731
+    final = new(sequences, heads, key_dim, value_dim)
+    if not keep:
+        return torch.empty_like(values), final, new(0), new(0)
+    return torch.empty_like(values), final, new(blocks, heads, key_dim, value_dim), new(batch, tokens, heads, value_dim)
+
+
+def _delta_forward(queries, keys, values, log_gates, beta, initial, offsets, scale, keep):
+    out, final, states, updates = _delta_outputs(queries, values, initial, offsets, keep)
+    if final.shape[0] == 0:
+        out.zero_()  # no sequence: rows outside all of them
+    else:
+        _abi.delta_forward(queries, keys, values, log_gates, beta, initial, offsets, scale, out, final,
+                           states if keep else None, updates if keep else None)
+    return out, final, states, updates
+
+
+@torch.library.custom_op("accelerated_scan::delta_forward", mutates_args=())
+def delta_forward(
+    queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_gates: torch.Tensor, beta: torch.Tensor,
+    initial: Optional[torch.Tensor], offsets: Optional[torch.Tensor], scale: float, keep: bool
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``keep``: also return what ``delta_backward`` needs (else empty tensors)."""
+    from . import delta
+
+    delta._check_scan(queries, keys, values, log_gates, beta, initial, offsets)
+    return _delta_forward(queries, keys, values, log_gates, beta, initial, offsets, scale, keep)
+
+
+@delta_forward.register_fake
+def _(queries, keys, values, log_gates, beta, initial, offsets, scale, keep):
+    return _delta_outputs(queries, values, initial, offsets, keep)
+
+
+def _delta_gradients(queries, keys, values, log_gates, beta, states, started, offsets):
+    """Empty gradients of the inputs; that of the initial states has no elements where there are none."""
+    sequences = queries.shape[0] if offsets is None else offsets.shape[0] - 1
+    shape = (sequences, values.shape[2], queries.shape[3], values.shape[3]) if started else (0,)
+    d_initial = torch.empty(shape, dtype=torch.float32, device=queries.device)
+    return (*(torch.empty_like(t) for t in (queries, keys, values, log_gates, beta)), d_initial)
+
+
+def _delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final, started):
+    grads = _delta_gradients(queries, keys, values, log_gates, beta, states, started, offsets)
+    if offsets is not None and offsets.shape[0] == 1:
+        for g in grads:
+            g.zero_()
+    else:
+        _abi.delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final,
+                            *grads[:5], grads[5] if started else None)
+    return grads
+
+
+@torch.library.custom_op("accelerated_scan::delta_backward", mutates_args=())
+def delta_backward(
+    queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_gates: torch.Tensor, beta: torch.Tensor,
+    states: torch.Tensor, updates: torch.Tensor, offsets: Optional[torch.Tensor], scale: float,
+    d_out: Optional[torch.Tensor], d_final: Optional[torch.Tensor], started: bool
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``started``: the forward pass had initial states, whose gradient is the last result."""
+    from . import delta
+
+    sequences = delta._check_scan(queries, keys, values, log_gates, beta, None, offsets)
+    state = (values.shape[2], queries.shape[3], values.shape[3])
+    blocks = _abi.delta_blocks(queries.shape[0] * queries.shape[1], sequences, offsets is not None)
+    for t, shape, dtype in ((states, (blocks, *state), torch.float32), (updates, values.shape, torch.float32),
+                            (d_out, values.shape, values.dtype), (d_final, (sequences, *state), torch.float32)):
+        if t is not None and (t.shape != shape or t.dtype != dtype or t.device != queries.device or not t.is_contiguous()):
+            raise RuntimeError(f"accelerated_scan: expected a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                               f"{queries.device}, got {t.dtype}, {tuple(t.shape)}")
+    return _delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final, started)
+
+
+@delta_backward.register_fake
+def _(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final, started):
+    return _delta_gradients(queries, keys, values, log_gates, beta, states, started, offsets)
+
+
+def delta_forward_run(*args):
+    return delta_forward(*args) if capturing() else _delta_forward(*args)
+
+
+def delta_backward_run(*args):
+    return delta_backward(*args) if capturing() else _delta_backward(*args)
+
+
+def _setup_delta_forward(ctx, inputs, output):
+    queries, keys, values, log_gates, beta, initial, offsets, scale, keep = inputs
+    if not keep:
+        raise RuntimeError("accelerated_scan: delta_forward is differentiable with keep=True only")
+    _, _, states, updates = output
+    ctx.save_for_backward(queries, keys, values, log_gates, beta, states, updates, offsets)
+    ctx.scale = scale
+    ctx.started = initial is not None
+    ctx.set_materialize_grads(False)
+
+
+def _backward_delta_forward(ctx, d_out, d_final, d_states, d_updates):
+    *inputs, states, updates, offsets = ctx.saved_tensors
+    if d_out is None and d_final is None:
+        return (None,) * 9
+    grads = delta_backward(*inputs, states, updates, offsets, ctx.scale,
+                           d_out.contiguous() if d_out is not None else None,
+                           d_final.contiguous() if d_final is not None else None, ctx.started)
+    return (*grads[:5], grads[5] if ctx.started else None, None, None, None)
+
+
+torch.library.register_autograd(
+    "accelerated_scan::delta_forward", _backward_delta_forward, setup_context=_setup_delta_forward)
+
+
+@torch.library.custom_op("accelerated_scan::delta_step", mutates_args=("states",))
+def delta_step(
+    queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_gates: torch.Tensor, beta: torch.Tensor,
+    states: torch.Tensor, slots: Optional[torch.Tensor], scale: float
+) -> torch.Tensor:
+    from . import delta
+
+    delta._check_step(queries, keys, values, log_gates, beta, states, slots)
+    out = torch.empty_like(values)
+    _abi.delta_step(queries, keys, values, log_gates, beta, states, slots, scale, out)
+    return out
+
+
+@delta_step.register_fake
+def _(queries, keys, values, log_gates, beta, states, slots, scale):
+    return torch.empty_like(values)
+
+
+@torch.library.custom_op("accelerated_scan::gated_norm", mutates_args=())
+def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
+    from . import norm
+
+    norm._check(x, gate, weight)
+    out = torch.empty_like(x)
+    if x.numel():
+        _abi.gated_norm(x, gate, weight, eps, out)
+    return out
+
+
+@gated_norm.register_fake
+def _(x, gate, weight, eps):
+    return torch.empty_like(x)
+
+
+def _gated_norm_backward(x, gate, weight, d_out, eps):
+    d_x, d_gate = torch.empty_like(x), torch.empty_like(gate)
+    if x.numel() == 0:
+        return d_x, d_gate, torch.zeros_like(weight)
+    d_weight = torch.empty_like(weight)
+    _abi.gated_norm_backward(x, gate, weight, eps, d_out, d_x, d_gate, d_weight)
+    return d_x, d_gate, d_weight
+
+
+@torch.library.custom_op("accelerated_scan::gated_norm_backward", mutates_args=())
+def gated_norm_backward(
+    x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, d_out: torch.Tensor, eps: float
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    from . import norm
+
+    norm._check(x, gate, weight)
+    if d_out.shape != x.shape or d_out.dtype != x.dtype or d_out.device != x.device or not d_out.is_contiguous():
+        raise RuntimeError("accelerated_scan: expected d_out to be contiguous, with the shape and dtype of x")
+    return _gated_norm_backward(x, gate, weight, d_out, eps)
+
+
+@gated_norm_backward.register_fake
+def _(x, gate, weight, d_out, eps):
+    return torch.empty_like(x), torch.empty_like(gate), torch.empty_like(weight)
+
+
+def gated_norm_backward_run(*args):
+    return gated_norm_backward(*args) if capturing() else _gated_norm_backward(*args)
+
+
+torch.library.register_autograd(
+    "accelerated_scan::gated_norm",
+    lambda ctx, grad: (*gated_norm_backward(*ctx.saved_tensors, grad.contiguous(), ctx.eps), None),
+    setup_context=lambda ctx, inputs, output: (ctx.save_for_backward(*inputs[:3]), setattr(ctx, "eps", inputs[3]))[0])

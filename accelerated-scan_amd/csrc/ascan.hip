@@ -366,6 +366,9 @@ const char* ascan_status_string(int status) {
         case ASCAN_ERR_OVERLAP: return "an output buffer overlaps an input or another output buffer of the call";
         case ASCAN_ERR_TOO_LARGE:
             return "the split-row table of this problem exceeds the library's static workspace (ASCAN_STATIC_WORKSPACE_BYTES)";
+        case ASCAN_ERR_BAD_HEADS:
+            return "unsupported heads: expecting key heads that divide the heads, a key size up to 128 and a value size up to 4096, multiples of 8";
+        case ASCAN_ERR_WORKSPACE: return "the workspace is smaller than the call's *_workspace_bytes function says";
         default: return "unknown status";
     }
 }

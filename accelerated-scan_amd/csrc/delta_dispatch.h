@@ -1,0 +1,121 @@
+// Launches the gated delta rule kernels for one element type.
+#ifndef ASCAN_DELTA_DISPATCH_H_
+#define ASCAN_DELTA_DISPATCH_H_
+
+#include "ascan.h"
+#include "delta_backward.h"
+#include "delta_step.h"
+#include "dispatch.h"
+
+namespace ascan {
+namespace {
+
+inline int delta_status(hipError_t e) {
+    if (e == hipSuccess) return ASCAN_OK;
+    g_last_hip_error = (int)e;
+    return ASCAN_ERR_LAUNCH;
+}
+
+inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+
+// The workspace's parts: table of the blocks' gates, T, P, and for the backward pass the state gradients
+// behind every block and the rows dR.
+template <int NS>
+struct DeltaParts {
+    size_t gates, t, p, d_states, d_rows, end;
+    DeltaParts(const DeltaShape& s, bool backward) {
+        const size_t entries = (size_t)s.blocks * s.heads;
+        gates = 0;
+        t = round_up(gates + entries * kGateFloats * 4);
+        p = round_up(t + entries * kMatrixBytes<NS>);
+        d_states = round_up(p + entries * kMatrixBytes<NS>);
+        d_rows = round_up(d_states + (backward ? entries * s.dk * s.dv * 4 : 0));
+        end = round_up(d_rows + (backward ? (size_t)s.rows * s.heads * s.dv * 4 : 0));
+    }
+};
+
+template <class... P, class... A>
+hipError_t delta_launch(void (*kernel)(P...), dim3 grid, size_t lds, hipStream_t stream, A... args) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, args...);
+    return hipGetLastError();
+}
+
+template <class E, int NI, int NS, int DK>
+hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void* log_gates, const void* beta,
+                   char* ws, const DeltaParts<NS>& at, bool upper, hipStream_t stream) {
+    using S = typename E::S;
+    return delta_launch(delta_prepare<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.heads),
+                        kPrepareBytes<E, NI, NS, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
+                        log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p, upper);
+}
+
+template <class E, int NI, int NS, int DK>
+int delta_forward_dk(const DeltaForward& f) {
+    using S = typename E::S;
+    const DeltaShape& s = f.shape;
+    const DeltaParts<NS> at(s, false);
+    if (s.blocks > 0) {
+        const hipError_t e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, f.workspace, at, false, f.stream);
+        if (e != hipSuccess) return delta_status(e);
+    }
+    const unsigned groups = (unsigned)((s.dv + kColumns - 1) / kColumns);
+    return delta_status(delta_launch(
+        delta_chain<E, NI, NS, DK>, dim3(groups, (unsigned)s.heads, (unsigned)s.sequences), kChainBytes<NI, DK>, f.stream,
+        s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
+        reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
+        static_cast<S*>(f.out), f.final, f.states, f.updates));
+}
+
+template <class E, int NI, int NS, int DK>
+int delta_backward_dk(const DeltaBackward& f) {
+    using S = typename E::S;
+    const DeltaShape& s = f.shape;
+    const DeltaParts<NS> at(s, true);
+    char* ws = f.workspace;
+    hipError_t e = hipSuccess;
+    if (s.blocks > 0) e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, ws, at, true, f.stream);
+    if (e != hipSuccess) return delta_status(e);
+    const unsigned groups = (unsigned)((s.dv + kColumns - 1) / kColumns);
+    const float* gates = reinterpret_cast<const float*>(ws + at.gates);
+    float* d_states = reinterpret_cast<float*>(ws + at.d_states);
+    float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3(groups, (unsigned)s.heads, (unsigned)s.sequences),
+                     kReverseBytes<NI, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
+                     static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
+                     f.d_initial, d_states, d_rows);
+    if (e != hipSuccess || s.blocks == 0) return delta_status(e);
+    return delta_status(delta_launch(
+        delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), kGradientBytes<NI, NS, DK>,
+        f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
+        static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
+        static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta));
+}
+
+template <class E, int Q, int N>
+int delta_step_rows(const DeltaStep& p) {
+    const int groups = (p.dv + 4 * Q - 1) / (4 * Q);
+    return delta_status(delta_launch(delta_step<E, Q, N>, dim3((unsigned)(p.batch * p.heads * groups)), 0, p.stream, p, groups));
+}
+
+template <class E>
+int delta_step_any(const DeltaStep& p) {
+    return p.dk <= 64 ? delta_step_rows<E, 32, 8>(p) : delta_step_rows<E, 32, 16>(p);
+}
+
+}  // namespace
+
+#define ASCAN_DEFINE_DELTA(suffix, E, NI, NS)                                                                   \
+    namespace ascan {                                                                                           \
+    int delta_forward_##suffix(const DeltaForward& f) {                                                         \
+        return f.shape.dk <= 64 ? delta_forward_dk<E, NI, NS, 64>(f) : delta_forward_dk<E, NI, NS, 128>(f);     \
+    }                                                                                                           \
+    int delta_backward_##suffix(const DeltaBackward& f) {                                                       \
+        return f.shape.dk <= 64 ? delta_backward_dk<E, NI, NS, 64>(f) : delta_backward_dk<E, NI, NS, 128>(f);   \
+    }                                                                                                           \
+    int delta_step_##suffix(const DeltaStep& p) { return delta_step_any<E>(p); }                                \
+    size_t delta_workspace_##suffix(const DeltaShape& s, bool backward) { return DeltaParts<NS>(s, backward).end; } \
+    }
+
+}  // namespace ascan
+
+#endif  // ASCAN_DELTA_DISPATCH_H_

@@ -1,0 +1,281 @@
+// Building blocks of the gated delta rule kernels: blocks of 64 tokens in LDS, operands of the
+// matrix instructions and their products.
+//
+// All products are chains of 16x16 tiles.  The accumulator of a tile holds, in lane l with
+// g = l / 16, column l % 16 and rows 4g .. 4g+3; an operand of a product of depth 32 holds, in lane
+// l, one row (left) or column (right) l % 16 and eight values of the depth axis.  The order of the
+// depth axis is free as long as both operands use the same one, so here lane group g holds depths
+// 4g .. 4g+3 and 16+4g .. 16+4g+3: then the accumulators of two stacked tiles ARE an operand of
+// the next product, and a state, its products and its update stay in the registers of one wave.
+//
+// Arithmetic (parameter P of an operand, its number of parts):
+//   P = 0   fp32 values and fp32 matrix instructions, 256 operations per clock and compute unit;
+//   P >= 1  a value is the sum of P bfloat16 parts (8 bits each: one part holds a bfloat16 value, two a
+//           half value without loss, or an fp32 value to 2^-16, three hold it to 2^-24), products are
+//           summed over the pairs of parts that count, at 4096 operations per clock and pair.
+#ifndef ASCAN_DELTA_TILE_H_
+#define ASCAN_DELTA_TILE_H_
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ascan {
+namespace {
+
+typedef float fx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bx8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 hx4 __attribute__((ext_vector_type(4)));
+typedef short sx4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 64;          // tokens of a block
+constexpr int kTiles = kBlock / 16;
+constexpr int kPairs = 6;           // products of depth 32 in a triangular 64 x 64 matrix of 16 x 16 tiles
+
+template <int P>
+struct Operand {
+    bx8 p[P];
+};
+template <>
+struct Operand<0> {
+    fx4 t[2];
+};
+
+// x as parts: each the rounding (to nearest even) of what the earlier ones leave.
+template <int P>
+__device__ __forceinline__ void set_parts(Operand<P>& o, int e, float x) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const __bf16 h = (__bf16)x;
+        o.p[i][e] = h;
+        x -= (float)h;
+    }
+}
+
+// Two stacked accumulator tiles as an operand.
+template <int P>
+__device__ __forceinline__ Operand<P> operand_of(const fx4& a, const fx4& b) {
+    Operand<P> o;
+    if constexpr (P == 0) {
+        o.t[0] = a;
+        o.t[1] = b;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            set_parts<P>(o, r, a[r]);
+            set_parts<P>(o, r + 4, b[r]);
+        }
+    }
+    return o;
+}
+
+// c + a * b over 32 depths.  Pairs of parts below the last bit kept of the product are left out:
+// part i of a has weight 2^-8i.
+template <int PA, int PB>
+__device__ __forceinline__ fx4 mma(const Operand<PA>& a, const Operand<PB>& b, fx4 c) {
+    if constexpr (PA == 0) {
+        static_assert(PB == 0, "operands of one kind");
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.t[t][r], b.t[t][r], c, 0, 0, 0);
+    } else {
+        constexpr int M = PA > PB ? PA : PB;
+#pragma unroll
+        for (int s = M - 1; s >= 0; --s)
+#pragma unroll
+            for (int i = 0; i < PA; ++i)
+                if (s - i >= 0 && s - i < PB)
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], c, 0, 0, 0);
+    }
+    return c;
+}
+
+// ---------------------------------------------------------------------------
+// Elements in memory
+// ---------------------------------------------------------------------------
+struct ElemF32 {
+    using S = float;
+    static constexpr bool kWide = true;
+    static __device__ __forceinline__ float get(S s) { return s; }
+    static __device__ __forceinline__ S put(float x) { return x; }
+};
+struct ElemBF16 {
+    using S = __bf16;
+    static constexpr bool kWide = false;
+    static __device__ __forceinline__ float get(S s) { return (float)s; }
+    static __device__ __forceinline__ S put(float x) { return (__bf16)x; }
+};
+struct ElemF16 {
+    using S = _Float16;
+    static constexpr bool kWide = false;
+    static __device__ __forceinline__ float get(S s) { return (float)s; }
+    static __device__ __forceinline__ S put(float x) { return (_Float16)x; }
+};
+
+// Eight neighbouring elements, as they travel from memory to LDS (16 or 32 aligned bytes).
+template <class E>
+struct Eight {
+    typename E::S v[8];
+};
+template <class E>
+__device__ __forceinline__ Eight<E> load8(const typename E::S* p, bool there) {
+    Eight<E> r;
+    if (there) {
+        if constexpr (E::kWide) {
+            const fx4 a = *reinterpret_cast<const fx4*>(p), b = *reinterpret_cast<const fx4*>(p + 4);
+            __builtin_memcpy(&r.v[0], &a, 16);
+            __builtin_memcpy(&r.v[4], &b, 16);
+        } else {
+            const fx4 a = *reinterpret_cast<const fx4*>(p);
+            __builtin_memcpy(&r.v[0], &a, 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = E::put(0.0f);
+    }
+    return r;
+}
+
+// Four neighbouring values to memory.
+template <class E>
+__device__ __forceinline__ void store4(typename E::S* p, const fx4& x) {
+    typename E::S s[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = E::put(x[r]);
+    if constexpr (E::kWide) {
+        fx4 v;
+        __builtin_memcpy(&v, s, 16);
+        *reinterpret_cast<fx4*>(p) = v;
+    } else {
+        uint64_t v;
+        __builtin_memcpy(&v, s, 8);
+        *reinterpret_cast<uint64_t*>(p) = v;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 64 rows of W values in LDS, as fp32 (P = 0) or as P planes of bfloat16 parts.  Rows are padded by
+// 16 bytes so that the 16 rows of an operand start in different banks.
+// ---------------------------------------------------------------------------
+template <int P, int W>
+struct Tile {
+    static constexpr int kStride = W + 8;
+    static constexpr int kPlane = kBlock * kStride;
+    static constexpr int kBytes = P * kPlane * 2;
+    __bf16* base;
+
+    __device__ __forceinline__ explicit Tile(void* p) : base(static_cast<__bf16*>(p)) {}
+
+    template <class E>
+    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) {
+        __bf16* at = base + row * kStride + col;
+        if constexpr (P == 1 && sizeof(typename E::S) == 2) {
+            fx4 v;
+            __builtin_memcpy(&v, x.v, 16);
+            *reinterpret_cast<fx4*>(at) = v;
+        } else {
+            Operand<P> o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) set_parts<P>(o, i, E::get(x.v[i]));
+#pragma unroll
+            for (int i = 0; i < P; ++i) *reinterpret_cast<bx8*>(at + i * kPlane) = o.p[i];
+        }
+    }
+    // Depths k0 .. k0+31 of row `row` (lane % 16 chooses the row in the caller).
+    __device__ __forceinline__ Operand<P> along(int row, int k0, int g) const {
+        Operand<P> o;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const __bf16* at = base + i * kPlane + row * kStride + k0 + 4 * g;
+            const bx4 a = *reinterpret_cast<const bx4*>(at), b = *reinterpret_cast<const bx4*>(at + 16);
+            o.p[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return o;
+    }
+    // Rows row0+4g .. +3 of column col0 + lane % 16: the transposing LDS read, whose 16 lanes of a group
+    // fetch four rows of 16 columns and receive a column each.
+    __device__ __forceinline__ bx4 column4(int plane, int row0, int col0, int lane) const {
+        const int g = lane >> 4, i = lane & 15;
+        __bf16* at = base + plane * kPlane + (row0 + 4 * g + (i >> 2)) * kStride + col0 + (i & 3) * 4;
+        const sx4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)at);
+        return __builtin_bit_cast(bx4, v);
+    }
+    // Depths row0 .. row0+31 of column col0 + lane % 16.
+    __device__ __forceinline__ Operand<P> down(int row0, int col0, int lane) const {
+        Operand<P> o;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const bx4 a = column4(i, row0, col0, lane), b = column4(i, row0 + 16, col0, lane);
+            o.p[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return o;
+    }
+    // The 16 x 16 tile at (row0, col0) in the accumulator's layout.
+    __device__ __forceinline__ fx4 tile(int row0, int col0, int lane) const {
+        fx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = P - 1; i >= 0; --i) {
+            const bx4 a = column4(i, row0, col0, lane);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] += (float)a[r];
+        }
+        return x;
+    }
+};
+
+template <int W>
+struct Tile<0, W> {
+    static constexpr int kStride = W + 4;
+    static constexpr int kBytes = kBlock * kStride * 4;
+    float* base;
+
+    __device__ __forceinline__ explicit Tile(void* p) : base(static_cast<float*>(p)) {}
+
+    template <class E>
+    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) {
+        fx4 a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = E::get(x.v[i]);
+            b[i] = E::get(x.v[i + 4]);
+        }
+        float* at = base + row * kStride + col;
+        *reinterpret_cast<fx4*>(at) = a;
+        *reinterpret_cast<fx4*>(at + 4) = b;
+    }
+    __device__ __forceinline__ Operand<0> along(int row, int k0, int g) const {
+        const float* at = base + row * kStride + k0 + 4 * g;
+        Operand<0> o;
+        o.t[0] = *reinterpret_cast<const fx4*>(at);
+        o.t[1] = *reinterpret_cast<const fx4*>(at + 16);
+        return o;
+    }
+    __device__ __forceinline__ fx4 tile(int row0, int col0, int lane) const {
+        const float* at = base + (row0 + 4 * (lane >> 4)) * kStride + col0 + (lane & 15);
+        fx4 x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = at[r * kStride];
+        return x;
+    }
+    __device__ __forceinline__ Operand<0> down(int row0, int col0, int lane) const {
+        Operand<0> o;
+        o.t[0] = tile(row0, col0, lane);
+        o.t[1] = tile(row0 + 16, col0, lane);
+        return o;
+    }
+};
+
+// Sum over the 16 lanes that share lane / 16.
+__device__ __forceinline__ float sum16(float x) {
+    x += __shfl_xor(x, 1);
+    x += __shfl_xor(x, 2);
+    x += __shfl_xor(x, 4);
+    x += __shfl_xor(x, 8);
+    return x;
+}
+
+}  // namespace
+}  // namespace ascan
+
+#endif  // ASCAN_DELTA_TILE_H_

@@ -72,7 +72,7 @@
 extern "C" {
 #endif
 
-#define ASCAN_ABI_VERSION 10
+#define ASCAN_ABI_VERSION 11
 
 /* Marks the exported entry points (the library is built with hidden visibility). */
 #define ASCAN_API __attribute__((visibility("default")))
@@ -103,7 +103,9 @@ enum ascan_status {
     ASCAN_ERR_LAUNCH        = 5, /* the HIP runtime refused the launch (see ascan_last_hip_error) */
     ASCAN_ERR_BAD_ACTIVATION = 6, /* gate is not an ascan_gate, or not available for this dtype */
     ASCAN_ERR_OVERLAP       = 7, /* an output buffer overlaps an input or another output of the call */
-    ASCAN_ERR_TOO_LARGE     = 8  /* ascan_forward_split_static: the table would not fit the static workspace */
+    ASCAN_ERR_TOO_LARGE     = 8, /* ascan_forward_split_static: the table would not fit the static workspace */
+    ASCAN_ERR_BAD_HEADS     = 9, /* ascan_delta_*: head counts or sizes that the kernels do not take */
+    ASCAN_ERR_WORKSPACE     = 10 /* ascan_delta_*, ascan_gated_norm_backward: the workspace is too small */
 };
 
 /* What the kernels make of the stored gate values (the *_gated entry points). */
@@ -385,6 +387,86 @@ ASCAN_API int ascan_backward_gated_values(const void* gate_inputs, const void* v
                                 const void* initial, const void* grad_out, void* d_gate_inputs, void* d_values,
                                 void* d_initial, int64_t rows, int64_t seqlen, int dtype, int gate,
                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gated delta rule: the recurrence of a matrix state per head,
+ *
+ *     S[t]   = a[t] S[t-1] + beta[t] k[t] (v[t] - (a[t] S[t-1])^T k[t])^T,   a[t] = exp(log_gate[t])
+ *     out[t] = scale S[t]^T q[t]
+ *
+ * on dense tensors with the features innermost: q and k (rows, key_heads, dk), v and out (rows, heads, dv),
+ * log_gates and beta (rows, heads), states fp32 (.., heads, dk, dv).  A row is a token; value head h uses key
+ * head h / (heads / key_heads).  dk is a multiple of 8 up to 128, dv a multiple of 8 up to 4096.  dtype is
+ * ASCAN_F32, ASCAN_BF16 or ASCAN_F16 and holds for q, k, v, out and their gradients; log_gates, beta and their
+ * gradients have it too, or are fp32 with ASCAN_DELTA_GATES_F32.  All buffers start on 16 bytes, except the gates.
+ *
+ *   - `sequences` sequences of rows / sequences tokens each where `offsets` is NULL; else packed ones, sequence n
+ *     being rows offsets[n] .. offsets[n+1]-1 (device memory, sequences + 1 ascending numbers; int32, or int64 with
+ *     ASCAN_DELTA_OFFSETS_I64).  Sequences may be empty: their final state is the initial one.  Outputs and
+ *     gradients of rows outside all sequences are zero.  A table that does not ascend gives unspecified values, and
+ *     no access outside the buffers;
+ *   - initial (or NULL for zeros) and final (or NULL) hold one state per sequence;
+ *   - states (ascan_delta_blocks() x heads x dk x dv) and updates (rows x heads x dv) are what the backward pass
+ *     needs of the forward pass; NULL where there will be none;
+ *   - d_out and d_final may be NULL (zeros), d_initial may be NULL (not wanted);
+ *   - the workspace has the size that ascan_delta_workspace_bytes gives, and belongs to the call until it has run.
+ *     Its contents on entry do not matter;
+ *   - a log gate below -1000, -inf among them, is a gate of zero: the state starts anew there;
+ *   - tokens are taken in blocks of 64 from the start of each sequence: a NaN or an infinity in a token can reach
+ *     the outputs of earlier tokens of its block, never those of earlier blocks or of other sequences.
+ *
+ * ascan_delta_step advances the states of `batch` conversations by one token (q and k (batch, key_heads, dk), ...) in
+ * place.  Row b uses states[slots[b]] (slots: int32, or int64 with ASCAN_DELTA_OFFSETS_I64), states[b] where slots is
+ * NULL.  Rows that name the same slot are consecutive tokens of it, in the order of the rows.  A slot outside
+ * 0 .. state_count-1 marks a row without a state: its output is zero.
+ */
+enum ascan_delta_flags {
+    ASCAN_DELTA_GATES_F32   = 1, /* log_gates, beta, d_log_gates and d_beta are fp32 whatever dtype says */
+    ASCAN_DELTA_OFFSETS_I64 = 2  /* offsets / slots are int64 */
+};
+
+/* Blocks of 64 tokens that the sequences of a call can have; -1 for sizes that a call would refuse. */
+ASCAN_API int64_t ascan_delta_blocks(int64_t rows, int64_t sequences, int packed);
+
+/* Workspace of a call (backward: of ascan_delta_backward); 0 also for sizes that a call would refuse. */
+ASCAN_API size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t dk, int64_t dv,
+                                             int dtype, int packed, int backward);
+
+ASCAN_API int ascan_delta_forward(const void* q, const void* k, const void* v, const void* log_gates, const void* beta,
+                                  const float* initial, const void* offsets, void* out, float* final, float* states,
+                                  float* updates, int64_t rows, int64_t sequences, int64_t heads, int64_t key_heads,
+                                  int64_t dk, int64_t dv, float scale, int dtype, int flags, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+ASCAN_API int ascan_delta_backward(const void* q, const void* k, const void* v, const void* log_gates, const void* beta,
+                                   const float* states, const float* updates, const void* offsets, const void* d_out,
+                                   const float* d_final, void* d_q, void* d_k, void* d_v, void* d_log_gates,
+                                   void* d_beta, float* d_initial, int64_t rows, int64_t sequences, int64_t heads,
+                                   int64_t key_heads, int64_t dk, int64_t dv, float scale, int dtype, int flags,
+                                   void* workspace, size_t workspace_bytes, void* stream);
+
+ASCAN_API int ascan_delta_step(const void* q, const void* k, const void* v, const void* log_gates, const void* beta,
+                               float* states, const void* slots, void* out, int64_t batch, int64_t state_count,
+                               int64_t heads, int64_t key_heads, int64_t dk, int64_t dv, float scale, int dtype,
+                               int flags, void* stream);
+
+/*
+ * Gated norm, the norm behind a delta rule layer: every row of a dense (rows, width) matrix becomes
+ *
+ *     out = weight * x / sqrt(mean(x^2) + eps) * gate / (1 + exp(-gate))
+ *
+ * with weight (width); one dtype (ASCAN_F32, ASCAN_BF16, ASCAN_F16) for all tensors.  The backward pass reads x,
+ * gate, weight and the gradient of out and writes the gradients of all three; d_weight is summed in an order that
+ * the sizes fix.
+ */
+ASCAN_API int ascan_gated_norm(const void* x, const void* gate, const void* weight, void* out, int64_t rows,
+                               int64_t width, float eps, int dtype, void* stream);
+
+ASCAN_API size_t ascan_gated_norm_workspace_bytes(int64_t rows, int64_t width);
+
+ASCAN_API int ascan_gated_norm_backward(const void* x, const void* gate, const void* weight, const void* d_out,
+                                        void* d_x, void* d_gate, void* d_weight, int64_t rows, int64_t width, float eps,
+                                        int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Static, human-readable text for an ascan_status code. */
 ASCAN_API const char* ascan_status_string(int status);
