@@ -18,6 +18,8 @@
 namespace ascan {
 namespace {
 
+constexpr int kColumns = 64;  // value columns that a workgroup takes at a time
+
 template <int NI, int DK>
 constexpr int kReverseBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, kColumns>::kBytes;
 

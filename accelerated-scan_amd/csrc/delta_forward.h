@@ -1,4 +1,11 @@
 // Forward pass of the gated delta rule: the chain over the blocks of a sequence (delta.h).
+//
+// The blocks of a sequence follow each other, so what counts is the time from a state to the next: a chain of
+// three products (K S0, T R, K^T U) that are too small to fill a wave's matrix unit for long.  A workgroup
+// of four waves therefore takes only 16 columns of one head's state and divides the rows: wave w keeps
+// state rows dk/4 w .. in its accumulators and computes tokens 16w .. 16w+15 of every block.  State, R and U
+// go round through LDS in the order in which the next product reads them, with one barrier each; everything
+// that comes from memory is requested one block ahead.
 #ifndef ASCAN_DELTA_FORWARD_H_
 #define ASCAN_DELTA_FORWARD_H_
 
@@ -7,14 +14,25 @@
 namespace ascan {
 namespace {
 
-constexpr int kColumns = 64;  // state columns of a workgroup: 16 to a wave
+// Where workgroup `id` of a chain kernel works.  Workgroups go round the eight dies one by one: the column
+// groups of a head, which read the same keys, queries and matrices, are put eight apart, behind one cache.
+struct ChainAt {
+    int64_t sequence;
+    int head, col0;
+    bool there;
+};
+__device__ __forceinline__ ChainAt chain_at(const DeltaShape& s) {
+    const int64_t groups = (s.dv + 15) / 16, id = blockIdx.x;
+    const int64_t unit = id / (8 * groups) * 8 + id % 8;
+    return ChainAt{unit / s.heads, (int)(unit % s.heads), (int)(id / 8 % groups) * 16, unit < s.sequences * s.heads};
+}
+inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads + 7) / 8 * 8 * ((s.dv + 15) / 16); }
 
-template <int NI, int DK>
-constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, kColumns>::kBytes;
+template <int NI, int NS, int DK>
+constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
+                            3 * Exchange<NS, 2>::kBytes;
 
-// A wave keeps 16 columns of the state in its accumulators from the first block to the last; keys, queries
-// and values of a block are shared by the workgroup's waves through LDS.
-// grid (column groups, heads, sequences), 256 threads.
+// grid chain_grid(), 256 threads.
 template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
@@ -23,141 +41,184 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
                                                    const char* __restrict__ p_in, const float* __restrict__ initial,
                                                    typename E::S* __restrict__ out, float* __restrict__ final,
                                                    float* __restrict__ states, float* __restrict__ updates) {
+    using ES = typename E::S;
+    constexpr int kDepths = DK / 32, kOwn = DK / 64, kCopies = DK / 32;  // operands of a row, state tiles of a wave, loads of a thread
     extern __shared__ __align__(16) char smem[];
-    __shared__ __align__(16) float gate[4 * kBlock];
-    const int64_t n = blockIdx.z;
-    const int head = blockIdx.y, key_head = head / (s.heads / s.key_heads);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int col0 = blockIdx.x * kColumns, col = col0 + 16 * wave + c;
+    const ChainAt where = chain_at(s);
+    if (!where.there) return;
+    const int64_t n = where.sequence;
+    const int head = where.head, key_head = head / (s.heads / s.key_heads);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int col0 = where.col0, col = col0 + c;
     const bool mine = col < s.dv;
     const SequenceAt at = sequence_at(s, n);
 
-    Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
-    Tile<NI, kColumns> vt(smem + 2 * Tile<NI, DK>::kBytes);
+    char* m = smem;
+    Tile<NI, DK> kt[2] = {Tile<NI, DK>(m), Tile<NI, DK>(m + Tile<NI, DK>::kBytes)};
+    m += 2 * Tile<NI, DK>::kBytes;
+    Tile<NI, 16> vt(m);
+    m += Tile<NI, 16>::kBytes;
+    Exchange<NS, kDepths> xs(m);
+    m += Exchange<NS, kDepths>::kBytes;
+    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes), xd(m + 2 * Exchange<NS, 2>::kBytes);
 
-    fx4 S[DK / 16];
-    const int64_t state_at = (n * s.heads + head) * s.dk * s.dv;
+    fx4 S[kOwn];
+    const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t)
+    for (int t = 0; t < kOwn; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * t + 4 * g + r;
-            S[t][r] = initial != nullptr && mine && row < s.dk ? initial[state_at + (int64_t)row * s.dv + col] : 0.0f;
+            const int row = 16 * (kOwn * wave + t) + 4 * g + r;
+            S[t][r] = initial != nullptr && mine && row < s.dk ? initial[state_at + (int64_t)row * s.dv] : 0.0f;
         }
 
-    for (int64_t first = 0; first < at.length; first += kBlock) {
-        const int64_t row0 = at.row + first, block = at.block + first / kBlock;
+    // what comes from memory for the block at `first`
+    Eight<E> k_raw[kCopies], v_raw, q_raw[kDepths];
+    Operand<NS> tm[2], pm[2];
+    fx4 beta, beta_since, until;
+    float since, whole;
+    const int token = 16 * wave + c;
+    const auto load_kv = [&](int64_t first) {
+        const int64_t row0 = at.row + first, left = at.length - first;
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
+            k_raw[i] = load8<E>(k + ((row0 + row) * s.key_heads + key_head) * s.dk + d, row < left && d < s.dk);
+        }
+        const int row = tid >> 1, d = col0 + (tid & 1) * 8;
+        v_raw = load8<E>(v + ((row0 + row) * s.heads + head) * s.dv + d, tid < 128 && row < left && d < s.dv);
+    };
+    const auto load_q = [&](int64_t first) {
+        const ES* from = q + ((at.row + first + token) * s.key_heads + key_head) * s.dk;
+#pragma unroll
+        for (int d = 0; d < kDepths; ++d) q_raw[d] = load_depths<E>(from, 32 * d, g, s.dk, token < at.length - first);
+    };
+    const auto entry_of = [&](int64_t first) { return (at.block + first / kBlock) * s.heads + head; };
+    const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
+        const char* mat = from + entry_of(first) * kMatrixBytes<NS>;
+        o[0] = matrix_operand<NS>(mat, pair_lower(wave, 0), lane);
+        if (wave >= 2) o[1] = matrix_operand<NS>(mat, pair_lower(wave, 1), lane);
+    };
+    const auto gate_row = [&](int64_t first, int row) { return gates + entry_of(first) * kGateFloats + row * kBlock; };
+
+    int64_t next = 0;
+    if (at.length > 0) {
+        load_kv(0);
+        load_q(0);
+        beta = *reinterpret_cast<const fx4*>(gate_row(0, kBeta) + 16 * wave + 4 * g);
+        beta_since = *reinterpret_cast<const fx4*>(gate_row(0, kBetaSince) + 16 * wave + 4 * g);
+        load_matrix(t_in, 0, tm);
+        until = *reinterpret_cast<const fx4*>(gate_row(0, kUntil) + 16 * wave + 4 * g);
+        load_matrix(p_in, 0, pm);
+        since = gate_row(0, kSince)[token];
+        whole = gate_row(0, kSince)[kBlock - 1];
+    }
+    for (int64_t first = 0; first < at.length; first = next) {
+        next = first + kBlock;
+        const int64_t ahead = next < at.length ? next : first;
+        const int64_t row0 = at.row + first;
         const int length = (int)(at.length - first < kBlock ? at.length - first : kBlock);
-        const int64_t entry = block * s.heads + head;
-        __syncthreads();
-        for (int i = tid; i < kBlock * DK / 8; i += 256) {
-            const int row = i / (DK / 8), d = i % (DK / 8) * 8;
-            const bool there = row < length && d < s.dk;
-            const int64_t from = ((row0 + row) * s.key_heads + key_head) * s.dk + d;
-            kt.template put8<E>(row, d, load8<E>(k + from, there));
-            qt.template put8<E>(row, d, load8<E>(q + from, there));
-        }
-        for (int i = tid; i < kBlock * kColumns / 8; i += 256) {
-            const int row = i / (kColumns / 8), d = i % (kColumns / 8) * 8;
-            const bool there = row < length && col0 + d < s.dv;
-            vt.template put8<E>(row, d, load8<E>(v + ((row0 + row) * s.heads + head) * s.dv + col0 + d, there));
-        }
-        gate[tid] = gates[entry * kGateFloats + tid];  // the first four rows of the table
-        __syncthreads();
-        const float whole = gate[kSince * kBlock + kBlock - 1];
-        const char* tm = t_in + entry * kMatrixBytes<NS>;
-        const char* pm = p_in + entry * kMatrixBytes<NS>;
+        Tile<NI, DK>& kb = kt[(first / kBlock) & 1];
 
         if (states != nullptr && mine) {
-            float* to = states + entry * s.dk * s.dv + col;
+            float* to = states + entry_of(first) * s.dk * s.dv + col;
 #pragma unroll
-            for (int t = 0; t < DK / 16; ++t)
+            for (int t = 0; t < kOwn; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * t + 4 * g + r < s.dk) to[(int64_t)(16 * t + 4 * g + r) * s.dv] = S[t][r];
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * (kOwn * wave + t) + 4 * g + r;
+                    if (row < s.dk) to[(int64_t)row * s.dv] = S[t][r];
+                }
         }
+#pragma unroll
+        for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, S[t]);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[i]);
+        if (tid < 128) vt.template put8<E>(tid >> 1, (tid & 1) * 8, v_raw);
+        lds_barrier();
+        load_kv(ahead);
 
         // K S0 (rows: tokens, columns: state columns) and (Q S0)^T (rows: state columns, columns: tokens)
-        fx4 u[kTiles], o[kTiles];
+        fx4 u = {0, 0, 0, 0}, o = {0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < kTiles; ++m) u[m] = o[m] = fx4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < DK / 32; ++d) {
-            const Operand<NS> so = operand_of<NS>(S[2 * d], S[2 * d + 1]);
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                u[m] = mma<NI, NS>(kt.along(16 * m + c, 32 * d, g), so, u[m]);
-                o[m] = mma<NS, NI>(so, qt.along(16 * m + c, 32 * d, g), o[m]);
-            }
+        for (int d = 0; d < kDepths; ++d) {
+            const Operand<NS> so = xs.get(d, lane);
+            u = mma<NI, NS>(kb.along(token, 32 * d, g), so, u);
+            o = mma<NS, NI>(so, operand_from<NI, E>(q_raw[d]), o);
         }
-        // R = diag(beta) V - diag(beta e^c) K S0, U = R + T R
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-            const fx4 b = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * m + 4 * g);
-            const fx4 bs = *reinterpret_cast<const fx4*>(gate + kBetaSince * kBlock + 16 * m + 4 * g);
-            const fx4 x = vt.tile(16 * m, 16 * wave, lane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) u[m][r] = b[r] * x[r] - bs[r] * u[m][r];
-        }
+        load_q(ahead);
+        // R = diag(beta) V - diag(beta e^c) K S0
         {
-            const Operand<NS> low = operand_of<NS>(u[0], u[1]), high = operand_of<NS>(u[2], u[3]);
+            const fx4 x = vt.tile(16 * wave, 0, lane);
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                u[m] = mma<NS, NS>(matrix_operand<NS>(tm, pair_lower(m, 0), lane), low, u[m]);
-                if (m >= 2) u[m] = mma<NS, NS>(matrix_operand<NS>(tm, pair_lower(m, 1), lane), high, u[m]);
+            for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * u[r];
+        }
+        beta = *reinterpret_cast<const fx4*>(gate_row(ahead, kBeta) + 16 * wave + 4 * g);
+        beta_since = *reinterpret_cast<const fx4*>(gate_row(ahead, kBetaSince) + 16 * wave + 4 * g);
+        xr.put(wave, lane, u);
+        lds_barrier();
+
+        // U = R + T R
+        u = mma<NS, NS>(tm[0], xr.get(0, lane), u);
+        if (wave >= 2) u = mma<NS, NS>(tm[1], xr.get(1, lane), u);
+        load_matrix(t_in, ahead, tm);
+        xu.put(wave, lane, u);
+        {
+            fx4 x;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = until[r] * u[r];
+            xd.put(wave, lane, x);
+        }
+        until = *reinterpret_cast<const fx4*>(gate_row(ahead, kUntil) + 16 * wave + 4 * g);
+        lds_barrier();
+
+        // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
+        {
+            const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) S[t][r] *= whole;
+                S[t] = mma<NI, NS>(kb.down(0, 16 * (kOwn * wave + t), lane), low, S[t]);
+                S[t] = mma<NI, NS>(kb.down(32, 16 * (kOwn * wave + t), lane), high, S[t]);
             }
         }
         // out^T = scale (Q S0)^T diag(e^c) + U^T P^T
         {
-            const Operand<NS> low = operand_of<NS>(u[0], u[1]), high = operand_of<NS>(u[2], u[3]);
+            const float f = s.scale * since;
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                const float f = s.scale * gate[kSince * kBlock + 16 * m + c];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[m][r] *= f;
-                o[m] = mma<NS, NS>(low, matrix_operand<NS>(pm, pair_lower(m, 0), lane), o[m]);
-                if (m >= 2) o[m] = mma<NS, NS>(high, matrix_operand<NS>(pm, pair_lower(m, 1), lane), o[m]);
-                const int row = 16 * m + c, d = col0 + 16 * wave + 4 * g;
-                if (row < length && d < s.dv) store4<E>(out + ((row0 + row) * s.heads + head) * s.dv + d, o[m]);
-            }
+            for (int r = 0; r < 4; ++r) o[r] *= f;
+            o = mma<NS, NS>(xu.get(0, lane), pm[0], o);
+            if (wave >= 2) o = mma<NS, NS>(xu.get(1, lane), pm[1], o);
+            const int d = col0 + 4 * g;
+            if (token < length && d < s.dv) store4<E>(out + ((row0 + token) * s.heads + head) * s.dv + d, o);
         }
+        load_matrix(p_in, ahead, pm);
+        since = gate_row(ahead, kSince)[token];
+        whole = gate_row(ahead, kSince)[kBlock - 1];
         if (updates != nullptr && mine) {
-            float* to = updates + (row0 * s.heads + head) * s.dv + col;
+            float* to = updates + ((row0 + 16 * wave + 4 * g) * s.heads + head) * s.dv + col;
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (16 * m + 4 * g + r < length) to[(int64_t)(16 * m + 4 * g + r) * s.heads * s.dv] = u[m][r];
-        }
-        // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-            const fx4 f = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * m + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) u[m][r] *= f[r];
-        }
-        const Operand<NS> low = operand_of<NS>(u[0], u[1]), high = operand_of<NS>(u[2], u[3]);
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) S[t][r] *= whole;
-            S[t] = mma<NI, NS>(kt.down(0, 16 * t, lane), low, S[t]);
-            S[t] = mma<NI, NS>(kt.down(32, 16 * t, lane), high, S[t]);
+            for (int r = 0; r < 4; ++r)
+                if (16 * wave + 4 * g + r < length) to[(int64_t)r * s.heads * s.dv] = u[r];
         }
     }
     if (final != nullptr && mine) {
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t)
+        for (int t = 0; t < kOwn; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (16 * t + 4 * g + r < s.dk) final[state_at + (int64_t)(16 * t + 4 * g + r) * s.dv + col] = S[t][r];
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * (kOwn * wave + t) + 4 * g + r;
+                if (row < s.dk) final[state_at + (int64_t)row * s.dv] = S[t][r];
+            }
     }
     // rows in front of the first and behind the last sequence are zero
     if (s.offsets != nullptr && mine) {
+        const int own = 4 * wave + g;
         if (n == 0)
-            for (int64_t row = g; row < offset_at(s, 0); row += 4) out[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
+            for (int64_t row = own; row < offset_at(s, 0); row += 16) out[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
         if (n == s.sequences - 1)
-            for (int64_t row = offset_at(s, s.sequences) + g; row < s.rows; row += 4)
+            for (int64_t row = offset_at(s, s.sequences) + own; row < s.rows; row += 16)
                 out[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
     }
 }

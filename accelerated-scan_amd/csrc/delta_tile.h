@@ -137,6 +137,43 @@ __device__ __forceinline__ Eight<E> load8(const typename E::S* p, bool there) {
     return r;
 }
 
+// Depths k0 .. k0+31 of a row in memory, as they travel: eight elements of a lane.
+template <class E>
+__device__ __forceinline__ Eight<E> load_depths(const typename E::S* p, int k0, int g, int width, bool there) {
+    Eight<E> r;
+    constexpr int kBytes = 4 * sizeof(typename E::S);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int d = k0 + 16 * h + 4 * g;
+        if (there && d < width) {
+            __builtin_memcpy(&r.v[4 * h], __builtin_assume_aligned(p + d, kBytes), kBytes);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.v[4 * h + i] = E::put(0.0f);
+        }
+    }
+    return r;
+}
+
+template <int P, class E>
+__device__ __forceinline__ Operand<P> operand_from(const Eight<E>& x) {
+    Operand<P> o;
+    if constexpr (P == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o.t[0][i] = E::get(x.v[i]);
+            o.t[1][i] = E::get(x.v[i + 4]);
+        }
+    } else if constexpr (P == 1) {
+        static_assert(sizeof(typename E::S) == 2, "one part holds a bfloat16 value");
+        __builtin_memcpy(&o.p[0], x.v, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) set_parts<P>(o, i, E::get(x.v[i]));
+    }
+    return o;
+}
+
 // Four neighbouring values to memory.
 template <class E>
 __device__ __forceinline__ void store4(typename E::S* p, const fx4& x) {
@@ -265,6 +302,48 @@ struct Tile<0, W> {
         return o;
     }
 };
+
+// Accumulator tiles that the waves of a workgroup hand to each other as operands: N operands of two stacked tiles.
+template <int P, int N>
+struct Exchange {
+    static constexpr int kBytes = (P == 0 ? 2 : P) * N * 64 * 16;
+    char* base;
+
+    __device__ __forceinline__ explicit Exchange(char* p) : base(p) {}
+
+    __device__ __forceinline__ void put(int tile, int lane, const fx4& x) {
+        if constexpr (P == 0) {
+            *reinterpret_cast<fx4*>(base + (tile * 64 + lane) * 16) = x;
+        } else {
+            Operand<P> o;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) set_parts<P>(o, r, x[r]);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+                *reinterpret_cast<bx4*>(base + ((i * N + (tile >> 1)) * 64 + lane) * 16 + (tile & 1) * 8) =
+                    __builtin_shufflevector(o.p[i], o.p[i], 0, 1, 2, 3);
+        }
+    }
+    __device__ __forceinline__ Operand<P> get(int n, int lane) const {
+        Operand<P> o;
+        if constexpr (P == 0) {
+            o.t[0] = *reinterpret_cast<const fx4*>(base + (2 * n * 64 + lane) * 16);
+            o.t[1] = *reinterpret_cast<const fx4*>(base + ((2 * n + 1) * 64 + lane) * 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) o.p[i] = *reinterpret_cast<const bx8*>(base + ((i * N + n) * 64 + lane) * 16);
+        }
+        return o;
+    }
+};
+
+// Workgroup barrier for data in LDS: loads from memory stay in flight across it, which __syncthreads() does not
+// promise.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 // Sum over the 16 lanes that share lane / 16.
 __device__ __forceinline__ float sum16(float x) {
