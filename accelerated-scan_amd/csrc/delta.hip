@@ -11,10 +11,12 @@ int element_bytes(int dtype) { return dtype == ASCAN_F32 ? 4 : (dtype == ASCAN_B
 
 constexpr int64_t kMaxHeads = 65535, kMaxRows = INT64_C(1) << 40, kMaxSequences = 65535;
 constexpr int64_t kMaxKeyDim = 128, kMaxValueDim = 4096;
+constexpr int64_t kMaxRowElements = INT64_C(1) << 22;  // of a token: 64 tokens stay below 2^31 bytes
 
 bool heads_ok(int64_t heads, int64_t key_heads, int64_t dk, int64_t dv) {
     return heads > 0 && heads <= kMaxHeads && key_heads > 0 && heads % key_heads == 0 && dk > 0 && dk <= kMaxKeyDim &&
-           dk % 8 == 0 && dv > 0 && dv <= kMaxValueDim && dv % 8 == 0;
+           dk % 8 == 0 && dv > 0 && dv <= kMaxValueDim && dv % 8 == 0 &&
+           heads * dv <= kMaxRowElements && key_heads * dk <= kMaxRowElements;
 }
 
 bool rows_ok(int64_t rows, int64_t sequences, bool packed) {

@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
         gate[tid] = gates[entry * kGateFloats + tid];
         __syncthreads();
         const float whole = gate[kSince * kBlock + kBlock - 1];
-        const char* tm = t_in + entry * kMatrixBytes<NS>;
-        const char* pm = p_in + entry * kMatrixBytes<NS>;
+        const Buffer tm = buffer_of(t_in + entry * kMatrixBytes<NS>, kMatrixBytes<NS>);
+        const Buffer pm = buffer_of(p_in + entry * kMatrixBytes<NS>, kMatrixBytes<NS>);
 
         if (mine) {
             float* to = d_states + entry * s.dk * s.dv + col;

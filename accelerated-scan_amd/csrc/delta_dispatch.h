@@ -58,8 +58,9 @@ int delta_forward_dk(const DeltaForward& f) {
         const hipError_t e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, f.workspace, at, false, f.stream);
         if (e != hipSuccess) return delta_status(e);
     }
+    const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, DK, true> : delta_chain<E, NI, NS, DK, false>;
     return delta_status(delta_launch(
-        delta_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), kChainBytes<NI, NS, DK>, f.stream,
+        chain, dim3((unsigned)chain_grid(s)), kChainBytes<NI, NS, DK>, f.stream,
         s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
         static_cast<S*>(f.out), f.final, f.states, f.updates));

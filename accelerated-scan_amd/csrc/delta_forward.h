@@ -32,8 +32,8 @@ template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
                             3 * Exchange<NS, 2>::kBytes;
 
-// grid chain_grid(), 256 threads.
-template <class E, int NI, int NS, int DK>
+// grid chain_grid(), 256 threads.  KEEP: write the states in front of the blocks and the rows U.
+template <class E, int NI, int NS, int DK, bool KEEP>
 __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
                                                    const typename E::S* __restrict__ v,
@@ -54,7 +54,6 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
     const SequenceAt at = sequence_at(s, n);
 
     char* m = smem;
-    Tile<NI, DK> kt[2] = {Tile<NI, DK>(m), Tile<NI, DK>(m + Tile<NI, DK>::kBytes)};
     m += 2 * Tile<NI, DK>::kBytes;
     Tile<NI, 16> vt(m);
     m += Tile<NI, 16>::kBytes;
@@ -72,63 +71,70 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
             S[t][r] = initial != nullptr && mine && row < s.dk ? initial[state_at + (int64_t)row * s.dv] : 0.0f;
         }
 
+    constexpr uint32_t kSize = sizeof(ES);
+    const uint32_t k_step = s.key_heads * s.dk * kSize, v_step = s.heads * s.dv * kSize;
+    const int64_t seq_row = uniform(at.row), seq_length = uniform(at.length), seq_block = uniform(at.block);
+    const int token = 16 * wave + c;
+
     // what comes from memory for the block at `first`
     Eight<E> k_raw[kCopies], v_raw, q_raw[kDepths];
     Operand<NS> tm[2], pm[2];
     fx4 beta, beta_since, until;
     float since, whole;
-    const int token = 16 * wave + c;
+    const auto rows_of = [&](const void* p, int64_t first, uint32_t step, int64_t at_head, uint32_t bytes) {
+        const int64_t left = seq_length - first < kBlock ? seq_length - first : kBlock;
+        return buffer_of(static_cast<const char*>(p) + (seq_row + first) * step + at_head, (left - 1) * (int64_t)step + bytes);
+    };
+    const auto entry_of = [&](int64_t first) { return (seq_block + first / kBlock) * s.heads + head; };
     const auto load_kv = [&](int64_t first) {
-        const int64_t row0 = at.row + first, left = at.length - first;
+        const Buffer kb = rows_of(k, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const Buffer vb = rows_of(v, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
             const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
-            k_raw[i] = load8<E>(k + ((row0 + row) * s.key_heads + key_head) * s.dk + d, row < left && d < s.dk);
+            k_raw[i] = fetch8<E>(kb, d < s.dk ? row * k_step + d * kSize : kOutside);
         }
-        const int row = tid >> 1, d = col0 + (tid & 1) * 8;
-        v_raw = load8<E>(v + ((row0 + row) * s.heads + head) * s.dv + d, tid < 128 && row < left && d < s.dv);
+        const int d = col0 + (tid & 1) * 8;
+        v_raw = fetch8<E>(vb, tid < 128 && d < s.dv ? (tid >> 1) * v_step + d * kSize : kOutside);
     };
     const auto load_q = [&](int64_t first) {
-        const ES* from = q + ((at.row + first + token) * s.key_heads + key_head) * s.dk;
+        const Buffer b = rows_of(q, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
 #pragma unroll
-        for (int d = 0; d < kDepths; ++d) q_raw[d] = load_depths<E>(from, 32 * d, g, s.dk, token < at.length - first);
+        for (int d = 0; d < kDepths; ++d) q_raw[d] = fetch_depths<E>(b, token * k_step, 32 * d, g, s.dk);
     };
-    const auto entry_of = [&](int64_t first) { return (at.block + first / kBlock) * s.heads + head; };
+    // (waves 0 and 1 have one operand to a row of tiles: their second load repeats the first)
     const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
-        const char* mat = from + entry_of(first) * kMatrixBytes<NS>;
-        o[0] = matrix_operand<NS>(mat, pair_lower(wave, 0), lane);
-        if (wave >= 2) o[1] = matrix_operand<NS>(mat, pair_lower(wave, 1), lane);
+        const Buffer b = buffer_of(from + entry_of(first) * kMatrixBytes<NS>, kMatrixBytes<NS>);
+        o[0] = matrix_operand<NS>(b, pair_lower(wave, 0), lane);
+        o[1] = matrix_operand<NS>(b, pair_lower(wave, wave >= 2 ? 1 : 0), lane);
     };
-    const auto gate_row = [&](int64_t first, int row) { return gates + entry_of(first) * kGateFloats + row * kBlock; };
+    const auto gates_of = [&](int64_t first) { return buffer_of(gates + entry_of(first) * kGateFloats, kGateFloats * 4); };
+    const uint32_t gate_rows = (16 * wave + 4 * g) * 4;
 
-    int64_t next = 0;
-    if (at.length > 0) {
+    if (seq_length > 0) {  // (an empty sequence has no table entry to read)
         load_kv(0);
         load_q(0);
-        beta = *reinterpret_cast<const fx4*>(gate_row(0, kBeta) + 16 * wave + 4 * g);
-        beta_since = *reinterpret_cast<const fx4*>(gate_row(0, kBetaSince) + 16 * wave + 4 * g);
+        const Buffer b = gates_of(0);
+        beta = fetch16(b, kBeta * 256 + gate_rows);
+        beta_since = fetch16(b, kBetaSince * 256 + gate_rows);
         load_matrix(t_in, 0, tm);
-        until = *reinterpret_cast<const fx4*>(gate_row(0, kUntil) + 16 * wave + 4 * g);
+        until = fetch16(b, kUntil * 256 + gate_rows);
         load_matrix(p_in, 0, pm);
-        since = gate_row(0, kSince)[token];
-        whole = gate_row(0, kSince)[kBlock - 1];
+        since = fetch4(b, kSince * 256 + token * 4);
+        whole = fetch4(b, kSince * 256 + (c | 63) * 4);
     }
-    for (int64_t first = 0; first < at.length; first = next) {
-        next = first + kBlock;
-        const int64_t ahead = next < at.length ? next : first;
-        const int64_t row0 = at.row + first;
-        const int length = (int)(at.length - first < kBlock ? at.length - first : kBlock);
-        Tile<NI, DK>& kb = kt[(first / kBlock) & 1];
+    for (int64_t first = 0; first < seq_length; first += kBlock) {
+        const int64_t ahead = first + kBlock < seq_length ? first + kBlock : first;
+        const Buffer gb = gates_of(ahead);
+        const Tile<NI, DK> kb(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes);
 
-        if (states != nullptr && mine) {
-            float* to = states + entry_of(first) * s.dk * s.dv + col;
+        if constexpr (KEEP) {
+            const Buffer to = buffer_of(states + entry_of(first) * s.dk * s.dv, (int64_t)s.dk * s.dv * 4);
 #pragma unroll
             for (int t = 0; t < kOwn; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * (kOwn * wave + t) + 4 * g + r;
-                    if (row < s.dk) to[(int64_t)row * s.dv] = S[t][r];
-                }
+                for (int r = 0; r < 4; ++r)
+                    put1<ElemF32>(to, mine ? ((16 * (kOwn * wave + t) + 4 * g + r) * s.dv + col) * 4 : kOutside, S[t][r]);
         }
 #pragma unroll
         for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, S[t]);
@@ -153,8 +159,8 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
             for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * u[r];
         }
-        beta = *reinterpret_cast<const fx4*>(gate_row(ahead, kBeta) + 16 * wave + 4 * g);
-        beta_since = *reinterpret_cast<const fx4*>(gate_row(ahead, kBetaSince) + 16 * wave + 4 * g);
+        beta = fetch16(gb, kBeta * 256 + gate_rows);
+        beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
         xr.put(wave, lane, u);
         lds_barrier();
 
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
             for (int r = 0; r < 4; ++r) x[r] = until[r] * u[r];
             xd.put(wave, lane, x);
         }
-        until = *reinterpret_cast<const fx4*>(gate_row(ahead, kUntil) + 16 * wave + 4 * g);
+        until = fetch16(gb, kUntil * 256 + gate_rows);
         lds_barrier();
 
         // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
@@ -191,16 +197,18 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
             o = mma<NS, NS>(xu.get(0, lane), pm[0], o);
             if (wave >= 2) o = mma<NS, NS>(xu.get(1, lane), pm[1], o);
             const int d = col0 + 4 * g;
-            if (token < length && d < s.dv) store4<E>(out + ((row0 + token) * s.heads + head) * s.dv + d, o);
+            const Buffer to = rows_of(out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
+            put4<E>(to, d < s.dv ? token * v_step + d * kSize : kOutside, o);
         }
         load_matrix(p_in, ahead, pm);
-        since = gate_row(ahead, kSince)[token];
-        whole = gate_row(ahead, kSince)[kBlock - 1];
-        if (updates != nullptr && mine) {
-            float* to = updates + ((row0 + 16 * wave + 4 * g) * s.heads + head) * s.dv + col;
+        since = fetch4(gb, kSince * 256 + token * 4);
+        whole = fetch4(gb, kSince * 256 + (c | 63) * 4);
+        if constexpr (KEEP) {
+            const uint32_t step = s.heads * s.dv * 4;
+            const Buffer to = rows_of(updates, first, step, (int64_t)head * s.dv * 4, s.dv * 4);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (16 * wave + 4 * g + r < length) to[(int64_t)r * s.heads * s.dv] = u[r];
+                put1<ElemF32>(to, mine ? (16 * wave + 4 * g + r) * step + col * 4 : kOutside, u[r]);
         }
     }
     if (final != nullptr && mine) {

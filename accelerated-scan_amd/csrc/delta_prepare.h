@@ -216,12 +216,8 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
             __builtin_memcpy(t_to + i * 32, t, 32);
             __builtin_memcpy(p_to + i * 32, p, 32);
         } else {
-            Operand<NS> to, po;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                set_parts<NS>(to, e, t[e]);
-                set_parts<NS>(po, e, p[e]);
-            }
+            const Operand<NS> to = operand_of<NS>(fx4{t[0], t[1], t[2], t[3]}, fx4{t[4], t[5], t[6], t[7]});
+            const Operand<NS> po = operand_of<NS>(fx4{p[0], p[1], p[2], p[3]}, fx4{p[4], p[5], p[6], p[7]});
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 *reinterpret_cast<bx8*>(t_to + (n * kPairs * 64 + i) * 16) = to.p[n];
@@ -233,15 +229,14 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
 
 // Operand `pair` of a matrix that delta_prepare wrote.
 template <int P>
-__device__ __forceinline__ Operand<P> matrix_operand(const char* m, int pair, int lane) {
+__device__ __forceinline__ Operand<P> matrix_operand(Buffer m, int pair, int lane) {
     Operand<P> o;
     if constexpr (P == 0) {
-        const fx4* p = reinterpret_cast<const fx4*>(m + (pair * 64 + lane) * 32);
-        o.t[0] = p[0];
-        o.t[1] = p[1];
+        o.t[0] = fetch16(m, (pair * 64 + lane) * 32);
+        o.t[1] = fetch16(m, (pair * 64 + lane) * 32 + 16);
     } else {
 #pragma unroll
-        for (int n = 0; n < P; ++n) o.p[n] = *reinterpret_cast<const bx8*>(m + ((n * kPairs + pair) * 64 + lane) * 16);
+        for (int n = 0; n < P; ++n) o.p[n] = __builtin_bit_cast(bx8, fetch16(m, ((n * kPairs + pair) * 64 + lane) * 16));
     }
     return o;
 }

@@ -41,14 +41,35 @@ struct Operand<0> {
     fx4 t[2];
 };
 
-// x as parts: each the rounding (to nearest even) of what the earlier ones leave.
+// Two values as parts, each the rounding (to nearest even) of what the earlier ones leave; the pair of part i as
+// a word, from which both come back as fp32 with one operation.
 template <int P>
-__device__ __forceinline__ void set_parts(Operand<P>& o, int e, float x) {
+__device__ __forceinline__ void pair_parts(float a, float b, uint32_t (&w)[P]) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const __bf16 h = (__bf16)x;
-        o.p[i][e] = h;
-        x -= (float)h;
+        const f2 x = {a, b};
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, b2));
+        if (i + 1 < P) {
+            a -= __builtin_bit_cast(float, w[i] << 16);
+            b -= __builtin_bit_cast(float, w[i] & 0xffff0000u);
+        }
+    }
+}
+// Elements e .. e+3 of an operand.
+template <int P>
+__device__ __forceinline__ void set_parts4(Operand<P>& o, int e, const fx4& x) {
+    uint32_t low[P], high[P];
+    pair_parts<P>(x[0], x[1], low);
+    pair_parts<P>(x[2], x[3], high);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        uint32_t w[4];
+        __builtin_memcpy(w, &o.p[i], 16);
+        w[e / 2] = low[i];
+        w[e / 2 + 1] = high[i];
+        __builtin_memcpy(&o.p[i], w, 16);
     }
 }
 
@@ -60,11 +81,8 @@ __device__ __forceinline__ Operand<P> operand_of(const fx4& a, const fx4& b) {
         o.t[0] = a;
         o.t[1] = b;
     } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            set_parts<P>(o, r, a[r]);
-            set_parts<P>(o, r + 4, b[r]);
-        }
+        set_parts4<P>(o, 0, a);
+        set_parts4<P>(o, 4, b);
     }
     return o;
 }
@@ -137,22 +155,84 @@ __device__ __forceinline__ Eight<E> load8(const typename E::S* p, bool there) {
     return r;
 }
 
-// Depths k0 .. k0+31 of a row in memory, as they travel: eight elements of a lane.
+// ---------------------------------------------------------------------------
+// Memory through buffer descriptors, whose hardware bounds check stands in for conditions: a load beyond the end
+// gives zero, a store there is dropped.  Without branches around them the compiler counts the requests in flight
+// and waits for the one it needs only; with them it waits for all.
+// ---------------------------------------------------------------------------
+typedef __amdgpu_buffer_rsrc_t Buffer;
+typedef uint32_t ux2 __attribute__((ext_vector_type(2)));
+typedef uint32_t ux4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t kOutside = 0x7ffffff0u;  // an offset beyond every buffer
+
+// `p` and `bytes` (below 2^31) the same in all lanes.
+__device__ __forceinline__ Buffer buffer_of(const void* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes < 0 ? 0 : (int)bytes, 0x00027000);
+}
+__device__ __forceinline__ fx4 fetch16(Buffer b, uint32_t at) {
+    return __builtin_bit_cast(fx4, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+}
+__device__ __forceinline__ float fetch4(Buffer b, uint32_t at) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0));
+}
+// Eight neighbouring elements at byte `at`.
 template <class E>
-__device__ __forceinline__ Eight<E> load_depths(const typename E::S* p, int k0, int g, int width, bool there) {
+__device__ __forceinline__ Eight<E> fetch8(Buffer b, uint32_t at) {
     Eight<E> r;
-    constexpr int kBytes = 4 * sizeof(typename E::S);
+    const fx4 x = fetch16(b, at);
+    __builtin_memcpy(&r.v[0], &x, 16);
+    if constexpr (E::kWide) {
+        const fx4 y = fetch16(b, at + 16);
+        __builtin_memcpy(&r.v[4], &y, 16);
+    }
+    return r;
+}
+// Depths k0 .. k0+31 of the row of `width` elements at byte `at`: eight elements of a lane.
+template <class E>
+__device__ __forceinline__ Eight<E> fetch_depths(Buffer b, uint32_t at, int k0, int g, int width) {
+    Eight<E> r;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int d = k0 + 16 * h + 4 * g;
-        if (there && d < width) {
-            __builtin_memcpy(&r.v[4 * h], __builtin_assume_aligned(p + d, kBytes), kBytes);
+        const uint32_t from = d < width ? at + d * (uint32_t)sizeof(typename E::S) : kOutside;
+        if constexpr (E::kWide) {
+            const fx4 x = fetch16(b, from);
+            __builtin_memcpy(&r.v[4 * h], &x, 16);
         } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r.v[4 * h + i] = E::put(0.0f);
+            const ux2 x = __builtin_amdgcn_raw_buffer_load_b64(b, from, 0, 0);
+            __builtin_memcpy(&r.v[4 * h], &x, 8);
         }
     }
     return r;
+}
+// Four neighbouring values, and one, to byte `at`.
+template <class E>
+__device__ __forceinline__ void put4(Buffer b, uint32_t at, const fx4& x) {
+    typename E::S s[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = E::put(x[r]);
+    if constexpr (E::kWide) {
+        ux4 v;
+        __builtin_memcpy(&v, s, 16);
+        __builtin_amdgcn_raw_buffer_store_b128(v, b, at, 0, 0);
+    } else {
+        ux2 v;
+        __builtin_memcpy(&v, s, 8);
+        __builtin_amdgcn_raw_buffer_store_b64(v, b, at, 0, 0);
+    }
+}
+template <class E>
+__device__ __forceinline__ void put1(Buffer b, uint32_t at, float x) {
+    const typename E::S s = E::put(x);
+    if constexpr (E::kWide) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, s), b, at, 0, 0);
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, s), b, at, 0, 0);
+    }
+}
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
 }
 
 template <int P, class E>
@@ -168,8 +248,13 @@ __device__ __forceinline__ Operand<P> operand_from(const Eight<E>& x) {
         static_assert(sizeof(typename E::S) == 2, "one part holds a bfloat16 value");
         __builtin_memcpy(&o.p[0], x.v, 16);
     } else {
+        fx4 a, b;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) set_parts<P>(o, i, E::get(x.v[i]));
+        for (int i = 0; i < 4; ++i) {
+            a[i] = E::get(x.v[i]);
+            b[i] = E::get(x.v[i + 4]);
+        }
+        o = operand_of<P>(a, b);
     }
     return o;
 }
@@ -205,16 +290,14 @@ struct Tile {
     __device__ __forceinline__ explicit Tile(void* p) : base(static_cast<__bf16*>(p)) {}
 
     template <class E>
-    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) {
+    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) const {
         __bf16* at = base + row * kStride + col;
         if constexpr (P == 1 && sizeof(typename E::S) == 2) {
             fx4 v;
             __builtin_memcpy(&v, x.v, 16);
             *reinterpret_cast<fx4*>(at) = v;
         } else {
-            Operand<P> o;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) set_parts<P>(o, i, E::get(x.v[i]));
+            const Operand<P> o = operand_from<P, E>(x);
 #pragma unroll
             for (int i = 0; i < P; ++i) *reinterpret_cast<bx8*>(at + i * kPlane) = o.p[i];
         }
@@ -270,7 +353,7 @@ struct Tile<0, W> {
     __device__ __forceinline__ explicit Tile(void* p) : base(static_cast<float*>(p)) {}
 
     template <class E>
-    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) {
+    __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) const {
         fx4 a, b;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -315,13 +398,12 @@ struct Exchange {
         if constexpr (P == 0) {
             *reinterpret_cast<fx4*>(base + (tile * 64 + lane) * 16) = x;
         } else {
-            Operand<P> o;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) set_parts<P>(o, r, x[r]);
+            uint32_t low[P], high[P];
+            pair_parts<P>(x[0], x[1], low);
+            pair_parts<P>(x[2], x[3], high);
 #pragma unroll
             for (int i = 0; i < P; ++i)
-                *reinterpret_cast<bx4*>(base + ((i * N + (tile >> 1)) * 64 + lane) * 16 + (tile & 1) * 8) =
-                    __builtin_shufflevector(o.p[i], o.p[i], 0, 1, 2, 3);
+                *reinterpret_cast<ux2*>(base + ((i * N + (tile >> 1)) * 64 + lane) * 16 + (tile & 1) * 8) = ux2{low[i], high[i]};
         }
     }
     __device__ __forceinline__ Operand<P> get(int n, int lane) const {
