@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
     for (int t = 0; t < DK / 16; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * t + 4 * g + r;
+            const int row = feature_row(t, g, r);
             D[t][r] = d_final != nullptr && mine && row < s.dk ? d_final[state_at + (int64_t)row * s.dv + col] : 0.0f;
         }
 
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
             for (int t = 0; t < DK / 16; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (16 * t + 4 * g + r < s.dk) to[(int64_t)(16 * t + 4 * g + r) * s.dv] = D[t][r];
+                    if (feature_row(t, g, r) < s.dk) to[(int64_t)feature_row(t, g, r) * s.dv] = D[t][r];
         }
         // dU = diag(e^(c[63]-c)) K D1 + P^T dO
         fx4 u[kTiles];
@@ -146,10 +146,10 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
         for (int t = 0; t < DK / 16; ++t) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) D[t][r] *= whole;
-            D[t] = mma<NI, NS>(qt.down(0, 16 * t, lane), w_low, D[t]);
-            D[t] = mma<NI, NS>(qt.down(32, 16 * t, lane), w_high, D[t]);
-            D[t] = mma<NI, NS>(kt.down(0, 16 * t, lane), low, D[t]);
-            D[t] = mma<NI, NS>(kt.down(32, 16 * t, lane), high, D[t]);
+            D[t] = mma<NI, NS>(qt.down_features(0, t, lane), w_low, D[t]);
+            D[t] = mma<NI, NS>(qt.down_features(32, t, lane), w_high, D[t]);
+            D[t] = mma<NI, NS>(kt.down_features(0, t, lane), low, D[t]);
+            D[t] = mma<NI, NS>(kt.down_features(32, t, lane), high, D[t]);
         }
     }
     if (d_initial != nullptr && mine) {
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
         for (int t = 0; t < DK / 16; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (16 * t + 4 * g + r < s.dk) d_initial[state_at + (int64_t)(16 * t + 4 * g + r) * s.dv + col] = D[t][r];
+                if (feature_row(t, g, r) < s.dk) d_initial[state_at + (int64_t)feature_row(t, g, r) * s.dv + col] = D[t][r];
     }
     if (s.offsets != nullptr && mine) {
         if (n == 0)
@@ -174,7 +174,7 @@ __device__ __forceinline__ Operand<P> memory_operand(const float* p, int64_t str
                                                      int cols, int g, fx4 (&raw)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int d = col + 16 * h + 4 * g;
+        const int d = col + 8 * g + 4 * h;
         raw[h] = fx4{0, 0, 0, 0};
         if (row < rows && d < cols) raw[h] = *reinterpret_cast<const fx4*>(p + row * stride + d);
     }

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
     for (int t = 0; t < kOwn; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * (kOwn * wave + t) + 4 * g + r;
+            const int row = feature_row(kOwn * wave + t, g, r);
             S[t][r] = initial != nullptr && mine && row < s.dk ? initial[state_at + (int64_t)row * s.dv] : 0.0f;
         }
 
@@ -94,13 +94,13 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
             const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
             k_raw[i] = fetch8<E>(kb, d < s.dk ? row * k_step + d * kSize : kOutside);
         }
-        const int d = col0 + (tid & 1) * 8;
-        v_raw = fetch8<E>(vb, tid < 128 && d < s.dv ? (tid >> 1) * v_step + d * kSize : kOutside);
+        const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
+        v_raw = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
     };
     const auto load_q = [&](int64_t first) {
         const Buffer b = rows_of(q, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
 #pragma unroll
-        for (int d = 0; d < kDepths; ++d) q_raw[d] = fetch_depths<E>(b, token * k_step, 32 * d, g, s.dk);
+        for (int d = 0; d < kDepths; ++d) q_raw[d] = fetch8<E>(b, 32 * d + 8 * g < s.dk ? token * k_step + (32 * d + 8 * g) * kSize : kOutside);
     };
     // (waves 0 and 1 have one operand to a row of tiles: their second load repeats the first)
     const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
@@ -119,10 +119,21 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
         beta_since = fetch16(b, kBetaSince * 256 + gate_rows);
         load_matrix(t_in, 0, tm);
         until = fetch16(b, kUntil * 256 + gate_rows);
-        load_matrix(p_in, 0, pm);
-        since = fetch4(b, kSince * 256 + token * 4);
         whole = fetch4(b, kSince * 256 + (c | 63) * 4);
     }
+    // out^T = scale (Q S0)^T diag(e^c) + U^T P^T of the block at `first`: finished while the next block's first
+    // product waits for its operands
+    fx4 o = {0, 0, 0, 0};
+    const auto finish = [&](int64_t first, const Operand<NS>& low, const Operand<NS>& high) {
+        const float f = s.scale * since;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] *= f;
+        o = mma<NS, NS>(low, pm[0], o);
+        if (wave >= 2) o = mma<NS, NS>(high, pm[1], o);
+        const int d = col0 + 4 * g;
+        const Buffer to = rows_of(out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
+        put4<E>(to, d < s.dv ? token * v_step + d * kSize : kOutside, o);
+    };
     for (int64_t first = 0; first < seq_length; first += kBlock) {
         const int64_t ahead = first + kBlock < seq_length ? first + kBlock : first;
         const Buffer gb = gates_of(ahead);
@@ -134,74 +145,79 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
             for (int t = 0; t < kOwn; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    put1<ElemF32>(to, mine ? ((16 * (kOwn * wave + t) + 4 * g + r) * s.dv + col) * 4 : kOutside, S[t][r]);
+                    put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, S[t][r]);
         }
 #pragma unroll
         for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, S[t]);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[i]);
-        if (tid < 128) vt.template put8<E>(tid >> 1, (tid & 1) * 8, v_raw);
+        vt.template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw);
         lds_barrier();
-        load_kv(ahead);
 
-        // K S0 (rows: tokens, columns: state columns) and (Q S0)^T (rows: state columns, columns: tokens)
-        fx4 u = {0, 0, 0, 0}, o = {0, 0, 0, 0};
+        // K S0 (rows: tokens, columns: state columns)
+        Operand<NS> so[kDepths];
+        Operand<NI> ko[kDepths];
 #pragma unroll
         for (int d = 0; d < kDepths; ++d) {
-            const Operand<NS> so = xs.get(d, lane);
-            u = mma<NI, NS>(kb.along(token, 32 * d, g), so, u);
-            o = mma<NS, NI>(so, operand_from<NI, E>(q_raw[d]), o);
+            so[d] = xs.get(d, lane);
+            ko[d] = kb.along(token, 32 * d, g);
         }
-        load_q(ahead);
-        // R = diag(beta) V - diag(beta e^c) K S0
-        {
-            const fx4 x = vt.tile(16 * wave, 0, lane);
+        const Operand<NS> u_low = xu.get(0, lane), u_high = xu.get(1, lane);  // of the block before
+        fx4 x = vt.tile(16 * wave, 0, lane);
+        load_kv(ahead);
+        __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
+        fx4 u = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * u[r];
-        }
+        for (int d = 0; d < kDepths; ++d) u = mma<NI, NS>(ko[d], so[d], u);
+        if (first > 0) finish(first - kBlock, u_low, u_high);
+        const Buffer here = gates_of(first);
+        load_matrix(p_in, first, pm);
+        since = fetch4(here, kSince * 256 + token * 4);
+        // R = diag(beta) V - diag(beta e^c) K S0
+#pragma unroll
+        for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * u[r];
+        xr.put(wave, lane, u);
         beta = fetch16(gb, kBeta * 256 + gate_rows);
         beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
-        xr.put(wave, lane, u);
         lds_barrier();
 
-        // U = R + T R
-        u = mma<NS, NS>(tm[0], xr.get(0, lane), u);
-        if (wave >= 2) u = mma<NS, NS>(tm[1], xr.get(1, lane), u);
+        // U = R + T R, and (Q S0)^T (rows: state columns, columns: tokens) while its operands come
+        {
+            const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            o = fx4{0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < kDepths; ++d) o = mma<NS, NI>(so[d], operand_from<NI, E>(q_raw[d]), o);
+            u = mma<NS, NS>(tm[0], low, u);
+            if (wave >= 2) u = mma<NS, NS>(tm[1], high, u);
+        }
+        load_q(ahead);
         load_matrix(t_in, ahead, tm);
         xu.put(wave, lane, u);
-        {
-            fx4 x;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = until[r] * u[r];
-            xd.put(wave, lane, x);
-        }
+        for (int r = 0; r < 4; ++r) x[r] = until[r] * u[r];
+        xd.put(wave, lane, x);
         until = fetch16(gb, kUntil * 256 + gate_rows);
         lds_barrier();
 
         // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
         {
             const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
+            Operand<NI> k_low[kOwn], k_high[kOwn];
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+                k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
+                k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) S[t][r] *= whole;
-                S[t] = mma<NI, NS>(kb.down(0, 16 * (kOwn * wave + t), lane), low, S[t]);
-                S[t] = mma<NI, NS>(kb.down(32, 16 * (kOwn * wave + t), lane), high, S[t]);
+                S[t] = mma<NI, NS>(k_low[t], low, S[t]);
+                S[t] = mma<NI, NS>(k_high[t], high, S[t]);
             }
         }
-        // out^T = scale (Q S0)^T diag(e^c) + U^T P^T
-        {
-            const float f = s.scale * since;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[r] *= f;
-            o = mma<NS, NS>(xu.get(0, lane), pm[0], o);
-            if (wave >= 2) o = mma<NS, NS>(xu.get(1, lane), pm[1], o);
-            const int d = col0 + 4 * g;
-            const Buffer to = rows_of(out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
-            put4<E>(to, d < s.dv ? token * v_step + d * kSize : kOutside, o);
-        }
-        load_matrix(p_in, ahead, pm);
-        since = fetch4(gb, kSince * 256 + token * 4);
         whole = fetch4(gb, kSince * 256 + (c | 63) * 4);
         if constexpr (KEEP) {
             const uint32_t step = s.heads * s.dv * 4;
@@ -211,12 +227,13 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
                 put1<ElemF32>(to, mine ? (16 * wave + 4 * g + r) * step + col * 4 : kOutside, u[r]);
         }
     }
+    if (seq_length > 0) finish((seq_length - 1) / kBlock * kBlock, xu.get(0, lane), xu.get(1, lane));
     if (final != nullptr && mine) {
 #pragma unroll
         for (int t = 0; t < kOwn; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * (kOwn * wave + t) + 4 * g + r;
+                const int row = feature_row(kOwn * wave + t, g, r);
                 if (row < s.dk) final[state_at + (int64_t)row * s.dv] = S[t][r];
             }
     }

@@ -4,9 +4,13 @@
 // All products are chains of 16x16 tiles.  The accumulator of a tile holds, in lane l with
 // g = l / 16, column l % 16 and rows 4g .. 4g+3; an operand of a product of depth 32 holds, in lane
 // l, one row (left) or column (right) l % 16 and eight values of the depth axis.  The order of the
-// depth axis is free as long as both operands use the same one, so here lane group g holds depths
-// 4g .. 4g+3 and 16+4g .. 16+4g+3: then the accumulators of two stacked tiles ARE an operand of
-// the next product, and a state, its products and its update stay in the registers of one wave.
+// depth axis is free as long as both operands use the same one, so the accumulators of two stacked
+// tiles ARE an operand of the next product: lane group g holds rows 4g .. 4g+3 of either tile.  What stands for
+// depths 32n .. 32n+31 there depends on what the tiles' rows are:
+//   - tokens: the tiles are rows 32n .. +15 and 32n+16 .. +31, the other operand is read `down` a column of a
+//     row-major tile with the transposing LDS read;
+//   - features: the rows of the two tiles are dealt out in fours, row 4g+r of tile i being feature
+//     32n + 8g + 4i + r (`feature_row`), so that the other operand is 16 neighbouring bytes `along` a row.
 //
 // Arithmetic (parameter P of an operand, its number of parts):
 //   P = 0   fp32 values and fp32 matrix instructions, 256 operations per clock and compute unit;
@@ -187,24 +191,6 @@ __device__ __forceinline__ Eight<E> fetch8(Buffer b, uint32_t at) {
     }
     return r;
 }
-// Depths k0 .. k0+31 of the row of `width` elements at byte `at`: eight elements of a lane.
-template <class E>
-__device__ __forceinline__ Eight<E> fetch_depths(Buffer b, uint32_t at, int k0, int g, int width) {
-    Eight<E> r;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int d = k0 + 16 * h + 4 * g;
-        const uint32_t from = d < width ? at + d * (uint32_t)sizeof(typename E::S) : kOutside;
-        if constexpr (E::kWide) {
-            const fx4 x = fetch16(b, from);
-            __builtin_memcpy(&r.v[4 * h], &x, 16);
-        } else {
-            const ux2 x = __builtin_amdgcn_raw_buffer_load_b64(b, from, 0, 0);
-            __builtin_memcpy(&r.v[4 * h], &x, 8);
-        }
-    }
-    return r;
-}
 // Four neighbouring values, and one, to byte `at`.
 template <class E>
 __device__ __forceinline__ void put4(Buffer b, uint32_t at, const fx4& x) {
@@ -276,6 +262,9 @@ __device__ __forceinline__ void store4(typename E::S* p, const fx4& x) {
     }
 }
 
+// Feature that row 4g + r of state tile t stands for.
+__device__ __forceinline__ constexpr int feature_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
+
 // ---------------------------------------------------------------------------
 // 64 rows of W values in LDS, as fp32 (P = 0) or as P planes of bfloat16 parts.  Rows are padded by
 // 16 bytes so that the 16 rows of an operand start in different banks.
@@ -306,10 +295,19 @@ struct Tile {
     __device__ __forceinline__ Operand<P> along(int row, int k0, int g) const {
         Operand<P> o;
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
-            const __bf16* at = base + i * kPlane + row * kStride + k0 + 4 * g;
-            const bx4 a = *reinterpret_cast<const bx4*>(at), b = *reinterpret_cast<const bx4*>(at + 16);
-            o.p[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int i = 0; i < P; ++i) o.p[i] = *reinterpret_cast<const bx8*>(base + i * kPlane + row * kStride + k0 + 8 * g);
+        return o;
+    }
+    // Depths row0 .. row0+31 (tokens) of the features of state tile t, in the order of feature_row().
+    __device__ __forceinline__ Operand<P> down_features(int row0, int t, int lane) const {
+        const int g = lane >> 4, i = lane & 15;
+        Operand<P> o;
+#pragma unroll
+        for (int n = 0; n < P; ++n) {
+            __bf16* at = base + n * kPlane + (row0 + 4 * g + (i >> 2)) * kStride + feature_row(t, i & 3, 0);
+            const sx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)at);
+            const sx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)(at + 16 * kStride));
+            o.p[n] = __builtin_shufflevector(__builtin_bit_cast(bx4, a), __builtin_bit_cast(bx4, b), 0, 1, 2, 3, 4, 5, 6, 7);
         }
         return o;
     }
@@ -365,10 +363,20 @@ struct Tile<0, W> {
         *reinterpret_cast<fx4*>(at + 4) = b;
     }
     __device__ __forceinline__ Operand<0> along(int row, int k0, int g) const {
-        const float* at = base + row * kStride + k0 + 4 * g;
+        const float* at = base + row * kStride + k0 + 8 * g;
         Operand<0> o;
         o.t[0] = *reinterpret_cast<const fx4*>(at);
-        o.t[1] = *reinterpret_cast<const fx4*>(at + 16);
+        o.t[1] = *reinterpret_cast<const fx4*>(at + 4);
+        return o;
+    }
+    __device__ __forceinline__ Operand<0> down_features(int row0, int t, int lane) const {
+        const float* at = base + (row0 + 4 * (lane >> 4)) * kStride + feature_row(t, (lane >> 2) & 3, lane & 3);
+        Operand<0> o;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            o.t[0][r] = at[r * kStride];
+            o.t[1][r] = at[(16 + r) * kStride];
+        }
         return o;
     }
     __device__ __forceinline__ fx4 tile(int row0, int col0, int lane) const {
