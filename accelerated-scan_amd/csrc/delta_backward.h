@@ -18,152 +18,226 @@
 namespace ascan {
 namespace {
 
-constexpr int kColumns = 64;  // value columns that a workgroup takes at a time
+constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
-template <int NI, int DK>
-constexpr int kReverseBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, kColumns>::kBytes;
+template <int NI, int NS, int DK>
+constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
+                              3 * Exchange<NS, 2>::kBytes;
 
-// The chain, last block first: 16 columns of D stay in a wave's accumulators.
-// grid (column groups, heads, sequences), 256 threads.
+// The chain, last block first, divided like the forward one: 16 columns of D to a workgroup, wave w keeps rows
+// dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.
+// grid chain_grid(), 256 threads.
 template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(256) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
     const char* __restrict__ p_in, const float* __restrict__ d_final, typename E::S* __restrict__ d_v,
     float* __restrict__ d_initial, float* __restrict__ d_states, float* __restrict__ d_rows) {
+    using ES = typename E::S;
+    constexpr int kDepths = DK / 32, kOwn = DK / 64, kCopies = DK / 32;
     extern __shared__ __align__(16) char smem[];
-    __shared__ __align__(16) float gate[4 * kBlock];
-    const int64_t n = blockIdx.z;
-    const int head = blockIdx.y, key_head = head / (s.heads / s.key_heads);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
-    const int col0 = blockIdx.x * kColumns, col = col0 + 16 * wave + c;
+    const ChainAt where = chain_at(s);
+    if (!where.there) return;
+    const int64_t n = where.sequence;
+    const int head = where.head, key_head = head / (s.heads / s.key_heads);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int col0 = where.col0, col = col0 + c;
     const bool mine = col < s.dv;
     const SequenceAt at = sequence_at(s, n);
 
-    Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
-    Tile<NI, kColumns> ot(smem + 2 * Tile<NI, DK>::kBytes);
+    // (queries are read between the second and the third barrier only: one tile is enough)
+    char* m = smem + 2 * Tile<NI, DK>::kBytes;
+    const Tile<NI, DK> qt(m);
+    m += Tile<NI, DK>::kBytes;
+    const Tile<NI, 16> ot(m);
+    m += Tile<NI, 16>::kBytes;
+    Exchange<NS, kDepths> xs(m);
+    m += Exchange<NS, kDepths>::kBytes;
+    Exchange<NS, 2> xr(m), xw(m + Exchange<NS, 2>::kBytes), xu(m + 2 * Exchange<NS, 2>::kBytes);
 
-    fx4 D[DK / 16];
-    const int64_t state_at = (n * s.heads + head) * s.dk * s.dv;
+    fx4 D[kOwn];
+    const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t)
+    for (int t = 0; t < kOwn; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = feature_row(t, g, r);
-            D[t][r] = d_final != nullptr && mine && row < s.dk ? d_final[state_at + (int64_t)row * s.dv + col] : 0.0f;
+            const int row = feature_row(kOwn * wave + t, g, r);
+            D[t][r] = d_final != nullptr && mine && row < s.dk ? d_final[state_at + (int64_t)row * s.dv] : 0.0f;
         }
 
-    for (int64_t first = (at.length - 1) / kBlock * kBlock; first >= 0 && at.length > 0; first -= kBlock) {
-        const int64_t row0 = at.row + first, block = at.block + first / kBlock;
-        const int length = (int)(at.length - first < kBlock ? at.length - first : kBlock);
-        const int64_t entry = block * s.heads + head;
-        __syncthreads();
-        for (int i = tid; i < kBlock * DK / 8; i += 256) {
-            const int row = i / (DK / 8), d = i % (DK / 8) * 8;
-            const bool there = row < length && d < s.dk;
-            const int64_t from = ((row0 + row) * s.key_heads + key_head) * s.dk + d;
-            kt.template put8<E>(row, d, load8<E>(k + from, there));
-            qt.template put8<E>(row, d, load8<E>(q + from, there));
-        }
-        for (int i = tid; i < kBlock * kColumns / 8; i += 256) {
-            const int row = i / (kColumns / 8), d = i % (kColumns / 8) * 8;
-            const bool there = d_out != nullptr && row < length && col0 + d < s.dv;
-            ot.template put8<E>(row, d, load8<E>(d_out + ((row0 + row) * s.heads + head) * s.dv + col0 + d, there));
-        }
-        gate[tid] = gates[entry * kGateFloats + tid];
-        __syncthreads();
-        const float whole = gate[kSince * kBlock + kBlock - 1];
-        const Buffer tm = buffer_of(t_in + entry * kMatrixBytes<NS>, kMatrixBytes<NS>);
-        const Buffer pm = buffer_of(p_in + entry * kMatrixBytes<NS>, kMatrixBytes<NS>);
-
-        if (mine) {
-            float* to = d_states + entry * s.dk * s.dv + col;
+    constexpr uint32_t kSize = sizeof(ES);
+    const uint32_t k_step = s.key_heads * s.dk * kSize, v_step = s.heads * s.dv * kSize, r_step = s.heads * s.dv * 4;
+    const int64_t seq_row = uniform(at.row), seq_length = uniform(at.length), seq_block = uniform(at.block);
+    const int token = 16 * wave + c;
+    const auto rows_of = [&](const void* p, int64_t first, uint32_t step, int64_t at_head, uint32_t bytes) {
+        const int64_t left = seq_length - first < kBlock ? seq_length - first : kBlock;
+        return buffer_of(static_cast<const char*>(p) + (seq_row + first) * step + at_head, (left - 1) * (int64_t)step + bytes);
+    };
+    const auto entry_of = [&](int64_t first) { return (seq_block + first / kBlock) * s.heads + head; };
+    Eight<E> k_raw[kCopies], q_raw[kCopies], o_raw;
+    Operand<NS> tm[2], pm[2];
+    fx4 beta, beta_since, until, since;
+    float whole;
+    const auto load_rows = [&](int64_t first) {
+        const Buffer kb = rows_of(k, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const Buffer qb = rows_of(q, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const Buffer ob = d_out != nullptr ? rows_of(d_out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize) : buffer_of(k, 0);
 #pragma unroll
-            for (int t = 0; t < DK / 16; ++t)
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
+            k_raw[i] = fetch8<E>(kb, d < s.dk ? row * k_step + d * kSize : kOutside);
+            q_raw[i] = fetch8<E>(qb, d < s.dk ? row * k_step + d * kSize : kOutside);
+        }
+        const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
+        o_raw = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+    };
+    // (waves 2 and 3 have one operand to a row of tiles: their first load repeats the second)
+    const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
+        const Buffer b = buffer_of(from + entry_of(first) * kMatrixBytes<NS>, kMatrixBytes<NS>);
+        o[0] = matrix_operand<NS>(b, pair_upper(wave, wave < 2 ? 0 : 1), lane);
+        o[1] = matrix_operand<NS>(b, pair_upper(wave, 1), lane);
+    };
+    const auto gates_of = [&](int64_t first) { return buffer_of(gates + entry_of(first) * kGateFloats, kGateFloats * 4); };
+    const uint32_t gate_rows = (16 * wave + 4 * g) * 4;
+
+    const int64_t last = (seq_length - 1) / kBlock * kBlock;
+    if (seq_length > 0) {  // (an empty sequence has no table entry to read)
+        load_rows(last);
+        load_matrix(p_in, last, pm);
+        const Buffer b = gates_of(last);
+        until = fetch16(b, kUntil * 256 + gate_rows);
+        since = fetch16(b, kSince * 256 + gate_rows);
+        load_matrix(t_in, last, tm);
+        beta = fetch16(b, kBeta * 256 + gate_rows);
+        beta_since = fetch16(b, kBetaSince * 256 + gate_rows);
+        whole = fetch4(b, kSince * 256 + (c | 63) * 4);
+    }
+    for (int64_t first = last; first >= 0 && seq_length > 0; first -= kBlock) {
+        const int64_t ahead = first > 0 ? first - kBlock : 0;
+        const Buffer gb = gates_of(ahead);
+        const Tile<NI, DK> kb(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes);
+        {
+            const Buffer to = buffer_of(d_states + entry_of(first) * s.dk * s.dv, (int64_t)s.dk * s.dv * 4);
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (feature_row(t, g, r) < s.dk) to[(int64_t)feature_row(t, g, r) * s.dv] = D[t][r];
+                    put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, D[t][r]);
         }
+#pragma unroll
+        for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, D[t]);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
+            kb.template put8<E>(row, d, k_raw[i]);
+            qt.template put8<E>(row, d, q_raw[i]);
+        }
+        ot.template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw);
+        lds_barrier();
+
         // dU = diag(e^(c[63]-c)) K D1 + P^T dO
-        fx4 u[kTiles];
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) u[m] = fx4{0, 0, 0, 0};
-#pragma unroll
-        for (int d = 0; d < DK / 32; ++d) {
-            const Operand<NS> so = operand_of<NS>(D[2 * d], D[2 * d + 1]);
-#pragma unroll
-            for (int m = 0; m < kTiles; ++m) u[m] = mma<NI, NS>(kt.along(16 * m + c, 32 * d, g), so, u[m]);
-        }
-        const Operand<NI> o_low = ot.down(0, 16 * wave, lane), o_high = ot.down(32, 16 * wave, lane);
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-            const fx4 f = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * m + 4 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) u[m][r] *= f[r];
-            if (m < 2) u[m] = mma<NS, NI>(matrix_operand<NS>(pm, pair_upper(m, 0), lane), o_low, u[m]);
-            u[m] = mma<NS, NI>(matrix_operand<NS>(pm, pair_upper(m, 1), lane), o_high, u[m]);
-        }
-        // dR = dU + T^T dU
+        fx4 u = {0, 0, 0, 0}, w;
         {
-            const Operand<NS> low = operand_of<NS>(u[0], u[1]), high = operand_of<NS>(u[2], u[3]);
+            Operand<NS> so[kDepths];
+            Operand<NI> ko[kDepths];
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                if (m < 2) u[m] = mma<NS, NS>(matrix_operand<NS>(tm, pair_upper(m, 0), lane), low, u[m]);
-                u[m] = mma<NS, NS>(matrix_operand<NS>(tm, pair_upper(m, 1), lane), high, u[m]);
+            for (int d = 0; d < kDepths; ++d) {
+                so[d] = xs.get(d, lane);
+                ko[d] = kb.along(token, 32 * d, g);
             }
-        }
-        if (mine) {
+            const Operand<NI> o_low = ot.down(0, 0, lane), o_high = ot.down(32, 0, lane);
+            w = ot.tile(16 * wave, 0, lane);
+            load_rows(ahead);
+            __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
+            fx4 po = {0, 0, 0, 0};
+            if (wave < 2) po = mma<NS, NI>(pm[0], o_low, po);
+            po = mma<NS, NI>(pm[1], o_high, po);
 #pragma unroll
-            for (int m = 0; m < kTiles; ++m) {
-                const fx4 b = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * m + 4 * g);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * m + 4 * g + r;
-                    if (row < length) {
-                        const int64_t to = ((row0 + row) * s.heads + head) * s.dv + col;
-                        d_v[to] = E::put(b[r] * u[m][r]);
-                        d_rows[to] = u[m][r];
-                    }
-                }
-            }
-        }
-        // D0 = e^c[63] D1 + Q^T diag(scale e^c) dO - K^T diag(beta e^c) dR
-        fx4 w[kTiles];
-#pragma unroll
-        for (int m = 0; m < kTiles; ++m) {
-            const fx4 f = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * m + 4 * g);
-            const fx4 b = *reinterpret_cast<const fx4*>(gate + kBetaSince * kBlock + 16 * m + 4 * g);
-            w[m] = ot.tile(16 * m, 16 * wave, lane);
+            for (int d = 0; d < kDepths; ++d) u = mma<NI, NS>(ko[d], so[d], u);
+            load_matrix(p_in, ahead, pm);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                w[m][r] *= s.scale * f[r];
-                u[m][r] *= -b[r];
+                u[r] = until[r] * u[r] + po[r];
+                w[r] *= s.scale * since[r];
             }
         }
-        const Operand<NS> low = operand_of<NS>(u[0], u[1]), high = operand_of<NS>(u[2], u[3]);
-        const Operand<NS> w_low = operand_of<NS>(w[0], w[1]), w_high = operand_of<NS>(w[2], w[3]);
+        xr.put(wave, lane, u);
+        xw.put(wave, lane, w);
+        until = fetch16(gb, kUntil * 256 + gate_rows);
+        since = fetch16(gb, kSince * 256 + gate_rows);
+        lds_barrier();
+
+        // dR = dU + T^T dU;  D0 = e^c[63] D1 + Q^T diag(scale e^c) dO while it waits
+        fx4 x;
+        {
+            const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane), w_low = xw.get(0, lane), w_high = xw.get(1, lane);
+            Operand<NI> q_low[kOwn], q_high[kOwn];
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
+            for (int t = 0; t < kOwn; ++t) {
+                q_low[t] = qt.down_features(0, kOwn * wave + t, lane);
+                q_high[t] = qt.down_features(32, kOwn * wave + t, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (wave < 2) u = mma<NS, NS>(tm[0], low, u);
+            u = mma<NS, NS>(tm[1], high, u);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) D[t][r] *= whole;
-            D[t] = mma<NI, NS>(qt.down_features(0, t, lane), w_low, D[t]);
-            D[t] = mma<NI, NS>(qt.down_features(32, t, lane), w_high, D[t]);
-            D[t] = mma<NI, NS>(kt.down_features(0, t, lane), low, D[t]);
-            D[t] = mma<NI, NS>(kt.down_features(32, t, lane), high, D[t]);
+            for (int t = 0; t < kOwn; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) D[t][r] *= whole;
+                D[t] = mma<NI, NS>(q_low[t], w_low, D[t]);
+                D[t] = mma<NI, NS>(q_high[t], w_high, D[t]);
+            }
         }
+        load_matrix(t_in, ahead, tm);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = -beta_since[r] * u[r];
+        xu.put(wave, lane, x);
+        beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
+        whole = fetch4(gb, kSince * 256 + (c | 63) * 4);
+        lds_barrier();
+
+        // D0 -= K^T diag(beta e^c) dR
+        {
+            const Operand<NS> low = xu.get(0, lane), high = xu.get(1, lane);
+            Operand<NI> k_low[kOwn], k_high[kOwn];
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+                k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
+                k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+                D[t] = mma<NI, NS>(k_low[t], low, D[t]);
+                D[t] = mma<NI, NS>(k_high[t], high, D[t]);
+            }
+        }
+        {
+            const Buffer to = rows_of(d_v, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
+            const Buffer rows = rows_of(d_rows, first, r_step, (int64_t)head * s.dv * 4, s.dv * 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                put1<E>(to, mine ? (16 * wave + 4 * g + r) * v_step + col * kSize : kOutside, beta[r] * u[r]);
+                put1<ElemF32>(rows, mine ? (16 * wave + 4 * g + r) * r_step + col * 4 : kOutside, u[r]);
+            }
+        }
+        beta = fetch16(gb, kBeta * 256 + gate_rows);
     }
     if (d_initial != nullptr && mine) {
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t)
+        for (int t = 0; t < kOwn; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (feature_row(t, g, r) < s.dk) d_initial[state_at + (int64_t)feature_row(t, g, r) * s.dv + col] = D[t][r];
+            for (int r = 0; r < 4; ++r) {
+                const int row = feature_row(kOwn * wave + t, g, r);
+                if (row < s.dk) d_initial[state_at + (int64_t)row * s.dv] = D[t][r];
+            }
     }
     if (s.offsets != nullptr && mine) {
+        const int own = 4 * wave + g;
         if (n == 0)
-            for (int64_t row = g; row < offset_at(s, 0); row += 4) d_v[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
+            for (int64_t row = own; row < offset_at(s, 0); row += 16) d_v[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
         if (n == s.sequences - 1)
-            for (int64_t row = offset_at(s, s.sequences) + g; row < s.rows; row += 4)
+            for (int64_t row = offset_at(s, s.sequences) + own; row < s.rows; row += 16)
                 d_v[(row * s.heads + head) * s.dv + col] = E::put(0.0f);
     }
 }

@@ -75,12 +75,10 @@ int delta_backward_dk(const DeltaBackward& f) {
     hipError_t e = hipSuccess;
     if (s.blocks > 0) e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, ws, at, true, f.stream);
     if (e != hipSuccess) return delta_status(e);
-    const unsigned groups = (unsigned)((s.dv + kColumns - 1) / kColumns);
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3(groups, (unsigned)s.heads, (unsigned)s.sequences),
-                     kReverseBytes<NI, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), kReverseBytes<NI, NS, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows);
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
