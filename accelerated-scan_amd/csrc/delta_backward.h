@@ -242,37 +242,34 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
     }
 }
 
-// Operand of 32 columns of a row-major fp32 matrix in memory: row `row`, columns col .. col + 31 below `cols`.
-template <int P>
-__device__ __forceinline__ Operand<P> memory_operand(const float* p, int64_t stride, int row, int rows, int col,
-                                                     int cols, int g, fx4 (&raw)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int d = col + 8 * g + 4 * h;
-        raw[h] = fx4{0, 0, 0, 0};
-        if (row < rows && d < cols) raw[h] = *reinterpret_cast<const fx4*>(p + row * stride + d);
-    }
-    return operand_of<P>(raw[0], raw[1]);
-}
-
+template <int NI, int NS>
+constexpr int kGradientShared = Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes > 4 * Exchange<NS, kPairs>::kBytes
+                                    ? Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes
+                                    : 4 * Exchange<NS, kPairs>::kBytes;
 template <int NI, int NS, int DK>
-constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes;
+constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS>;
 
-// A block of one key head and all value heads that share it; a wave owns 16 of the tokens.
-// grid (blocks, key heads), 256 threads.
+// A block of one key head and all value heads that share it.  A wave owns 16 features of keys and queries and dk/2
+// of the tokens, so that each row of the two states is read by one wave only (or two); the 64 x 64 products of
+// tokens with tokens are divided among the waves by tiles and go round through LDS.  What bounds it are the two fp32
+// states per block, 8 bytes per cell against 2 for an input; the next 64 value columns are requested while these are
+// computed.
+// grid (blocks, key heads), 512 threads.
 template <class E, int NI, int NS, int DK>
-__global__ __launch_bounds__(256) void delta_gradients(
+__global__ __launch_bounds__(512) void delta_gradients(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ v, const typename E::S* __restrict__ d_out, const float* __restrict__ gates,
     const float* __restrict__ states, const float* __restrict__ updates, const float* __restrict__ d_states,
     const float* __restrict__ d_rows, typename E::S* __restrict__ d_q, typename E::S* __restrict__ d_k,
     void* __restrict__ d_log_gates, void* __restrict__ d_beta) {
+    using ES = typename E::S;
+    constexpr int kFeatures = DK / 16, kTok = DK / 32;  // tiles of features, and of tokens that a wave owns
     extern __shared__ __align__(16) char smem[];
     __shared__ __align__(16) float gate[kGateFloats];
-    __shared__ float dc[kBlock], db[kBlock], whole_terms[4];
+    __shared__ float dots[8][3][16 * kTok], value_dots[kBlock], whole_terms[8];
     const int64_t block = blockIdx.x;
     const int key_head = blockIdx.y, share = s.heads / s.key_heads;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
 
     // rows in front of the first and behind the last sequence: zero gradients, 64 rows to a workgroup
     if (s.offsets != nullptr) {
@@ -280,7 +277,7 @@ __global__ __launch_bounds__(256) void delta_gradients(
         const int64_t spans[2][2] = {{0, before}, {behind, s.rows}};
         for (int i = 0; i < 2; ++i)
             for (int64_t row = spans[i][0] + block * kBlock + wave; row < spans[i][1] && row < spans[i][0] + (block + 1) * kBlock;
-                 row += 4) {
+                 row += 8) {
                 for (int d = lane; d < s.dk; d += 64) {
                     d_q[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
                     d_k[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
@@ -290,114 +287,182 @@ __global__ __launch_bounds__(256) void delta_gradients(
                     if (s.wide_gates) {
                         static_cast<float*>(d_log_gates)[to] = static_cast<float*>(d_beta)[to] = 0.0f;
                     } else {
-                        static_cast<typename E::S*>(d_log_gates)[to] = static_cast<typename E::S*>(d_beta)[to] = E::put(0.0f);
+                        static_cast<ES*>(d_log_gates)[to] = static_cast<ES*>(d_beta)[to] = E::put(0.0f);
                     }
                 }
             }
     }
-    const BlockAt at = block_at(s, block);
-    if (at.length <= 0) return;
+    const BlockAt found = block_at(s, block);
+    if (found.length <= 0) return;
+    const int64_t row0 = uniform(found.row);
+    const int length = __builtin_amdgcn_readfirstlane(found.length);
 
-    Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
+    const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
     char* more = smem + 2 * Tile<NI, DK>::kBytes;
-    Tile<NI, kColumns> ot(more);
-    Tile<NS, kColumns> ut(more + Tile<NI, kColumns>::kBytes);
-    Tile<NS, kColumns> rt(more + Tile<NI, kColumns>::kBytes + Tile<NS, kColumns>::kBytes);
+    const Tile<NI, kColumns> ot(more);
+    const Tile<NS, kColumns> ut(more + Tile<NI, kColumns>::kBytes);
+    const Tile<NS, kColumns> rt(more + Tile<NI, kColumns>::kBytes + Tile<NS, kColumns>::kBytes);
+    // the products of tokens take the place of the three tiles once those are done with
+    Exchange<NS, kPairs> f_rows(more), l_rows(more + Exchange<NS, kPairs>::kBytes), f_cols(more + 2 * Exchange<NS, kPairs>::kBytes),
+        l_cols(more + 3 * Exchange<NS, kPairs>::kBytes);
 
-    for (int i = tid; i < kBlock * DK / 8; i += 256) {
-        const int row = i / (DK / 8), d = i % (DK / 8) * 8;
-        const bool there = row < at.length && d < s.dk;
-        const int64_t from = ((at.row + row) * s.key_heads + key_head) * s.dk + d;
-        kt.template put8<E>(row, d, load8<E>(k + from, there));
-        qt.template put8<E>(row, d, load8<E>(q + from, there));
+    constexpr uint32_t kSize = sizeof(ES);
+    const uint32_t k_step = s.key_heads * s.dk * kSize, v_step = s.heads * s.dv * kSize, r_step = s.heads * s.dv * 4;
+    const auto rows_of = [&](const void* p, uint32_t step, int64_t at_head, uint32_t bytes) {
+        return buffer_of(static_cast<const char*>(p) + row0 * step + at_head, (length - 1) * (int64_t)step + bytes);
+    };
+    {
+        const Buffer kb = rows_of(k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const Buffer qb = rows_of(q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) {
+            const int row = (tid + 512 * i) / (DK / 8), d = (tid + 512 * i) % (DK / 8) * 8;
+            const uint32_t from = d < s.dk ? row * k_step + d * kSize : kOutside;
+            const Eight<E> kv = fetch8<E>(kb, from), qv = fetch8<E>(qb, from);
+            kt.template put8<E>(row, d, kv);
+            qt.template put8<E>(row, d, qv);
+        }
     }
 
-    fx4 q_sum[DK / 16], k_sum[DK / 16];
+    // what comes from memory for 64 value columns of a head
+    const int feature0 = 16 * (wave % kFeatures), tile0 = wave / kFeatures * kTok;  // own features, first own tile of tokens
+    const int groups = (s.dv + kColumns - 1) / kColumns;
+    Eight<E> o_raw, v_raw;
+    Eight<ElemF32> u_raw, r_raw;
+    fx4 s_raw[2][2], d_raw[2][2];
+    const auto load = [&](int turn) {
+        const int head = key_head * share + turn / groups, col0 = turn % groups * kColumns;
+        const int64_t entry = block * s.heads + head, at_head = (int64_t)head * s.dv;
+        const int row = tid >> 3, d = col0 + (tid & 7) * 8;
+        const uint32_t from = d < s.dv ? row * v_step + d * kSize : kOutside, from_r = d < s.dv ? row * r_step + d * 4 : kOutside;
+        o_raw = fetch8<E>(d_out != nullptr ? rows_of(d_out, v_step, at_head * kSize, s.dv * kSize) : buffer_of(k, 0), from);
+        v_raw = fetch8<E>(rows_of(v, v_step, at_head * kSize, s.dv * kSize), from);
+        u_raw = fetch8<ElemF32>(rows_of(updates, r_step, at_head * 4, s.dv * 4), from_r);
+        r_raw = fetch8<ElemF32>(rows_of(d_rows, r_step, at_head * 4, s.dv * 4), from_r);
+        const int64_t cells = (int64_t)s.dk * s.dv;
+        const Buffer sb = buffer_of(states + entry * cells, cells * 4), db = buffer_of(d_states + entry * cells, cells * 4);
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t) q_sum[t] = k_sum[t] = fx4{0, 0, 0, 0};
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int e = col0 + 32 * i + 8 * g + 4 * h;
+                const uint32_t cell = e < s.dv ? ((feature0 + c) * s.dv + e) * 4 : kOutside;
+                s_raw[i][h] = fetch16(sb, cell);
+                d_raw[i][h] = fetch16(db, cell);
+            }
+    };
 
-    for (int h = 0; h < share; ++h) {
-        const int head = key_head * share + h;
+    fx4 q_sum[kTok], k_sum[kTok];
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) q_sum[t] = k_sum[t] = fx4{0, 0, 0, 0};
+    fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B of a head: own tokens, own features
+    // tile `own` of tokens against all: dO U^T (waves 0 to 3) or dR U^T (4 to 7), with the own tokens as columns and
+    // earlier tokens as rows, and with the own tokens as columns, where the other factor is U, and later tokens as rows
+    const int own = wave & 3;
+    const bool second = wave >= 4;
+    fx4 early[kTiles], late[kTiles];
+    float value_dot = 0.0f, whole_term = 0.0f;
+
+    load(0);
+    for (int turn = 0; turn < share * groups; ++turn) {
+        const int head = key_head * share + turn / groups;
         const int64_t entry = block * s.heads + head;
-        __syncthreads();
-        for (int i = tid; i < kGateFloats; i += 256) gate[i] = gates[entry * kGateFloats + i];
-        fx4 x[DK / 16], a[DK / 16], b[DK / 16];  // dQ, A and B of this head
-        // dO U^T and dR U^T: with the wave's tokens as columns (rows: earlier tokens) and as columns of later rows
-        fx4 oc[kTiles], rc[kTiles], orow[kTiles], rrow[kTiles];
-        fx4 rv = {0, 0, 0, 0};
-        float whole_term = 0.0f;
+        if (turn % groups == 0) {
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
+            for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) oc[t] = rc[t] = orow[t] = rrow[t] = fx4{0, 0, 0, 0};
-
-        for (int col0 = 0; col0 < s.dv; col0 += kColumns) {
-            __syncthreads();
-            for (int i = tid; i < kBlock * kColumns / 8; i += 256) {
-                const int row = i / (kColumns / 8), d = i % (kColumns / 8) * 8;
-                const bool there = row < at.length && col0 + d < s.dv;
-                const int64_t from = ((at.row + row) * s.heads + head) * s.dv + col0 + d;
-                ot.template put8<E>(row, d, load8<E>(d_out + from, there && d_out != nullptr));
-                ut.template put8<ElemF32>(row, d, load8<ElemF32>(updates + from, there));
-                rt.template put8<ElemF32>(row, d, load8<ElemF32>(d_rows + from, there));
+            for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
+            value_dot = whole_term = 0.0f;
+        }
+        lds_barrier();
+        if (turn % groups == 0 && tid < kGateFloats) gate[tid] = gates[entry * kGateFloats + tid];
+        {
+            const int row = tid >> 3, d = (tid & 7) * 8;
+            ot.template put8<E>(row, d, o_raw);
+            ut.template put8<ElemF32>(row, d, u_raw);
+            rt.template put8<ElemF32>(row, d, r_raw);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) value_dot += r_raw.v[i] * E::get(v_raw.v[i]);
+        }
+        Operand<NS> so[2], dd[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            so[i] = operand_of<NS>(s_raw[i][0], s_raw[i][1]);
+            dd[i] = operand_of<NS>(d_raw[i][0], d_raw[i][1]);
+            if (tile0 == 0) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) whole_term += s_raw[i][h][e] * d_raw[i][h][e];
             }
-            __syncthreads();
-            // dR . v of the wave's tokens: a token to a row of the accumulator, four columns to a lane
-            {
-                const int row = 16 * wave + c;
-                float sum = 0.0f;
-                if (row < at.length) {
-                    const int64_t from = ((at.row + row) * s.heads + head) * s.dv + col0;
+        }
+        lds_barrier();
+        if (turn + 1 < share * groups) load(turn + 1);
 #pragma unroll
-                    for (int d = 4 * g; d < kColumns; d += 16)
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (col0 + d < s.dv) sum += d_rows[from + d + r] * E::get(v[from + d + r]);
-                }
-                rv[0] += sum;
+            for (int t = 0; t < kTok; ++t) {
+                const int row = 16 * (tile0 + t) + c;
+                x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
+                a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
+                b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
             }
-#pragma unroll
-            for (int d = 0; d < kColumns; d += 32) {
-                const Operand<NI> o = ot.along(16 * wave + c, d, g);
-                const Operand<NS> u = ut.along(16 * wave + c, d, g), r = rt.along(16 * wave + c, d, g);
-#pragma unroll
-                for (int t = 0; t < DK / 16; ++t) {
-                    fx4 raw_s[2], raw_d[2];
-                    const Operand<NS> so = memory_operand<NS>(states + entry * s.dk * s.dv, s.dv, 16 * t + c, s.dk, col0 + d, s.dv, g, raw_s);
-                    const Operand<NS> dd = memory_operand<NS>(d_states + entry * s.dk * s.dv, s.dv, 16 * t + c, s.dk, col0 + d, s.dv, g, raw_d);
-                    x[t] = mma<NI, NS>(o, so, x[t]);
-                    a[t] = mma<NS, NS>(r, so, a[t]);
-                    b[t] = mma<NS, NS>(u, dd, b[t]);
-                    if (t % 4 == wave) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) whole_term += raw_s[i][e] * raw_d[i][e];
-                    }
-                }
+            const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
+            if (!second) {
+                const Operand<NI> o = ot.along(16 * own + c, 32 * i, g);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
-                    if (t <= wave) {
-                        const Operand<NS> e = ut.along(16 * t + c, d, g);
-                        oc[t] = mma<NS, NI>(e, o, oc[t]);
-                        rc[t] = mma<NS, NS>(e, r, rc[t]);
-                    }
-                    if (t >= wave) {
-                        orow[t] = mma<NI, NS>(ot.along(16 * t + c, d, g), u, orow[t]);
-                        rrow[t] = mma<NS, NS>(rt.along(16 * t + c, d, g), u, rrow[t]);
-                    }
+                    if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
+                    if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
+                }
+            } else {
+                const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
+                    if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
                 }
             }
         }
+        if (turn % groups != groups - 1) continue;
 
-        // factors of the parts that went through the state
-        const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * wave + 4 * g);
-        const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * wave + 4 * g);
-        const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * wave + 4 * g);
-        fx4 carried = {0, 0, 0, 0};
+        // all columns of the head are in: the products of tokens, weighted, to all waves
+        lds_barrier();
 #pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            const fx4 kv = kt.tile(16 * wave, 16 * t, lane);
+        for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int there = 16 * t + 4 * g + r, here = 16 * own + c;
+                const float far = (gate[kSumHigh * kBlock + here] - gate[kSumHigh * kBlock + there]) +
+                                  (gate[kSumLow * kBlock + here] - gate[kSumLow * kBlock + there]);
+                if (!second) {
+                    early[t][r] = there <= here ? s.scale * expf(far) * early[t][r] : 0.0f;
+                    late[t][r] = there >= here ? s.scale * expf(-far) * late[t][r] : 0.0f;
+                } else {
+                    early[t][r] = there < here ? -expf(far) * early[t][r] : 0.0f;
+                    late[t][r] = there > here ? -gate[kBeta * kBlock + there] * expf(-far) * late[t][r] : 0.0f;
+                }
+            }
+            const Exchange<NS, kPairs>&rows = second ? l_rows : f_rows, &cols = second ? l_cols : f_cols;
+            if (t <= (own | 1)) Exchange<NS, kPairs>(rows).put(2 * pair_lower(own, t >> 1) + (t & 1), lane, early[t]);
+            if (t >= (own & 2)) Exchange<NS, kPairs>(cols).put(2 * pair_upper(own, t >> 1) + (t & 1), lane, late[t]);
+        }
+        lds_barrier();
+        fx4 carried = {0, 0, 0, 0};
+        Operand<NI> ko[2], qo[2];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            ko[p] = kt.down(32 * p, feature0, lane);
+            qo[p] = qt.down(32 * p, feature0, lane);
+        }
+#pragma unroll
+        for (int t = 0; t < kTok; ++t) {
+            const int tile = tile0 + t;
+            // factors of the parts that went through the state
+            const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * tile + 4 * g);
+            const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * tile + 4 * g);
+            const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * tile + 4 * g);
+            const fx4 kv = kt.tile(16 * tile, feature0, lane), qv = qt.tile(16 * tile, feature0, lane);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[t][r] *= s.scale * since[r];
@@ -405,99 +470,81 @@ __global__ __launch_bounds__(256) void delta_gradients(
                 b[t][r] *= until[r];
                 carried[r] += kv[r] * b[t][r];
             }
-        }
-        whole_term *= gate[kSince * kBlock + kBlock - 1];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) whole_term += carried[r];
-
-        // weights of pairs of tokens inside the block
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+            for (int p = 0; p < 2; ++p) {
+                if (p <= (tile >> 1)) {
+                    x[t] = mma<NS, NI>(f_rows.get(pair_lower(tile, p), lane), ko[p], x[t]);
+                    a[t] = mma<NS, NI>(l_rows.get(pair_lower(tile, p), lane), ko[p], a[t]);
+                }
+                if (p >= (tile >> 1)) {
+                    b[t] = mma<NS, NI>(f_cols.get(pair_upper(tile, p), lane), qo[p], b[t]);
+                    b[t] = mma<NS, NI>(l_cols.get(pair_upper(tile, p), lane), ko[p], b[t]);
+                }
+            }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int there = 16 * t + 4 * g + r, here = 16 * wave + c;
-                const float high = gate[kSumHigh * kBlock + here] - gate[kSumHigh * kBlock + there];
-                const float low = gate[kSumLow * kBlock + here] - gate[kSumLow * kBlock + there];
-                const float ec = there <= here ? expf(high + low) : 0.0f;    // `there` earlier than the wave's token
-                const float er = there >= here ? expf(-(high + low)) : 0.0f; // `there` later
-                oc[t][r] = there <= here ? s.scale * ec * oc[t][r] : 0.0f;
-                rc[t][r] = there < here ? -ec * rc[t][r] : 0.0f;
-                orow[t][r] = there >= here ? s.scale * er * orow[t][r] : 0.0f;
-                rrow[t][r] = there > here ? -gate[kBeta * kBlock + there] * er * rrow[t][r] : 0.0f;
-            }
-        }
-        fx4 dots_q = {0, 0, 0, 0}, dots_a = {0, 0, 0, 0}, dots_b = {0, 0, 0, 0};
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const Operand<NS> o1 = operand_of<NS>(oc[2 * p], oc[2 * p + 1]), r1 = operand_of<NS>(rc[2 * p], rc[2 * p + 1]);
-            const Operand<NS> o2 = operand_of<NS>(orow[2 * p], orow[2 * p + 1]), r2 = operand_of<NS>(rrow[2 * p], rrow[2 * p + 1]);
-#pragma unroll
-            for (int t = 0; t < DK / 16; ++t) {
-                const Operand<NI> ko = kt.down(32 * p, 16 * t, lane), qo = qt.down(32 * p, 16 * t, lane);
-                x[t] = mma<NS, NI>(o1, ko, x[t]);
-                a[t] = mma<NS, NI>(r1, ko, a[t]);
-                b[t] = mma<NS, NI>(o2, qo, b[t]);
-                b[t] = mma<NS, NI>(r2, ko, b[t]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < DK / 16; ++t) {
-            const fx4 kv = kt.tile(16 * wave, 16 * t, lane), qv = qt.tile(16 * wave, 16 * t, lane);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                dots_q[r] += qv[r] * x[t][r];
-                dots_a[r] += kv[r] * a[t][r];
-                dots_b[r] += kv[r] * b[t][r];
+                const float dq = sum16(qv[r] * x[t][r]), da = sum16(kv[r] * a[t][r]), db = sum16(kv[r] * b[t][r]);
+                if (c == 0) {
+                    dots[wave][0][16 * t + 4 * g + r] = dq;
+                    dots[wave][1][16 * t + 4 * g + r] = da;
+                    dots[wave][2][16 * t + 4 * g + r] = db;
+                }
                 q_sum[t][r] += x[t][r];
                 k_sum[t][r] += beta[r] * a[t][r] + b[t][r];
             }
         }
-        const float dot_v = rv[0] + __shfl_xor(rv[0], 16);
-        const float token_v = dot_v + __shfl_xor(dot_v, 32);  // of token 16 wave + lane % 16
+        whole_term *= gate[kSince * kBlock + kBlock - 1];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float dq = sum16(dots_q[r]), da = sum16(dots_a[r]), dbb = sum16(dots_b[r]);
-            const float vr = __shfl(token_v, 4 * g + r);
-            if (c == 0) {
-                dc[16 * wave + 4 * g + r] = dq + beta[r] * da - dbb;
-                db[16 * wave + 4 * g + r] = vr + da;
-            }
-        }
+        for (int r = 0; r < 4; ++r) whole_term += carried[r];
         whole_term = sum16(whole_term);
         whole_term += __shfl_xor(whole_term, 16);
         whole_term += __shfl_xor(whole_term, 32);
         if (lane == 0) whole_terms[wave] = whole_term;
-        __syncthreads();
+        value_dot += __shfl_xor(value_dot, 1);
+        value_dot += __shfl_xor(value_dot, 2);
+        value_dot += __shfl_xor(value_dot, 4);
+        if ((tid & 7) == 0) value_dots[tid >> 3] = value_dot;
+        lds_barrier();
         if (wave == 0) {
-            float sum = dc[lane];
+            // token `lane`: over the tiles of features, then the sums from it on
+            float dq = 0.0f, da = 0.0f, db = 0.0f, whole = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kFeatures; ++i) {
+                const int w = lane / (16 * kTok) * kFeatures + i;
+                dq += dots[w][0][lane % (16 * kTok)];
+                da += dots[w][1][lane % (16 * kTok)];
+                db += dots[w][2][lane % (16 * kTok)];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) whole += whole_terms[i];
+            float sum = dq + gate[kBeta * kBlock + lane] * da - db;
 #pragma unroll
             for (int d = 1; d < 64; d *= 2) {
                 const float y = __shfl_down(sum, d);
                 if (lane + d < 64) sum += y;
             }
-            sum += whole_terms[0] + whole_terms[1] + whole_terms[2] + whole_terms[3];
-            if (lane < at.length) {
-                const int64_t to = (at.row + lane) * s.heads + head;
+            sum += whole;
+            if (lane < length) {
+                const int64_t to = (row0 + lane) * s.heads + head;
                 if (s.wide_gates) {
                     static_cast<float*>(d_log_gates)[to] = sum;
-                    static_cast<float*>(d_beta)[to] = db[lane];
+                    static_cast<float*>(d_beta)[to] = value_dots[lane] + da;
                 } else {
-                    static_cast<typename E::S*>(d_log_gates)[to] = E::put(sum);
-                    static_cast<typename E::S*>(d_beta)[to] = E::put(db[lane]);
+                    static_cast<ES*>(d_log_gates)[to] = E::put(sum);
+                    static_cast<ES*>(d_beta)[to] = E::put(value_dots[lane] + da);
                 }
             }
         }
     }
+    const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+    const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
 #pragma unroll
-    for (int t = 0; t < DK / 16; ++t)
+    for (int t = 0; t < kTok; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * wave + 4 * g + r, d = 16 * t + c;
-            if (row < at.length && d < s.dk) {
-                const int64_t to = ((at.row + row) * s.key_heads + key_head) * s.dk + d;
-                d_q[to] = E::put(q_sum[t][r]);
-                d_k[to] = E::put(k_sum[t][r]);
-            }
+            const uint32_t to = feature0 + c < s.dk ? (16 * (tile0 + t) + 4 * g + r) * k_step + (feature0 + c) * kSize : kOutside;
+            put1<E>(qb, to, q_sum[t][r]);
+            put1<E>(kb, to, k_sum[t][r]);
         }
 }
 

@@ -35,8 +35,8 @@ struct DeltaParts {
 };
 
 template <class... P, class... A>
-hipError_t delta_launch(void (*kernel)(P...), dim3 grid, size_t lds, hipStream_t stream, A... args) {
-    hipLaunchKernelGGL(kernel, grid, dim3(256), lds, stream, args...);
+hipError_t delta_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t lds, hipStream_t stream, A... args) {
+    hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, stream, args...);
     return hipGetLastError();
 }
 
@@ -44,7 +44,7 @@ template <class E, int NI, int NS, int DK>
 hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void* log_gates, const void* beta,
                    char* ws, const DeltaParts<NS>& at, bool upper, hipStream_t stream) {
     using S = typename E::S;
-    return delta_launch(delta_prepare<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.heads),
+    return delta_launch(delta_prepare<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
                         kPrepareBytes<E, NI, NS, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
                         log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p, upper);
 }
@@ -60,7 +60,7 @@ int delta_forward_dk(const DeltaForward& f) {
     }
     const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, DK, true> : delta_chain<E, NI, NS, DK, false>;
     return delta_status(delta_launch(
-        chain, dim3((unsigned)chain_grid(s)), kChainBytes<NI, NS, DK>, f.stream,
+        chain, dim3((unsigned)chain_grid(s)), 256, kChainBytes<NI, NS, DK>, f.stream,
         s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
         static_cast<S*>(f.out), f.final, f.states, f.updates));
@@ -78,12 +78,12 @@ int delta_backward_dk(const DeltaBackward& f) {
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), kReverseBytes<NI, NS, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 256, kReverseBytes<NI, NS, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows);
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
     return delta_status(delta_launch(
-        delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), kGradientBytes<NI, NS, DK>,
+        delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), 512, kGradientBytes<NI, NS, DK>,
         f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
         static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
         static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta));
@@ -92,7 +92,7 @@ int delta_backward_dk(const DeltaBackward& f) {
 template <class E, int Q, int N>
 int delta_step_rows(const DeltaStep& p) {
     const int groups = (p.dv + 4 * Q - 1) / (4 * Q);
-    return delta_status(delta_launch(delta_step<E, Q, N>, dim3((unsigned)(p.batch * p.heads * groups)), 0, p.stream, p, groups));
+    return delta_status(delta_launch(delta_step<E, Q, N>, dim3((unsigned)(p.batch * p.heads * groups)), 256, 0, p.stream, p, groups));
 }
 
 template <class E>
