@@ -112,8 +112,7 @@ _SIGNATURES = {
     "ascan_delta_blocks": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
     "ascan_delta_workspace_bytes": (
         ctypes.c_size_t,
-        [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
-         ctypes.c_int, ctypes.c_int, ctypes.c_int],
+        [ctypes.c_int64] * 6 + [ctypes.c_int, ctypes.c_int, ctypes.c_int],
     ),
     "ascan_delta_forward": (
         ctypes.c_int,
@@ -431,14 +430,13 @@ def _delta_sizes(q, v, log_gates, offsets):
 
 
 @functools.lru_cache(maxsize=1024)
-def _delta_workspace_bytes(rows, sequences, heads, dk, dv, code, packed, backward) -> int:
-    return (_lib or load()).ascan_delta_workspace_bytes(rows, sequences, heads, dk, dv, code, packed, backward)
+def _delta_workspace_bytes(rows, sequences, heads, key_heads, dk, dv, code, packed, backward) -> int:
+    return (_lib or load()).ascan_delta_workspace_bytes(rows, sequences, heads, key_heads, dk, dv, code, packed, backward)
 
 
 def _delta_workspace(sizes, code, packed, backward, device):
     """Scratch memory of a delta rule call; freed by the caching allocator in stream order after its kernels."""
-    rows, sequences, heads, _, dk, dv = sizes
-    nbytes = _delta_workspace_bytes(rows, sequences, heads, dk, dv, code, 1 if packed else 0, 1 if backward else 0)
+    nbytes = _delta_workspace_bytes(*sizes, code, 1 if packed else 0, 1 if backward else 0)
     return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
 

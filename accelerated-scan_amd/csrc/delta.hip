@@ -97,11 +97,11 @@ int64_t ascan_delta_blocks(int64_t rows, int64_t sequences, int packed) {
     return rows_ok(rows, sequences, packed != 0) ? delta_blocks(rows, sequences, packed != 0) : -1;
 }
 
-size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t dk, int64_t dv, int dtype,
-                                   int packed, int backward) {
-    if (element_bytes(dtype) == 0 || !heads_ok(heads, 1, dk, dv) || !rows_ok(rows, sequences, packed != 0)) return 0;
+size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t key_heads, int64_t dk,
+                                   int64_t dv, int dtype, int packed, int backward) {
+    if (element_bytes(dtype) == 0 || !heads_ok(heads, key_heads, dk, dv) || !rows_ok(rows, sequences, packed != 0)) return 0;
     static const int32_t some = 0;  // only whether there are offsets counts here
-    return workspace_of(shape_of(packed ? &some : nullptr, rows, sequences, heads, 1, dk, dv, 1.0f, 0), dtype, backward != 0);
+    return workspace_of(shape_of(packed ? &some : nullptr, rows, sequences, heads, key_heads, dk, dv, 1.0f, 0), dtype, backward != 0);
 }
 
 int ascan_delta_forward(const void* q, const void* k, const void* v, const void* log_gates, const void* beta,

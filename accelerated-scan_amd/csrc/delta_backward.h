@@ -261,7 +261,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
     const typename E::S* __restrict__ v, const typename E::S* __restrict__ d_out, const float* __restrict__ gates,
     const float* __restrict__ states, const float* __restrict__ updates, const float* __restrict__ d_states,
     const float* __restrict__ d_rows, typename E::S* __restrict__ d_q, typename E::S* __restrict__ d_k,
-    void* __restrict__ d_log_gates, void* __restrict__ d_beta) {
+    void* __restrict__ d_log_gates, void* __restrict__ d_beta, float* sums) {
     using ES = typename E::S;
     constexpr int kFeatures = DK / 16, kTok = DK / 32;  // tiles of features, and of tokens that a wave owns
     extern __shared__ __align__(16) char smem[];
@@ -324,109 +324,123 @@ __global__ __launch_bounds__(512) void delta_gradients(
         }
     }
 
-    // what comes from memory for 64 value columns of a head
     const int feature0 = 16 * (wave % kFeatures), tile0 = wave / kFeatures * kTok;  // own features, first own tile of tokens
     const int groups = (s.dv + kColumns - 1) / kColumns;
+    // what comes from memory for 64 value columns of a head
     Eight<E> o_raw, v_raw;
     Eight<ElemF32> u_raw, r_raw;
     fx4 s_raw[2][2], d_raw[2][2];
-    const auto load = [&](int turn) {
-        const int head = key_head * share + turn / groups, col0 = turn % groups * kColumns;
-        const int64_t entry = block * s.heads + head, at_head = (int64_t)head * s.dv;
-        const int row = tid >> 3, d = col0 + (tid & 7) * 8;
+    const auto load_rows = [&](int head, int group) {
+        const int64_t at_head = (int64_t)head * s.dv;
+        const int row = tid >> 3, d = group * kColumns + (tid & 7) * 8;
         const uint32_t from = d < s.dv ? row * v_step + d * kSize : kOutside, from_r = d < s.dv ? row * r_step + d * 4 : kOutside;
         o_raw = fetch8<E>(d_out != nullptr ? rows_of(d_out, v_step, at_head * kSize, s.dv * kSize) : buffer_of(k, 0), from);
         v_raw = fetch8<E>(rows_of(v, v_step, at_head * kSize, s.dv * kSize), from);
         u_raw = fetch8<ElemF32>(rows_of(updates, r_step, at_head * 4, s.dv * 4), from_r);
         r_raw = fetch8<ElemF32>(rows_of(d_rows, r_step, at_head * 4, s.dv * 4), from_r);
-        const int64_t cells = (int64_t)s.dk * s.dv;
+    };
+    const auto load_states = [&](int head, int group) {
+        const int64_t entry = block * s.heads + head, cells = (int64_t)s.dk * s.dv;
         const Buffer sb = buffer_of(states + entry * cells, cells * 4), db = buffer_of(d_states + entry * cells, cells * 4);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int e = col0 + 32 * i + 8 * g + 4 * h;
+                const int e = group * kColumns + 32 * i + 8 * g + 4 * h;
                 const uint32_t cell = e < s.dv ? ((feature0 + c) * s.dv + e) * 4 : kOutside;
                 s_raw[i][h] = fetch16(sb, cell);
                 d_raw[i][h] = fetch16(db, cell);
             }
     };
+    const auto stage_rows = [&]() {
+        const int row = tid >> 3, d = (tid & 7) * 8;
+        ot.template put8<E>(row, d, o_raw);
+        ut.template put8<ElemF32>(row, d, u_raw);
+        rt.template put8<ElemF32>(row, d, r_raw);
+    };
+    float* const mine = sums + (((block * s.key_heads + key_head) * 16 + wave) * kTok * 64 + lane) * 4;  // dK's half is 8 waves on
 
-    fx4 q_sum[kTok], k_sum[kTok];
-#pragma unroll
-    for (int t = 0; t < kTok; ++t) q_sum[t] = k_sum[t] = fx4{0, 0, 0, 0};
-    fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B of a head: own tokens, own features
-    // tile `own` of tokens against all: dO U^T (waves 0 to 3) or dR U^T (4 to 7), with the own tokens as columns and
-    // earlier tokens as rows, and with the own tokens as columns, where the other factor is U, and later tokens as rows
-    const int own = wave & 3;
-    const bool second = wave >= 4;
-    fx4 early[kTiles], late[kTiles];
-    float value_dot = 0.0f, whole_term = 0.0f;
-
-    load(0);
-    for (int turn = 0; turn < share * groups; ++turn) {
-        const int head = key_head * share + turn / groups;
+#pragma unroll 1
+    for (int head = key_head * share; head < (key_head + 1) * share; ++head) {
         const int64_t entry = block * s.heads + head;
-        if (turn % groups == 0) {
+        fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B of the head: own tokens, own features
+        float value_dot = 0.0f, whole_term = 0.0f;
 #pragma unroll
-            for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
-            value_dot = whole_term = 0.0f;
-        }
-        lds_barrier();
-        if (turn % groups == 0 && tid < kGateFloats) gate[tid] = gates[entry * kGateFloats + tid];
-        {
-            const int row = tid >> 3, d = (tid & 7) * 8;
-            ot.template put8<E>(row, d, o_raw);
-            ut.template put8<ElemF32>(row, d, u_raw);
-            rt.template put8<ElemF32>(row, d, r_raw);
+        for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
+        load_rows(head, 0);
+        load_states(head, 0);
+#pragma unroll 1
+        for (int group = 0; group < groups; ++group) {
+            lds_barrier();
+            if (group == 0 && tid < kGateFloats) gate[tid] = gates[entry * kGateFloats + tid];
+            stage_rows();
 #pragma unroll
             for (int i = 0; i < 8; ++i) value_dot += r_raw.v[i] * E::get(v_raw.v[i]);
-        }
-        Operand<NS> so[2], dd[2];
+            Operand<NS> so[2], dd[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            so[i] = operand_of<NS>(s_raw[i][0], s_raw[i][1]);
-            dd[i] = operand_of<NS>(d_raw[i][0], d_raw[i][1]);
-            if (tile0 == 0) {
+            for (int i = 0; i < 2; ++i) {
+                so[i] = operand_of<NS>(s_raw[i][0], s_raw[i][1]);
+                dd[i] = operand_of<NS>(d_raw[i][0], d_raw[i][1]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) whole_term += s_raw[i][h][e] * d_raw[i][h][e];
             }
-        }
-        lds_barrier();
-        if (turn + 1 < share * groups) load(turn + 1);
+            lds_barrier();
+            // (behind the last group the one before it, which the products of tokens take next)
+            const int next = group + 1 < groups ? group + 1 : (groups > 1 ? groups - 2 : 0);
+            load_rows(head, next);
+            load_states(head, next);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int t = 0; t < kTok; ++t) {
-                const int row = 16 * (tile0 + t) + c;
-                x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
-                a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
-                b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
-            }
-            const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
-            if (!second) {
-                const Operand<NI> o = ot.along(16 * own + c, 32 * i, g);
-#pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
-                    if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
+                for (int t = 0; t < kTok; ++t) {
+                    const int row = 16 * (tile0 + t) + c;
+                    __builtin_amdgcn_sched_barrier(0);
+                    x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
+                    a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
+                    b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
                 }
-            } else {
-                const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
+        }
+        // Tokens against tokens, from the last group of columns back: tile `own` against all in dO U^T (waves 0 to 3) or
+        // dR U^T (4 to 7), with the own tokens as columns and earlier ones as rows, and with the own tokens as columns,
+        // where the other factor is U, and later ones as rows.
+        const int own = wave & 3;
+        const bool second = wave >= 4;
+        fx4 early[kTiles], late[kTiles];
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) {
-                    if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
-                    if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
+        for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
+#pragma unroll 1
+        for (int group = groups - 1; group >= 0; --group) {
+            if (group < groups - 1) {
+                lds_barrier();
+                stage_rows();
+                lds_barrier();
+                load_rows(head, group > 0 ? group - 1 : 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                __builtin_amdgcn_sched_barrier(0);
+                const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
+                if (!second) {
+                    const Operand<NI> o = ot.along(16 * own + c, 32 * i, g);
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
+                        if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
+                    }
+                } else {
+                    const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
+                        if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
+                    }
                 }
             }
         }
-        if (turn % groups != groups - 1) continue;
 
-        // all columns of the head are in: the products of tokens, weighted, to all waves
+        // weighted, the products of tokens go to all waves
         lds_barrier();
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
@@ -458,6 +472,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
 #pragma unroll
         for (int t = 0; t < kTok; ++t) {
             const int tile = tile0 + t;
+            __builtin_amdgcn_sched_barrier(0);  // (a tile at a time: the registers of two would not fit)
             // factors of the parts that went through the state
             const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * tile + 4 * g);
             const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * tile + 4 * g);
@@ -489,11 +504,36 @@ __global__ __launch_bounds__(512) void delta_gradients(
                     dots[wave][1][16 * t + 4 * g + r] = da;
                     dots[wave][2][16 * t + 4 * g + r] = db;
                 }
-                q_sum[t][r] += x[t][r];
-                k_sum[t][r] += beta[r] * a[t][r] + b[t][r];
+                b[t][r] += beta[r] * a[t][r];  // dK
             }
         }
-        whole_term *= gate[kSince * kBlock + kBlock - 1];
+        // over the heads that share the keys: by way of memory, where this wave alone reads what it wrote
+        if (head > key_head * share) {
+#pragma unroll
+            for (int t = 0; t < kTok; ++t) {
+                x[t] += *reinterpret_cast<const fx4*>(mine + t * 256);
+                b[t] += *reinterpret_cast<const fx4*>(mine + (8 * kTok + t) * 256);
+            }
+        }
+        if (head + 1 < (key_head + 1) * share) {
+#pragma unroll
+            for (int t = 0; t < kTok; ++t) {
+                *reinterpret_cast<fx4*>(mine + t * 256) = x[t];
+                *reinterpret_cast<fx4*>(mine + (8 * kTok + t) * 256) = b[t];
+            }
+        } else {
+            const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+            const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+#pragma unroll
+            for (int t = 0; t < kTok; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t to = feature0 + c < s.dk ? (16 * (tile0 + t) + 4 * g + r) * k_step + (feature0 + c) * kSize : kOutside;
+                    put1<E>(qb, to, x[t][r]);
+                    put1<E>(kb, to, b[t][r]);
+                }
+        }
+        whole_term = tile0 == 0 ? whole_term * gate[kSince * kBlock + kBlock - 1] : 0.0f;  // a cell counts once
 #pragma unroll
         for (int r = 0; r < 4; ++r) whole_term += carried[r];
         whole_term = sum16(whole_term);
@@ -536,16 +576,6 @@ __global__ __launch_bounds__(512) void delta_gradients(
             }
         }
     }
-    const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-    const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-#pragma unroll
-    for (int t = 0; t < kTok; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t to = feature0 + c < s.dk ? (16 * (tile0 + t) + 4 * g + r) * k_step + (feature0 + c) * kSize : kOutside;
-            put1<E>(qb, to, q_sum[t][r]);
-            put1<E>(kb, to, k_sum[t][r]);
-        }
 }
 
 }  // namespace

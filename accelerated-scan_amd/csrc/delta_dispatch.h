@@ -19,10 +19,10 @@ inline int delta_status(hipError_t e) {
 inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 
 // The workspace's parts: table of the blocks' gates, T, P, and for the backward pass the state gradients
-// behind every block and the rows dR.
+// behind every block, the rows dR and sums over heads that share their keys.
 template <int NS>
 struct DeltaParts {
-    size_t gates, t, p, d_states, d_rows, end;
+    size_t gates, t, p, d_states, d_rows, sums, end;
     DeltaParts(const DeltaShape& s, bool backward) {
         const size_t entries = (size_t)s.blocks * s.heads;
         gates = 0;
@@ -30,7 +30,8 @@ struct DeltaParts {
         p = round_up(t + entries * kMatrixBytes<NS>);
         d_states = round_up(p + entries * kMatrixBytes<NS>);
         d_rows = round_up(d_states + (backward ? entries * s.dk * s.dv * 4 : 0));
-        end = round_up(d_rows + (backward ? (size_t)s.rows * s.heads * s.dv * 4 : 0));
+        sums = round_up(d_rows + (backward ? (size_t)s.rows * s.heads * s.dv * 4 : 0));
+        end = round_up(sums + (backward && s.heads > s.key_heads ? (size_t)s.blocks * s.key_heads * 2 * kBlock * (s.dk <= 64 ? 64 : 128) * 4 : 0));
     }
 };
 
@@ -86,7 +87,8 @@ int delta_backward_dk(const DeltaBackward& f) {
         delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), 512, kGradientBytes<NI, NS, DK>,
         f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
         static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
-        static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta));
+        static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta,
+        reinterpret_cast<float*>(ws + at.sums)));
 }
 
 template <class E, int Q, int N>

@@ -429,8 +429,8 @@ enum ascan_delta_flags {
 ASCAN_API int64_t ascan_delta_blocks(int64_t rows, int64_t sequences, int packed);
 
 /* Workspace of a call (backward: of ascan_delta_backward); 0 also for sizes that a call would refuse. */
-ASCAN_API size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t dk, int64_t dv,
-                                             int dtype, int packed, int backward);
+ASCAN_API size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t key_heads,
+                                             int64_t dk, int64_t dv, int dtype, int packed, int backward);
 
 ASCAN_API int ascan_delta_forward(const void* q, const void* k, const void* v, const void* log_gates, const void* beta,
                                   const float* initial, const void* offsets, void* out, float* final, float* states,
