@@ -450,11 +450,11 @@ __global__ __launch_bounds__(512) void delta_gradients(
                 const float far = (gate[kSumHigh * kBlock + here] - gate[kSumHigh * kBlock + there]) +
                                   (gate[kSumLow * kBlock + here] - gate[kSumLow * kBlock + there]);
                 if (!second) {
-                    early[t][r] = there <= here ? s.scale * expf(far) * early[t][r] : 0.0f;
-                    late[t][r] = there >= here ? s.scale * expf(-far) * late[t][r] : 0.0f;
+                    early[t][r] = there <= here ? s.scale * exp_of(far) * early[t][r] : 0.0f;
+                    late[t][r] = there >= here ? s.scale * exp_of(-far) * late[t][r] : 0.0f;
                 } else {
-                    early[t][r] = there < here ? -expf(far) * early[t][r] : 0.0f;
-                    late[t][r] = there > here ? -gate[kBeta * kBlock + there] * expf(-far) * late[t][r] : 0.0f;
+                    early[t][r] = there < here ? -exp_of(far) * early[t][r] : 0.0f;
+                    late[t][r] = there > here ? -gate[kBeta * kBlock + there] * exp_of(-far) * late[t][r] : 0.0f;
                 }
             }
             const Exchange<NS, kPairs>&rows = second ? l_rows : f_rows, &cols = second ? l_cols : f_cols;

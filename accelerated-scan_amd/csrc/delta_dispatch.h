@@ -46,7 +46,7 @@ hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void
                    char* ws, const DeltaParts<NS>& at, bool upper, hipStream_t stream) {
     using S = typename E::S;
     return delta_launch(delta_prepare<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
-                        kPrepareBytes<E, NI, NS, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
+                        kPrepareBytes<NI, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
                         log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p, upper);
 }
 

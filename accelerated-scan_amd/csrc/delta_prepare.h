@@ -72,10 +72,24 @@ __device__ __forceinline__ float load_gate(const DeltaShape& s, const void* p, i
     return s.wide_gates ? static_cast<const float*>(p)[i] : E::get(static_cast<const typename E::S*>(p)[i]);
 }
 
-template <class E, int NI, int NS, int DK>
-constexpr int kPrepareBytes = (2 * Tile<NI, DK>::kBytes > 3 * kBlock * 65 * 4 ? 2 * Tile<NI, DK>::kBytes : 3 * kBlock * 65 * 4);
+constexpr int kMatrixRow = kBlock + 4;  // floats from row to row of a matrix in LDS: 16-byte rows, banks apart
+template <int NI, int DK>
+constexpr int kPrepareBytes = 2 * Tile<NI, DK>::kBytes > 2 * kBlock * kMatrixRow * 4 ? 2 * Tile<NI, DK>::kBytes
+                                                                                    : 2 * kBlock * kMatrixRow * 4;
+
+// c + a * b for two 16 x 16 tiles, fp32: a given by its rows, b as an accumulator holds it.
+__device__ __forceinline__ fx4 tile_product(const fx4& a, const fx4& b, fx4 c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+    return c;
+}
 
 // grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.
+//
+// P leaves from the accumulators: the tile K_j Q_i^T has token i in a lane's column and its rows j along the depth, as
+// the operand wants it (Q_i K_j^T for the transpose).  The inverse of I + L is made by substitution inside the
+// diagonal's 16 x 16 tiles, which is exact to rounding whatever the keys are (a series in L is not: its
+// terms grow), and joined from there to 32 and to 64 with fp32 products.
 template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
                                                      const typename E::S* __restrict__ k,
@@ -83,146 +97,220 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
                                                      float* __restrict__ gates, char* __restrict__ t_out,
                                                      char* __restrict__ p_out, bool upper) {
     extern __shared__ __align__(16) char smem[];
-    __shared__ double sum[kBlock];
-    __shared__ float rate[kBlock];
+    __shared__ float high[kBlock], low[kBlock], rate[kBlock];
     const int64_t block = blockIdx.x;
     const int head = blockIdx.y, key_head = head / (s.heads / s.key_heads);
     const BlockAt at = block_at(s, block);
     if (at.length <= 0) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, c = lane & 15;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
 
-    Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
-    for (int i = tid; i < kBlock * DK / 8; i += 256) {
-        const int row = i / (DK / 8), col = i % (DK / 8) * 8;
-        const bool there = row < at.length && col < s.dk;
-        const int64_t from = ((at.row + row) * s.key_heads + key_head) * s.dk + col;
-        kt.template put8<E>(row, col, load8<E>(k + from, there));
-        qt.template put8<E>(row, col, load8<E>(q + from, there));
-    }
-    if (wave == 0) {
-        const bool there = lane < at.length;
-        const int64_t from = (at.row + lane) * s.heads + head;
-        const float b = there ? load_gate<E>(s, beta, from) : 0.0f;
-        double x = there ? gate_sum_term(load_gate<E>(s, log_gates, from)) : 0.0;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double y = __shfl_up(x, d);
-            if (lane >= d) x += y;
+    const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
+    {
+        constexpr uint32_t kSize = sizeof(typename E::S);
+        const int64_t row0 = uniform(at.row);
+        const int length = __builtin_amdgcn_readfirstlane(at.length);
+        const uint32_t step = s.key_heads * s.dk * kSize;
+        const int64_t from = row0 * step + (int64_t)key_head * s.dk * kSize, bytes = (length - 1) * (int64_t)step + s.dk * kSize;
+        const Buffer kb = buffer_of(reinterpret_cast<const char*>(k) + from, bytes);
+        const Buffer qb = buffer_of(reinterpret_cast<const char*>(q) + from, bytes);
+        float b = 0.0f, x = 0.0f;
+        if (wave == 0 && lane < length) {
+            b = load_gate<E>(s, beta, (row0 + lane) * s.heads + head);
+            x = load_gate<E>(s, log_gates, (row0 + lane) * s.heads + head);
         }
-        const double whole = __shfl(x, 63);
-        sum[lane] = x;
-        rate[lane] = b;
-        float* to = gates + (block * s.heads + head) * kGateFloats + lane;
-        const float since = expf((float)x), high = (float)x;
-        to[kBeta * kBlock] = b;
-        to[kBetaSince * kBlock] = b * since;
-        to[kSince * kBlock] = since;
-        to[kUntil * kBlock] = expf((float)(whole - x));
-        to[kSumHigh * kBlock] = high;
-        to[kSumLow * kBlock] = (float)(x - (double)high);
+        Eight<E> k_raw[DK / 32], q_raw[DK / 32];
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i) {
+            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
+            const uint32_t cell = d < s.dk ? row * step + d * kSize : kOutside;
+            k_raw[i] = fetch8<E>(kb, cell);
+            q_raw[i] = fetch8<E>(qb, cell);
+        }
+        if (wave == 0) {
+            double sum = gate_sum_term(x);  // (0 behind the last token, like its beta)
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const double y = __shfl_up(sum, d);
+                if (lane >= d) sum += y;
+            }
+            const double whole = __shfl(sum, 63);
+            float* to = gates + (block * s.heads + head) * kGateFloats + lane;
+            const float since = exp_of((float)sum), h = (float)sum, l = (float)(sum - (double)h);
+            high[lane] = h;
+            low[lane] = l;
+            rate[lane] = b;
+            to[kBeta * kBlock] = b;
+            to[kBetaSince * kBlock] = b * since;
+            to[kSince * kBlock] = since;
+            to[kUntil * kBlock] = exp_of((float)(whole - sum));
+            to[kSumHigh * kBlock] = h;
+            to[kSumLow * kBlock] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < DK / 32; ++i) {
+            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
+            kt.template put8<E>(row, d, k_raw[i]);
+            qt.template put8<E>(row, d, q_raw[i]);
+        }
     }
     __syncthreads();
 
-    fx4 kk[kTiles], qk[kTiles];
+    // kk: K_j K_i^T with i the own tile and j up to it.  pq: K_j Q_i^T, or with `upper` Q_i K_j^T for j the own tile and
+    // i from it on
+    fx4 kk[kTiles], pq[kTiles];
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) kk[j] = qk[j] = fx4{0, 0, 0, 0};
+    for (int j = 0; j < kTiles; ++j) kk[j] = pq[j] = fx4{0, 0, 0, 0};
+#pragma unroll
     for (int d = 0; d < DK; d += 32) {
-        const Operand<NI> a = kt.along(16 * wave + c, d, g), b = qt.along(16 * wave + c, d, g);
+        const Operand<NI> mine = kt.along(16 * wave + c, d, g), theirs = upper ? mine : qt.along(16 * wave + c, d, g);
 #pragma unroll
         for (int j = 0; j < kTiles; ++j) {
             if (j <= wave) {
                 const Operand<NI> o = kt.along(16 * j + c, d, g);
-                kk[j] = mma<NI, NI>(a, o, kk[j]);
-                qk[j] = mma<NI, NI>(b, o, qk[j]);
+                kk[j] = mma<NI, NI>(o, mine, kk[j]);
+                if (!upper) pq[j] = mma<NI, NI>(o, theirs, pq[j]);
             }
+            if (upper && j >= wave) pq[j] = mma<NI, NI>(qt.along(16 * j + c, d, g), theirs, pq[j]);
         }
     }
-    __syncthreads();  // the tiles' memory is taken over by the three matrices
+    const int here = 16 * wave + c;
+    const float high_here = high[here], low_here = low[here], rate_here = rate[here];
+    __syncthreads();  // the tiles' memory is taken over by L^T and the inverse
 
-    constexpr int kRow = 65;
-    float *lm = reinterpret_cast<float*>(smem), *xm = lm + kBlock * kRow, *pm = xm + kBlock * kRow;
+    float *lt = reinterpret_cast<float*>(smem), *xm = lt + kBlock * kMatrixRow;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j) {
+        const int row0 = 16 * j + 4 * g;
+        const fx4 h = *reinterpret_cast<const fx4*>(high + row0), l = *reinterpret_cast<const fx4*>(low + row0);
+        fx4 e;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * wave + 4 * g + r, col = 16 * j + c;
-            float l = 0.0f, p = 0.0f;
-            if (col <= row) {
-                const float e = expf((float)(sum[row] - sum[col]));
-                p = s.scale * e * qk[j][r];
-                if (col < row) l = rate[row] * e * kk[j][r];
+            const float far = (high_here - h[r]) + (low_here - l[r]);
+            e[r] = exp_of(j <= wave ? far : -far);  // (a tile on the diagonal needs its lower half only, or its upper)
+        }
+        if (j <= wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                lt[(row0 + r) * kMatrixRow + here] = row0 + r < here ? rate_here * e[r] * kk[j][r] : 0.0f;
+        }
+        if (upper && j == wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) e[r] = exp_of(-((high_here - h[r]) + (low_here - l[r])));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            pq[j][r] = (upper ? row0 + r >= here : row0 + r <= here) ? s.scale * e[r] * pq[j][r] : 0.0f;
+    }
+    {
+        char* to = p_out + (block * s.heads + head) * kMatrixBytes<NS>;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool there = upper ? h >= (wave >> 1) : h <= (wave >> 1);
+            if (there) {
+                const int i = (upper ? pair_upper(wave, h) : pair_lower(wave, h)) * 64 + lane;
+                const Operand<NS> o = operand_of<NS>(pq[2 * h], pq[2 * h + 1]);
+                if constexpr (NS == 0) {
+                    reinterpret_cast<fx4*>(to + i * 32)[0] = o.t[0];
+                    reinterpret_cast<fx4*>(to + i * 32)[1] = o.t[1];
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
+                }
             }
-            lm[row * kRow + col] = l;
-            pm[row * kRow + col] = p;
-            xm[row * kRow + col] = 0.0f;
         }
     }
-    __syncthreads();
-
-    // inverse of I + L: the diagonal's 16 x 16 tiles by substitution, a column to a lane (and its copies)
+    // (a wave's diagonal tile of L is its own work: no barrier before the substitution)
     {
         float x[16];
-        const float* l = lm + 16 * wave * (kRow + 1);
+        const float* l = lt + 16 * wave * (kMatrixRow + 1);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == c ? 1.0f : 0.0f;
+        for (int i = 0; i < 16; ++i) x[i] = i == c ? 1.0f : 0.0f;
 #pragma unroll
-            for (int j = 0; j < i; ++j) v -= l[i * kRow + j] * x[j];
-            x[i] = v;
+        for (int i = 0; i < 15; ++i) {
+            // row i of the column is final: off the rows below with it
+            float column[16];
+#pragma unroll
+            for (int n = (i + 1) / 4; n < 4; ++n) {
+                const fx4 part = *reinterpret_cast<const fx4*>(l + i * kMatrixRow + 4 * n);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) column[4 * n + r] = part[r];
+            }
+#pragma unroll
+            for (int n = i + 1; n < 16; ++n) x[n] = fmaf(-column[n], x[i], x[n]);
         }
         if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) xm[(16 * wave + i) * kRow + 16 * wave + c] = x[i];
+            for (int i = 0; i < 16; ++i) xm[(16 * wave + i) * kMatrixRow + here] = x[i];
+        }
+        if ((wave & 1) == 0) {  // the zero tile beside it that an operand spans
+#pragma unroll
+            for (int r = 0; r < 4; ++r) xm[(16 * wave + 4 * g + r) * kMatrixRow + here + 16] = 0.0f;
         }
     }
     __syncthreads();
-    // tile (i, j) of the inverse = -X(i, i) sum over k from j to i - 1 of L(i, k) X(k, j), one distance i - j at a time
+    const auto l_rows = [&](int i, int n) {  // tile (i, n) of L by its rows
+        fx4 o;
 #pragma unroll
-    for (int d = 1; d < kTiles; ++d) {
-        const int j = wave, i = wave + d;
-        if (i < kTiles) {
-            fx4 acc = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-            for (int n = j; n < i; ++n) {
+        for (int r = 0; r < 4; ++r) o[r] = lt[(16 * n + 4 * g + r) * kMatrixRow + 16 * i + c];
+        return o;
+    };
+    const auto x_rows = [&](int i, int n) { return *reinterpret_cast<const fx4*>(xm + (16 * i + c) * kMatrixRow + 16 * n + 4 * g); };
+    const auto x_tile = [&](int i, int n) {
+        fx4 o;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(lm[(16 * i + c) * kRow + 16 * n + 4 * g + r],
-                                                               xm[(16 * n + 4 * g + r) * kRow + 16 * j + c], acc, 0, 0, 0);
-            }
+        for (int r = 0; r < 4; ++r) o[r] = xm[(16 * i + 4 * g + r) * kMatrixRow + 16 * n + c];
+        return o;
+    };
+    const auto put_tile = [&](int i, int n, const fx4& o, float sign) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                y = __builtin_amdgcn_mfma_f32_16x16x4f32(xm[(16 * i + c) * kRow + 16 * i + 4 * g + r], acc[r], y, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) xm[(16 * i + 4 * g + r) * kRow + 16 * j + c] = -y[r];
-        }
-        __syncthreads();
+        for (int r = 0; r < 4; ++r) xm[(16 * i + 4 * g + r) * kMatrixRow + 16 * n + c] = sign * o[r];
+    };
+    const fx4 zero = {0, 0, 0, 0};
+    if (wave < 2) {  // tiles (1, 0) and (3, 2)
+        const int n = 2 * wave;
+        put_tile(n + 1, n, tile_product(x_rows(n + 1, n + 1), tile_product(l_rows(n + 1, n), x_tile(n, n), zero), zero), -1.0f);
     }
+    __syncthreads();
+    {
+        // the lower left quarter: -X(2..3, 2..3) M, M = L(2..3, 0..1) X(0..1, 0..1), a tile to a wave; M waits in the
+        // upper right quarter, which nobody reads
+        const int i = 2 + (wave >> 1), j = wave & 1;
+        fx4 m = tile_product(l_rows(i, 1), x_tile(1, j), zero);
+        if (j == 0) m = tile_product(l_rows(i, 0), x_tile(0, 0), m);
+        put_tile(i - 2, j + 2, m, 1.0f);
+        __syncthreads();
+        fx4 y = tile_product(x_rows(i, 2), x_tile(0, j + 2), zero);
+        if (i == 3) y = tile_product(x_rows(3, 3), x_tile(1, j + 2), y);
+        put_tile(i, j, y, -1.0f);
+    }
+    __syncthreads();
 
-    char* t_to = t_out + (block * s.heads + head) * kMatrixBytes<NS>;
-    char* p_to = p_out + (block * s.heads + head) * kMatrixBytes<NS>;
+    char* to = t_out + (block * s.heads + head) * kMatrixBytes<NS>;
     for (int i = tid; i < kPairs * 64; i += 256) {
         const int pair = i >> 6;
         const int m = upper ? (pair < 4 ? pair >> 1 : pair - 2) : (pair < 2 ? pair : (pair + 2) >> 1);
         const int h = upper ? (pair < 4 ? pair & 1 : 1) : (pair < 2 ? 0 : pair & 1);
-        const int row = 16 * m + c;
-        float t[8], p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int col = 32 * h + 4 * g + (e & 3) + (e & 4) * 4;
-            const int from = upper ? col * kRow + row : row * kRow + col;
-            t[e] = xm[from] - (row == col ? 1.0f : 0.0f);
-            p[e] = pm[from];
-        }
-        if constexpr (NS == 0) {
-            __builtin_memcpy(t_to + i * 32, t, 32);
-            __builtin_memcpy(p_to + i * 32, p, 32);
+        const int row = 16 * m + c, col = 32 * h + 4 * g;
+        fx4 a, b;
+        if (upper) {
+            a = x_tile(2 * h, m);
+            b = x_tile(2 * h + 1, m);
         } else {
-            const Operand<NS> to = operand_of<NS>(fx4{t[0], t[1], t[2], t[3]}, fx4{t[4], t[5], t[6], t[7]});
-            const Operand<NS> po = operand_of<NS>(fx4{p[0], p[1], p[2], p[3]}, fx4{p[4], p[5], p[6], p[7]});
+            a = x_rows(m, 2 * h);
+            b = x_rows(m, 2 * h + 1);
+        }
 #pragma unroll
-            for (int n = 0; n < NS; ++n) {
-                *reinterpret_cast<bx8*>(t_to + (n * kPairs * 64 + i) * 16) = to.p[n];
-                *reinterpret_cast<bx8*>(p_to + (n * kPairs * 64 + i) * 16) = po.p[n];
-            }
+        for (int r = 0; r < 4; ++r) {
+            a[r] -= row == col + r ? 1.0f : 0.0f;
+            b[r] -= row == col + 16 + r ? 1.0f : 0.0f;
+        }
+        const Operand<NS> o = operand_of<NS>(a, b);
+        if constexpr (NS == 0) {
+            reinterpret_cast<fx4*>(to + i * 32)[0] = o.t[0];
+            reinterpret_cast<fx4*>(to + i * 32)[1] = o.t[1];
+        } else {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
         }
     }
 }

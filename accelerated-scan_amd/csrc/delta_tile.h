@@ -435,13 +435,28 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Sum over the 16 lanes that share lane / 16.
+// Sum over the 16 lanes that share lane / 16, to all of them: rotations within the row of lanes.
+template <int N>
+__device__ __forceinline__ float rotated(float x) {
+    const int i = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x120 + N, 0xf, 0xf, false));
+}
 __device__ __forceinline__ float sum16(float x) {
-    x += __shfl_xor(x, 1);
-    x += __shfl_xor(x, 2);
-    x += __shfl_xor(x, 4);
-    x += __shfl_xor(x, 8);
+    x += rotated<8>(x);
+    x += rotated<4>(x);
+    x += rotated<2>(x);
+    x += rotated<1>(x);
     return x;
+}
+
+// e^x to 2^-22 of its value: 2^(x log2 e) from the hardware, with the product's rounding error put back.
+__device__ __forceinline__ float exp_of(float x) {
+    constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f;  // log2 e
+    x = fmaxf(x, -200.0f);  // (0 from there on, and -inf has no product with a rounding error)
+    const float t = x * kHigh;
+    const float rest = fmaf(x, kHigh, -t) + x * kLow;
+    const float p = __builtin_amdgcn_exp2f(t);
+    return fmaf(p, rest * 0.693147182f, p);
 }
 
 }  // namespace
