@@ -45,9 +45,10 @@ template <class E, int NI, int NS, int DK>
 hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void* log_gates, const void* beta,
                    char* ws, const DeltaParts<NS>& at, bool upper, hipStream_t stream) {
     using S = typename E::S;
-    return delta_launch(delta_prepare<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
+    const auto kernel = upper ? delta_prepare<E, NI, NS, DK, true> : delta_prepare<E, NI, NS, DK, false>;
+    return delta_launch(kernel, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
                         kPrepareBytes<NI, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
-                        log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p, upper);
+                        log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p);
 }
 
 template <class E, int NI, int NS, int DK>

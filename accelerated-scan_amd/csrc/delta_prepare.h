@@ -44,7 +44,7 @@ __device__ __forceinline__ SequenceAt sequence_at(const DeltaShape& s, int64_t n
 __device__ __forceinline__ BlockAt block_at(const DeltaShape& s, int64_t block) {
     int64_t n;
     if (s.offsets == nullptr) {
-        n = block / ((s.tokens + kBlock - 1) / kBlock);
+        n = (uint32_t)block / (uint32_t)((s.tokens + kBlock - 1) / kBlock);  // (both below 2^31)
     } else {
         // first entries ascend with the sequence: count those at or before this one
         const int lane = threadIdx.x & 63;
@@ -84,18 +84,41 @@ __device__ __forceinline__ fx4 tile_product(const fx4& a, const fx4& b, fx4 c) {
     return c;
 }
 
+// Sums over the lanes of a wave up to each, 64 bits wide: shifts within rows of 16 lanes, then rows onto later rows.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double x) {
+    const uint64_t w = __builtin_bit_cast(uint64_t, x);
+    const uint32_t a = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)w, CTRL, ROWS, 0xf, false);
+    const uint32_t b = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(w >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)b << 32 | a);
+}
+__device__ __forceinline__ double wave_prefix(double x) {
+    x += moved<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: 0 where there is no lane
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);  // row_bcast 15 to rows 1 and 3
+    x += moved<0x143, 0xc>(x);  // row_bcast 31 to rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ double last_lane(double x) {
+    const uint64_t w = __builtin_bit_cast(uint64_t, x);
+    const uint32_t a = __builtin_amdgcn_readlane((int)(uint32_t)w, 63), b = __builtin_amdgcn_readlane((int)(uint32_t)(w >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t)b << 32 | a);
+}
+
 // grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.
 //
 // P leaves from the accumulators: the tile K_j Q_i^T has token i in a lane's column and its rows j along the depth, as
 // the operand wants it (Q_i K_j^T for the transpose).  The inverse of I + L is made by substitution inside the
 // diagonal's 16 x 16 tiles, which is exact to rounding whatever the keys are (a series in L is not: its
 // terms grow), and joined from there to 32 and to 64 with fp32 products.
-template <class E, int NI, int NS, int DK>
-__global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
+template <class E, int NI, int NS, int DK, bool upper>
+__global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
                                                      const typename E::S* __restrict__ k,
                                                      const void* __restrict__ log_gates, const void* __restrict__ beta,
                                                      float* __restrict__ gates, char* __restrict__ t_out,
-                                                     char* __restrict__ p_out, bool upper) {
+                                                     char* __restrict__ p_out) {
     extern __shared__ __align__(16) char smem[];
     __shared__ float high[kBlock], low[kBlock], rate[kBlock];
     const int64_t block = blockIdx.x;
@@ -105,6 +128,7 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
 
     const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
+    float b = 0.0f, x = 0.0f;
     {
         constexpr uint32_t kSize = sizeof(typename E::S);
         const int64_t row0 = uniform(at.row);
@@ -113,7 +137,6 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
         const int64_t from = row0 * step + (int64_t)key_head * s.dk * kSize, bytes = (length - 1) * (int64_t)step + s.dk * kSize;
         const Buffer kb = buffer_of(reinterpret_cast<const char*>(k) + from, bytes);
         const Buffer qb = buffer_of(reinterpret_cast<const char*>(q) + from, bytes);
-        float b = 0.0f, x = 0.0f;
         if (wave == 0 && lane < length) {
             b = load_gate<E>(s, beta, (row0 + lane) * s.heads + head);
             x = load_gate<E>(s, log_gates, (row0 + lane) * s.heads + head);
@@ -126,26 +149,6 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
             k_raw[i] = fetch8<E>(kb, cell);
             q_raw[i] = fetch8<E>(qb, cell);
         }
-        if (wave == 0) {
-            double sum = gate_sum_term(x);  // (0 behind the last token, like its beta)
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const double y = __shfl_up(sum, d);
-                if (lane >= d) sum += y;
-            }
-            const double whole = __shfl(sum, 63);
-            float* to = gates + (block * s.heads + head) * kGateFloats + lane;
-            const float since = exp_of((float)sum), h = (float)sum, l = (float)(sum - (double)h);
-            high[lane] = h;
-            low[lane] = l;
-            rate[lane] = b;
-            to[kBeta * kBlock] = b;
-            to[kBetaSince * kBlock] = b * since;
-            to[kSince * kBlock] = since;
-            to[kUntil * kBlock] = exp_of((float)(whole - sum));
-            to[kSumHigh * kBlock] = h;
-            to[kSumLow * kBlock] = l;
-        }
 #pragma unroll
         for (int i = 0; i < DK / 32; ++i) {
             const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
@@ -154,6 +157,22 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
         }
     }
     __syncthreads();
+    if (wave == 0) {
+        double sum = gate_sum_term(x);  // (0 behind the last token, like its beta)
+        sum = wave_prefix(sum);
+        const double whole = last_lane(sum);
+        float* to = gates + (block * s.heads + head) * kGateFloats + lane;
+        const float since = exp_of((float)sum), h = (float)sum, l = (float)(sum - (double)h);
+        high[lane] = h;
+        low[lane] = l;
+        rate[lane] = b;
+        to[kBeta * kBlock] = b;
+        to[kBetaSince * kBlock] = b * since;
+        to[kSince * kBlock] = since;
+        to[kUntil * kBlock] = exp_of((float)(whole - sum));
+        to[kSumHigh * kBlock] = h;
+        to[kSumLow * kBlock] = l;
+    }
 
     // kk: K_j K_i^T with i the own tile and j up to it.  pq: K_j Q_i^T, or with `upper` Q_i K_j^T for j the own tile and
     // i from it on
@@ -174,8 +193,8 @@ __global__ __launch_bounds__(256) void delta_prepare(DeltaShape s, const typenam
         }
     }
     const int here = 16 * wave + c;
-    const float high_here = high[here], low_here = low[here], rate_here = rate[here];
     __syncthreads();  // the tiles' memory is taken over by L^T and the inverse
+    const float high_here = high[here], low_here = low[here], rate_here = rate[here];
 
     float *lt = reinterpret_cast<float*>(smem), *xm = lt + kBlock * kMatrixRow;
 #pragma unroll
