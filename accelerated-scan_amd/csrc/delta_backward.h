@@ -28,7 +28,7 @@ constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + 
 // dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.
 // grid chain_grid(), 256 threads.
 template <class E, int NI, int NS, int DK>
-__global__ __launch_bounds__(256) void delta_reverse_chain(
+__global__ __launch_bounds__(256, 2) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
     const char* __restrict__ p_in, const float* __restrict__ d_final, typename E::S* __restrict__ d_v,
@@ -152,12 +152,16 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
             fx4 po = {0, 0, 0, 0};
             if (wave < 2) po = mma<NS, NI>(pm[0], o_low, po);
             po = mma<NS, NI>(pm[1], o_high, po);
+            fx4 u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
 #pragma unroll
-            for (int d = 0; d < kDepths; ++d) u = mma<NI, NS>(ko[d], so[d], u);
+            for (int d = 0; d < kDepths; d += 2) {
+                u = mma<NI, NS>(ko[d], so[d], u);
+                u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
+            }
             load_matrix(p_in, ahead, pm);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                u[r] = until[r] * u[r] + po[r];
+                u[r] = until[r] * (u[r] + u2[r]) + po[r];
                 w[r] *= s.scale * since[r];
             }
         }
@@ -178,8 +182,12 @@ __global__ __launch_bounds__(256) void delta_reverse_chain(
                 q_high[t] = qt.down_features(32, kOwn * wave + t, lane);
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (wave < 2) u = mma<NS, NS>(tm[0], low, u);
             u = mma<NS, NS>(tm[1], high, u);
+            if (wave < 2) {
+                const fx4 more = mma<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] += more[r];
+            }
 #pragma unroll
             for (int t = 0; t < kOwn; ++t) {
 #pragma unroll

@@ -34,7 +34,7 @@ constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + Ex
 
 // grid chain_grid(), 256 threads.  KEEP: write the states in front of the blocks and the rows U.
 template <class E, int NI, int NS, int DK, bool KEEP>
-__global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
+__global__ __launch_bounds__(256, 2) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
                                                    const typename E::S* __restrict__ v,
                                                    const float* __restrict__ gates, const char* __restrict__ t_in,
@@ -129,7 +129,11 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r] *= f;
         o = mma<NS, NS>(low, pm[0], o);
-        if (wave >= 2) o = mma<NS, NS>(high, pm[1], o);
+        if (wave >= 2) {
+            const fx4 more = mma<NS, NS>(high, pm[1], fx4{0, 0, 0, 0});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] += more[r];
+        }
         const int d = col0 + 4 * g;
         const Buffer to = rows_of(out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
         put4<E>(to, d < s.dv ? token * v_step + d * kSize : kOutside, o);
@@ -166,16 +170,19 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
         fx4 x = vt.tile(16 * wave, 0, lane);
         load_kv(ahead);
         __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
-        fx4 u = {0, 0, 0, 0};
+        fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
 #pragma unroll
-        for (int d = 0; d < kDepths; ++d) u = mma<NI, NS>(ko[d], so[d], u);
+        for (int d = 0; d < kDepths; d += 2) {
+            u = mma<NI, NS>(ko[d], so[d], u);
+            u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
+        }
         if (first > 0) finish(first - kBlock, u_low, u_high);
         const Buffer here = gates_of(first);
         load_matrix(p_in, first, pm);
         since = fetch4(here, kSince * 256 + token * 4);
         // R = diag(beta) V - diag(beta e^c) K S0
 #pragma unroll
-        for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * u[r];
+        for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * (u[r] + u2[r]);
         xr.put(wave, lane, u);
         beta = fetch16(gb, kBeta * 256 + gate_rows);
         beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
@@ -189,7 +196,11 @@ __global__ __launch_bounds__(256) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
             for (int d = 0; d < kDepths; ++d) o = mma<NS, NI>(so[d], operand_from<NI, E>(q_raw[d]), o);
             u = mma<NS, NS>(tm[0], low, u);
-            if (wave >= 2) u = mma<NS, NS>(tm[1], high, u);
+            if (wave >= 2) {
+                u2 = mma<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] += u2[r];
+            }
         }
         load_q(ahead);
         load_matrix(t_in, ahead, tm);

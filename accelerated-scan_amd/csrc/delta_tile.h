@@ -331,12 +331,15 @@ struct Tile {
     }
     // The 16 x 16 tile at (row0, col0) in the accumulator's layout.
     __device__ __forceinline__ fx4 tile(int row0, int col0, int lane) const {
-        fx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        fx4 x;
 #pragma unroll
         for (int i = P - 1; i >= 0; --i) {
-            const bx4 a = column4(i, row0, col0, lane);
+            const uint64_t w = __builtin_bit_cast(uint64_t, column4(i, row0, col0, lane));
+            const uint32_t a = (uint32_t)w, b = (uint32_t)(w >> 32);
+            const fx4 part = {__builtin_bit_cast(float, a << 16), __builtin_bit_cast(float, a & 0xffff0000u),
+                              __builtin_bit_cast(float, b << 16), __builtin_bit_cast(float, b & 0xffff0000u)};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] += (float)a[r];
+            for (int r = 0; r < 4; ++r) x[r] = i == P - 1 ? part[r] : x[r] + part[r];
         }
         return x;
     }
