@@ -266,21 +266,29 @@ __device__ __forceinline__ void store4(typename E::S* p, const fx4& x) {
 __device__ __forceinline__ constexpr int feature_row(int t, int g, int r) { return 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r; }
 
 // ---------------------------------------------------------------------------
-// 64 rows of W values in LDS, as fp32 (P = 0) or as P planes of bfloat16 parts.  Rows are padded by
-// 16 bytes so that the 16 rows of an operand start in different banks.
+// 64 rows of W values in LDS, as fp32 (P = 0, rows padded by 16 bytes) or as P planes of bfloat16 parts.  The planes'
+// rows have no padding; their 16-byte pieces change places instead, so that neither the 16 rows of an operand (a piece of
+// each) nor the four rows of a transposing read (four pieces of each, every one 16 or 32 bytes on) meet in a bank.
 // ---------------------------------------------------------------------------
 template <int P, int W>
 struct Tile {
-    static constexpr int kStride = W + 8;
+    static constexpr int kStride = W < 64 ? W + 8 : W;
     static constexpr int kPlane = kBlock * kStride;
     static constexpr int kBytes = P * kPlane * 2;
     __bf16* base;
+
+    // Where element (row, col) stands; columns col .. col+7 stay together for col a multiple of 8.
+    static __device__ __forceinline__ int place(int row, int col) {
+        if constexpr (W < 64) return row * kStride + col;
+        const int turn = W >= 128 ? (row & 3) * 4 + ((row >> 2) & 3) : (row & 2) * 2 + ((row >> 2) & 3);
+        return row * kStride + (col ^ (turn * 8));
+    }
 
     __device__ __forceinline__ explicit Tile(void* p) : base(static_cast<__bf16*>(p)) {}
 
     template <class E>
     __device__ __forceinline__ void put8(int row, int col, const Eight<E>& x) const {
-        __bf16* at = base + row * kStride + col;
+        __bf16* at = base + place(row, col);
         if constexpr (P == 1 && sizeof(typename E::S) == 2) {
             fx4 v;
             __builtin_memcpy(&v, x.v, 16);
@@ -295,7 +303,7 @@ struct Tile {
     __device__ __forceinline__ Operand<P> along(int row, int k0, int g) const {
         Operand<P> o;
 #pragma unroll
-        for (int i = 0; i < P; ++i) o.p[i] = *reinterpret_cast<const bx8*>(base + i * kPlane + row * kStride + k0 + 8 * g);
+        for (int i = 0; i < P; ++i) o.p[i] = *reinterpret_cast<const bx8*>(base + i * kPlane + place(row, k0 + 8 * g));
         return o;
     }
     // Depths row0 .. row0+31 (tokens) of the features of state tile t, in the order of feature_row().
@@ -304,7 +312,7 @@ struct Tile {
         Operand<P> o;
 #pragma unroll
         for (int n = 0; n < P; ++n) {
-            __bf16* at = base + n * kPlane + (row0 + 4 * g + (i >> 2)) * kStride + feature_row(t, i & 3, 0);
+            __bf16* at = base + n * kPlane + place(row0 + 4 * g + (i >> 2), feature_row(t, i & 3, 0));
             const sx4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)at);
             const sx4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)(at + 16 * kStride));
             o.p[n] = __builtin_shufflevector(__builtin_bit_cast(bx4, a), __builtin_bit_cast(bx4, b), 0, 1, 2, 3, 4, 5, 6, 7);
@@ -315,7 +323,7 @@ struct Tile {
     // fetch four rows of 16 columns and receive a column each.
     __device__ __forceinline__ bx4 column4(int plane, int row0, int col0, int lane) const {
         const int g = lane >> 4, i = lane & 15;
-        __bf16* at = base + plane * kPlane + (row0 + 4 * g + (i >> 2)) * kStride + col0 + (i & 3) * 4;
+        __bf16* at = base + plane * kPlane + place(row0 + 4 * g + (i >> 2), col0 + (i & 3) * 4);
         const sx4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)at);
         return __builtin_bit_cast(bx4, v);
     }
