@@ -26,7 +26,7 @@ constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + 
 
 // The chain, last block first, divided like the forward one: 16 columns of D to a workgroup, wave w keeps rows
 // dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.
-// grid chain_grid(), 256 threads.
+// q and k: the copies that delta_prepare made.  grid chain_grid(), 256 threads.
 template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(256, 2) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(256, 2) void delta_reverse_chain(
         }
 
     constexpr uint32_t kSize = sizeof(ES);
-    const uint32_t k_step = s.key_heads * s.dk * kSize, v_step = s.heads * s.dv * kSize, r_step = s.heads * s.dv * 4;
+    const uint32_t v_step = s.heads * s.dv * kSize, r_step = s.heads * s.dv * 4;
     const int64_t seq_row = uniform(at.row), seq_length = uniform(at.length), seq_block = uniform(at.block);
     const int token = 16 * wave + c;
     const auto rows_of = [&](const void* p, int64_t first, uint32_t step, int64_t at_head, uint32_t bytes) {
@@ -79,14 +79,13 @@ __global__ __launch_bounds__(256, 2) void delta_reverse_chain(
     fx4 beta, beta_since, until, since;
     float whole;
     const auto load_rows = [&](int64_t first) {
-        const Buffer kb = rows_of(k, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-        const Buffer qb = rows_of(q, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const int64_t copy = ((seq_block + first / kBlock) * s.key_heads + key_head) * kBlock * DK;
+        const Buffer kb = buffer_of(k + copy, kBlock * DK * kSize), qb = buffer_of(q + copy, kBlock * DK * kSize);
         const Buffer ob = d_out != nullptr ? rows_of(d_out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize) : buffer_of(k, 0);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
-            k_raw[i] = fetch8<E>(kb, d < s.dk ? row * k_step + d * kSize : kOutside);
-            q_raw[i] = fetch8<E>(qb, d < s.dk ? row * k_step + d * kSize : kOutside);
+            k_raw[i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
+            q_raw[i] = fetch8<E>(qb, (tid + 256 * i) * 8 * kSize);
         }
         const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
         o_raw = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
@@ -262,7 +261,7 @@ constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS
 // tokens with tokens are divided among the waves by tiles and go round through LDS.  What bounds it are the two fp32
 // states per block, 8 bytes per cell against 2 for an input; the next 64 value columns are requested while these are
 // computed.
-// grid (blocks, key heads), 512 threads.
+// q and k: the copies that delta_prepare made.  grid (blocks, key heads), 512 threads.
 template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(512) void delta_gradients(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
@@ -320,12 +319,12 @@ __global__ __launch_bounds__(512) void delta_gradients(
         return buffer_of(static_cast<const char*>(p) + row0 * step + at_head, (length - 1) * (int64_t)step + bytes);
     };
     {
-        const Buffer kb = rows_of(k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-        const Buffer qb = rows_of(q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+        const int64_t copy = (block * s.key_heads + key_head) * kBlock * DK;
+        const Buffer kb = buffer_of(k + copy, kBlock * DK * kSize), qb = buffer_of(q + copy, kBlock * DK * kSize);
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) {
             const int row = (tid + 512 * i) / (DK / 8), d = (tid + 512 * i) % (DK / 8) * 8;
-            const uint32_t from = d < s.dk ? row * k_step + d * kSize : kOutside;
+            const uint32_t from = (tid + 512 * i) * 8 * kSize;
             const Eight<E> kv = fetch8<E>(kb, from), qv = fetch8<E>(qb, from);
             kt.template put8<E>(row, d, kv);
             qt.template put8<E>(row, d, qv);

@@ -18,17 +18,20 @@ inline int delta_status(hipError_t e) {
 
 inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 
-// The workspace's parts: table of the blocks' gates, T, P, and for the backward pass the state gradients
-// behind every block, the rows dR and sums over heads that share their keys.
+// The workspace's parts: table of the blocks' gates, T, P, copies of keys and queries, and for the backward
+// pass the state gradients behind every block, the rows dR and sums over heads that share their keys.
 template <int NS>
 struct DeltaParts {
-    size_t gates, t, p, d_states, d_rows, sums, end;
-    DeltaParts(const DeltaShape& s, bool backward) {
+    size_t gates, t, p, k, q, d_states, d_rows, sums, end;
+    DeltaParts(const DeltaShape& s, bool backward, size_t element) {
         const size_t entries = (size_t)s.blocks * s.heads;
+        const size_t copy = (size_t)s.blocks * s.key_heads * kBlock * (s.dk <= 64 ? 64 : 128) * element;
         gates = 0;
         t = round_up(gates + entries * kGateFloats * 4);
         p = round_up(t + entries * kMatrixBytes<NS>);
-        d_states = round_up(p + entries * kMatrixBytes<NS>);
+        k = round_up(p + entries * kMatrixBytes<NS>);
+        q = round_up(k + copy);
+        d_states = round_up(q + copy);
         d_rows = round_up(d_states + (backward ? entries * s.dk * s.dv * 4 : 0));
         sums = round_up(d_rows + (backward ? (size_t)s.rows * s.heads * s.dv * 4 : 0));
         end = round_up(sums + (backward && s.heads > s.key_heads ? (size_t)s.blocks * s.key_heads * 2 * kBlock * (s.dk <= 64 ? 64 : 128) * 4 : 0));
@@ -48,14 +51,15 @@ hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void
     const auto kernel = upper ? delta_prepare<E, NI, NS, DK, true> : delta_prepare<E, NI, NS, DK, false>;
     return delta_launch(kernel, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
                         kPrepareBytes<NI, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
-                        log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p);
+                        log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p,
+                        reinterpret_cast<S*>(ws + at.k), reinterpret_cast<S*>(ws + at.q));
 }
 
 template <class E, int NI, int NS, int DK>
 int delta_forward_dk(const DeltaForward& f) {
     using S = typename E::S;
     const DeltaShape& s = f.shape;
-    const DeltaParts<NS> at(s, false);
+    const DeltaParts<NS> at(s, false, sizeof(S));
     if (s.blocks > 0) {
         const hipError_t e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, f.workspace, at, false, f.stream);
         if (e != hipSuccess) return delta_status(e);
@@ -63,7 +67,7 @@ int delta_forward_dk(const DeltaForward& f) {
     const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, DK, true> : delta_chain<E, NI, NS, DK, false>;
     return delta_status(delta_launch(
         chain, dim3((unsigned)chain_grid(s)), 512, kChainBytes<NI, NS, DK>, f.stream,
-        s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
+        s, reinterpret_cast<const S*>(f.workspace + at.q), reinterpret_cast<const S*>(f.workspace + at.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
         static_cast<S*>(f.out), f.final, f.states, f.updates));
 }
@@ -72,7 +76,7 @@ template <class E, int NI, int NS, int DK>
 int delta_backward_dk(const DeltaBackward& f) {
     using S = typename E::S;
     const DeltaShape& s = f.shape;
-    const DeltaParts<NS> at(s, true);
+    const DeltaParts<NS> at(s, true, sizeof(S));
     char* ws = f.workspace;
     hipError_t e = hipSuccess;
     if (s.blocks > 0) e = prepare<E, NI, NS, DK>(s, f.q, f.k, f.log_gates, f.beta, ws, at, true, f.stream);
@@ -80,13 +84,13 @@ int delta_backward_dk(const DeltaBackward& f) {
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 256, kReverseBytes<NI, NS, DK>, f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 256, kReverseBytes<NI, NS, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows);
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
     return delta_status(delta_launch(
         delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), 512, kGradientBytes<NI, NS, DK>,
-        f.stream, s, static_cast<const S*>(f.q), static_cast<const S*>(f.k), static_cast<const S*>(f.v),
+        f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k), static_cast<const S*>(f.v),
         static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
         static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta,
         reinterpret_cast<float*>(ws + at.sums)));
@@ -114,7 +118,7 @@ int delta_step_any(const DeltaStep& p) {
         return f.shape.dk <= 64 ? delta_backward_dk<E, NI, NS, 64>(f) : delta_backward_dk<E, NI, NS, 128>(f);   \
     }                                                                                                           \
     int delta_step_##suffix(const DeltaStep& p) { return delta_step_any<E>(p); }                                \
-    size_t delta_workspace_##suffix(const DeltaShape& s, bool backward) { return DeltaParts<NS>(s, backward).end; } \
+    size_t delta_workspace_##suffix(const DeltaShape& s, bool backward) { return DeltaParts<NS>(s, backward, sizeof(E::S)).end; } \
     }
 
 }  // namespace ascan

@@ -31,9 +31,9 @@ inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads +
 
 template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                            3 * Exchange<NS, 2>::kBytes;
+                            3 * Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
 
-// grid chain_grid(), 512 threads.  KEEP: write the states in front of the blocks and the rows U.
+// q and k: the copies that delta_prepare made.  grid chain_grid(), 512 threads.  KEEP: write the states in front of the blocks and the rows U.
 template <class E, int NI, int NS, int DK, bool KEEP>
 __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
@@ -62,31 +62,43 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
     Exchange<NS, kDepths> xs(m);
     m += Exchange<NS, kDepths>::kBytes;
     Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes), xd(m + 2 * Exchange<NS, 2>::kBytes);
+    m += 3 * Exchange<NS, 2>::kBytes;
+    char* const matrix_at = m;
+    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NS>);
 
     constexpr uint32_t kSize = sizeof(ES);
-    const uint32_t k_step = s.key_heads * s.dk * kSize, v_step = s.heads * s.dv * kSize;
+    const uint32_t v_step = s.heads * s.dv * kSize;
     const int64_t seq_row = uniform(at.row), seq_length = uniform(at.length), seq_block = uniform(at.block);
     const int token = 16 * wave + c;
-    const auto rows_of = [&](const void* p, int64_t first, uint32_t step, int64_t at_head, uint32_t bytes) {
-        const int64_t left = seq_length - first < kBlock ? seq_length - first : kBlock;
-        return buffer_of(static_cast<const char*>(p) + (seq_row + first) * step + at_head, (left - 1) * (int64_t)step + bytes);
+    // Where the block at hand begins in a tensor or table; moved on by a constant from block to block.
+    const auto rows_of = [&](const char* p, int64_t first, uint32_t step, uint32_t bytes) {
+        const int64_t left = seq_length - first;
+        return buffer_of(p, left <= 0 ? 0 : ((left < kBlock ? (int)left : kBlock) - 1) * (int)step + (int)bytes);
     };
-    const auto entry_of = [&](int64_t first) { return (seq_block + first / kBlock) * s.heads + head; };
-    const auto gates_of = [&](int64_t first) { return buffer_of(gates + entry_of(first) * kGateFloats, kGateFloats * 4); };
+    const auto start_of = [&](const void* p, uint32_t step, int64_t at_head) { return static_cast<const char*>(p) + seq_row * step + at_head; };
+    const int64_t entry0 = seq_block * s.heads + head;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    constexpr int kKeyBytes = kBlock * DK * kSize;  // of a block, in the copies
+    const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
+    const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
+    const auto gates_here = [&]() { return buffer_of(gate_p, kGateFloats * 4); };
     // (waves 0 and 1 have one operand to a row of tiles: their second load lies outside and gives zero)
-    const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
-        const Buffer b = buffer_of(from + entry_of(first) * kMatrixBytes<NS>, kMatrixBytes<NS>);
+    const auto load_matrix = [&](const char* from, Operand<NS>(&o)[2]) {
+        const Buffer b = buffer_of(from, kMatrixBytes<NS>);
         o[0] = matrix_operand<NS>(b, pair_lower(wave, 0), lane);
         o[1] = matrix_operand<NS>(b, wave >= 2 ? pair_lower(wave, 1) : (int)(kOutside >> 12), lane);
     };
-    const auto ahead_of = [&](int64_t first) { return first + kBlock < seq_length ? first + kBlock : first; };
     const auto keys_at = [&](int64_t first) { return Tile<NI, DK>(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes); };
+    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NS>; };
+    const auto gate_of = [&](int64_t first) { return gate_at + ((first / kBlock) & 1) * 4 * kBlock; };
     const auto values_at = [&](int64_t first) { return Tile<NI, 16>(vt_at + ((first / kBlock) & 1) * Tile<NI, 16>::kBytes); };
 
     // An empty sequence has no table entry to read: its state is handed through.
     if (keeper) {
         fx4 S[kOwn];
         const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
+        [[maybe_unused]] char* state_p = reinterpret_cast<char*>(states + entry0 * s.dk * s.dv);
+        [[maybe_unused]] char* update_p = reinterpret_cast<char*>(updates + (seq_row * s.heads + head) * s.dv);
 #pragma unroll
         for (int t = 0; t < kOwn; ++t)
 #pragma unroll
@@ -94,21 +106,23 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                 const int row = feature_row(kOwn * wave + t, g, r);
                 S[t][r] = initial != nullptr && mine && row < s.dk ? initial[state_at + (int64_t)row * s.dv] : 0.0f;
             }
-        const uint32_t gate_rows = (16 * wave + 4 * g) * 4;
-        Operand<NS> tm[2];
-        fx4 beta, beta_since, until;
-        float whole;
+        Operand<NI> ko[kDepths];
+        fx4 x, beta, beta_since;
+        const auto gate_rows = [&](int64_t first, int row) { return *reinterpret_cast<const fx4*>(gate_of(first) + row * kBlock + 16 * wave + 4 * g); };
+        const auto read_block = [&](int64_t first) {  // what of the block at `first` the first product takes beside the state
+#pragma unroll
+            for (int d = 0; d < kDepths; ++d) ko[d] = keys_at(first).along(token, 32 * d, g);
+            x = values_at(first).tile(16 * wave, 0, lane);
+            beta = gate_rows(first, kBeta);
+            beta_since = gate_rows(first, kBetaSince);
+        };
+        __builtin_amdgcn_s_setprio(3);
         if (seq_length > 0) {
-            const Buffer b = gates_of(0);
-            beta = fetch16(b, kBeta * 256 + gate_rows);
-            beta_since = fetch16(b, kBetaSince * 256 + gate_rows);
-            load_matrix(t_in, 0, tm);
-            until = fetch16(b, kUntil * 256 + gate_rows);
-            whole = fetch4(b, kSince * 256 + (c | 63) * 4);
+            lds_barrier();  // the first block's keys and values are there
+            read_block(0);
         }
         for (int64_t first = 0; first < seq_length; first += kBlock) {
-            const int64_t ahead = ahead_of(first);
-            const Buffer gb = gates_of(ahead);
+            const bool more = first + kBlock < seq_length;
             const Tile<NI, DK> kb = keys_at(first);
 #pragma unroll
             for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, S[t]);
@@ -116,16 +130,17 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
 
             // K S0 (rows: tokens, columns: state columns)
             fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-            fx4 x;
+            Operand<NS> tm[2];
+            fx4 until;
+            float whole;
             {
                 Operand<NS> so[kDepths];
-                Operand<NI> ko[kDepths];
 #pragma unroll
-                for (int d = 0; d < kDepths; ++d) {
-                    so[d] = xs.get(d, lane);
-                    ko[d] = kb.along(token, 32 * d, g);
-                }
-                x = values_at(first).tile(16 * wave, 0, lane);
+                for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
+                tm[0] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane);
+                tm[1] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
+                until = gate_rows(first, kUntil);
+                whole = gate_of(first)[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
@@ -139,19 +154,15 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
             xr.put(wave, lane, u);
             lds_barrier();
 
-            // U = R + T R
+            // U = R + T R; what the next products take of the keys is read on the way
+            Operand<NI> k_low[kOwn], k_high[kOwn];
             {
                 const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
-                if constexpr (KEEP) {  // (the state, while these come)
-                    const Buffer to = buffer_of(states + entry_of(first) * s.dk * s.dv, (int64_t)s.dk * s.dv * 4);
 #pragma unroll
-                    for (int t = 0; t < kOwn; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, S[t][r]);
+                for (int t = 0; t < kOwn; ++t) {
+                    k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
+                    k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
-                beta = fetch16(gb, kBeta * 256 + gate_rows);
-                beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
                 __builtin_amdgcn_sched_barrier(0);
                 u = mma<NS, NS>(tm[0], low, u);
                 if (wave >= 2) {
@@ -160,40 +171,55 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 }
             }
+            {
+                fx4 y;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = until[r] * u[r];
-            xd.put(wave, lane, x);
+                for (int r = 0; r < 4; ++r) y[r] = until[r] * u[r];
+                xd.put(wave, lane, y);
+            }
             xu.put(wave, lane, u);
             lds_barrier();
 
             // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
             {
                 const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
-                Operand<NI> k_low[kOwn], k_high[kOwn];
+                if constexpr (KEEP) {  // (the state in front of the block, while these come)
+                    const Buffer to = buffer_of(state_p, (int64_t)s.dk * s.dv * 4);
 #pragma unroll
-                for (int t = 0; t < kOwn; ++t) {
-                    k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
-                    k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
+                    for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, S[t][r]);
                 }
-                load_matrix(t_in, ahead, tm);
-                until = fetch16(gb, kUntil * 256 + gate_rows);
                 __builtin_amdgcn_sched_barrier(0);
+                fx4 S2[kOwn];
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) S[t][r] *= whole;
                     S[t] = mma<NI, NS>(k_low[t], low, S[t]);
-                    S[t] = mma<NI, NS>(k_high[t], high, S[t]);
+                    S2[t] = mma<NI, NS>(k_high[t], high, fx4{0, 0, 0, 0});
                 }
-            }
-            whole = fetch4(gb, kSince * 256 + (c | 63) * 4);
-            if constexpr (KEEP) {
-                const uint32_t step = s.heads * s.dv * 4;
-                const Buffer to = rows_of(updates, first, step, (int64_t)head * s.dv * 4, s.dv * 4);
+                read_block(more ? first + kBlock : first);
+                if constexpr (KEEP) {
+                    const uint32_t step = s.heads * s.dv * 4;
+                    const Buffer to = rows_of(update_p, first, step, s.dv * 4);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    put1<ElemF32>(to, mine ? (16 * wave + 4 * g + r) * step + col * 4 : kOutside, u[r]);
+                    for (int r = 0; r < 4; ++r)
+                        put1<ElemF32>(to, mine ? (16 * wave + 4 * g + r) * step + col * 4 : kOutside, u[r]);
+                    state_p += (int64_t)s.heads * s.dk * s.dv * 4;
+                    update_p += (int64_t)step * kBlock;
+                }
+#pragma unroll
+                for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[t][r] += S2[t][r];
             }
+        }
+        if (((seq_length + kBlock - 1) / kBlock) & 1) {  // the other waves go on by two blocks
+            lds_barrier();
+            lds_barrier();
+            lds_barrier();
         }
         if (final != nullptr && mine) {
 #pragma unroll
@@ -205,40 +231,66 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                 }
         }
     } else if (seq_length > 0) {
-        Eight<E> k_raw[kCopies], v_raw, q_raw[kDepths];
-        Operand<NS> pm[2];
-        float since;
-        const auto load_kv = [&](int64_t first) {
-            const Buffer kb = rows_of(k, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-            const Buffer vb = rows_of(v, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
+        Eight<E> k_raw[2][kCopies], v_raw[2], q_raw[2][kDepths];  // of the next two blocks
+        Operand<NS> pm[2][2];
+        float since[2], gate_raw[2];
+        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
+        static_assert(kMatrixBytes<NS> % (16 * 256) == 0, "pieces of a matrix to a thread");
+        fx4 t_raw[2][kPieces];
+        const int64_t v_head = (int64_t)head * s.dv * kSize, copy0 = (seq_block * s.key_heads + key_head) * kBlock * DK;
+        const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head), *q_p = reinterpret_cast<const char*>(q + copy0);
+        const char *p_p = p_in + entry0 * kMatrixBytes<NS>, *t_p = t_in + entry0 * kMatrixBytes<NS>, *out_p = start_of(out, v_step, v_head);
+        const char* load_gate_p = gate_p;
+        const auto load_block = [&](int64_t first, int set) {
+            const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) {
-                const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
-                k_raw[i] = fetch8<E>(kb, d < s.dk ? row * k_step + d * kSize : kOutside);
-            }
+            for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
-            v_raw = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+            v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            gate_raw[set] = fetch4(buffer_of(load_gate_p, kGateFloats * 4), tid * 4);
+            if (first + kBlock < seq_length) {
+                k_p += k_move;
+                v_p += v_move;
+                t_p += matrix_move;
+                load_gate_p += gate_move;
+            }
         };
-        const auto stage_kv = [&](int64_t first) {
+        const auto stage_block = [&](int64_t first, int set) {
             const Tile<NI, DK> kb = keys_at(first);
 #pragma unroll
-            for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[i]);
-            values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw);
-        };
-        const auto load_q = [&](int64_t first) {
-            const Buffer b = rows_of(q, first, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+            for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
+            values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
 #pragma unroll
-            for (int d = 0; d < kDepths; ++d)
-                q_raw[d] = fetch8<E>(b, 32 * d + 8 * g < s.dk ? token * k_step + (32 * d + 8 * g) * kSize : kOutside);
+            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
+            gate_of(first)[tid] = gate_raw[set];
         };
-        load_kv(0);
-        load_q(0);
-        load_matrix(p_in, 0, pm);
-        since = fetch4(gates_of(0), kSince * 256 + token * 4);
-        stage_kv(0);
-        load_kv(ahead_of(0));
-        for (int64_t first = 0; first < seq_length; first += kBlock) {
-            const int64_t ahead = ahead_of(first);
+        const auto load_outputs = [&](int64_t first, int set) {  // what the block's outputs take beside state and updates
+            const Buffer b = buffer_of(q_p, kKeyBytes);
+#pragma unroll
+            for (int d = 0; d < kDepths; ++d) q_raw[set][d] = fetch8<E>(b, ((wave * kDepths + d) * 64 + lane) * 8 * kSize);
+            load_matrix(p_p, pm[set]);
+            since[set] = fetch4(gates_here(), kSince * 256 + token * 4);
+            if (first + kBlock < seq_length) {
+                q_p += k_move;
+                p_p += matrix_move;
+                gate_p += gate_move;
+            }
+        };
+        // (in the order in which the loop goes on)
+        load_block(0, 0);
+        load_block(kBlock, 1);
+        load_outputs(0, 0);
+        stage_block(0, 0);
+        load_block(2 * kBlock, 0);
+        load_outputs(kBlock, 1);
+        lds_barrier();
+        // The block's own loads are in set `own`, the next one's in the other.  Loads come back in the order of their
+        // issue, so all of them run two blocks ahead: one that did not would make its wait one for all before it.
+        // Behind the last block loads give zero and stores are dropped, so no condition stands around either.
+        const auto block = [&](int64_t first, int own) {
             lds_barrier();
             // (Q S0)^T (rows: state columns, columns: tokens)
             fx4 o = {0, 0, 0, 0}, o2 = {0, 0, 0, 0};
@@ -249,31 +301,33 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
-                    o = mma<NS, NI>(so[d], operand_from<NI, E>(q_raw[d]), o);
-                    o2 = mma<NS, NI>(so[d + 1], operand_from<NI, E>(q_raw[d + 1]), o2);
+                    o = mma<NS, NI>(so[d], operand_from<NI, E>(q_raw[own][d]), o);
+                    o2 = mma<NS, NI>(so[d + 1], operand_from<NI, E>(q_raw[own][d + 1]), o2);
                 }
             }
-            load_q(ahead);
             lds_barrier();
-            // the other tiles' readers are behind the first barrier
-            if (ahead != first) stage_kv(ahead);
-            load_kv(ahead_of(ahead));
-            const float f = s.scale * since;
+            // the tiles' last readers are behind the first barrier
+            stage_block(first + kBlock, own ^ 1);
+            load_block(first + 3 * kBlock, own ^ 1);
+            const float f = s.scale * since[own];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = f * (o[r] + o2[r]);
             lds_barrier();
             // out^T = scale (Q S0)^T diag(e^c) + U^T P^T
-            o = mma<NS, NS>(xu.get(0, lane), pm[0], o);
+            o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
             if (wave >= 2) {
-                o2 = mma<NS, NS>(xu.get(1, lane), pm[1], fx4{0, 0, 0, 0});
+                o2 = mma<NS, NS>(xu.get(1, lane), pm[own][1], fx4{0, 0, 0, 0});
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] += o2[r];
             }
+            load_outputs(first + 2 * kBlock, own);
             const int d = col0 + 4 * g;
-            const Buffer to = rows_of(out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
-            put4<E>(to, d < s.dv ? token * v_step + d * kSize : kOutside, o);
-            load_matrix(p_in, ahead, pm);
-            since = fetch4(gates_of(ahead), kSince * 256 + token * 4);
+            put4<E>(rows_of(out_p, first, v_step, s.dv * kSize), d < s.dv ? token * v_step + d * kSize : kOutside, o);
+            out_p += v_move;
+        };
+        for (int64_t first = 0; first < seq_length; first += 2 * kBlock) {
+            block(first, 0);
+            block(first + kBlock, 1);
         }
     }
     // rows in front of the first and behind the last sequence are zero

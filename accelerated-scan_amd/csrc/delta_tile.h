@@ -245,6 +245,14 @@ __device__ __forceinline__ Operand<P> operand_from(const Eight<E>& x) {
     return o;
 }
 
+template <class E>
+__device__ __forceinline__ void store8(typename E::S* p, const Eight<E>& x) {
+    fx4 v[sizeof(x.v) / 16];
+    __builtin_memcpy(v, x.v, sizeof(x.v));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(x.v) / 16; ++i) reinterpret_cast<fx4*>(p)[i] = v[i];
+}
+
 // Four neighbouring values to memory.
 template <class E>
 __device__ __forceinline__ void store4(typename E::S* p, const fx4& x) {
