@@ -66,7 +66,7 @@ int delta_forward_dk(const DeltaForward& f) {
     }
     const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, DK, true> : delta_chain<E, NI, NS, DK, false>;
     return delta_status(delta_launch(
-        chain, dim3((unsigned)chain_grid(s)), 512, kChainBytes<NI, NS, DK>, f.stream,
+        chain, dim3((unsigned)chain_grid(s)), 768, kChainBytes<NI, NS, DK>, f.stream,
         s, reinterpret_cast<const S*>(f.workspace + at.q), reinterpret_cast<const S*>(f.workspace + at.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
         static_cast<S*>(f.out), f.final, f.states, f.updates));

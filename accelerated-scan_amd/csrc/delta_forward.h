@@ -4,9 +4,10 @@
 // three products (K S0, T R, K^T U) that are too small to fill a wave's matrix unit for long.  A workgroup
 // therefore takes only 16 columns of one head's state and divides the rows: state wave w (0 to 3) keeps state rows
 // dk/4 w .. in its accumulators and computes tokens 16w .. 16w+15 of every block.  State, R and U go round through LDS
-// in the order in which the next product reads them, with one barrier each.  Four more waves, one beside each
-// of the first on its SIMD, do what the chain does not wait for: they bring keys and values to LDS a block ahead and
-// compute the outputs.
+// in the order in which the next product reads them, with one barrier each.  What the chain does not wait for
+// is done by waves of their own beside these on the same SIMDs: four compute the outputs, four bring keys, values, T
+// and gates to LDS blocks ahead.  (The loads are 66 KiB a block, which the 64 bytes per clock of a compute unit's
+// cache turn into 1100 clocks of issue: a wave that loads is late for its barrier if it has anything else to do.)
 #ifndef ASCAN_DELTA_FORWARD_H_
 #define ASCAN_DELTA_FORWARD_H_
 
@@ -33,9 +34,9 @@ template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
                             3 * Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
 
-// q and k: the copies that delta_prepare made.  grid chain_grid(), 512 threads.  KEEP: write the states in front of the blocks and the rows U.
+// q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.  KEEP: write the states in front of the blocks and the rows U.
 template <class E, int NI, int NS, int DK, bool KEEP>
-__global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
+__global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
                                                    const typename E::S* __restrict__ v,
                                                    const float* __restrict__ gates, const char* __restrict__ t_in,
@@ -50,7 +51,8 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
     const int64_t n = where.sequence;
     const int head = where.head, key_head = head / (s.heads / s.key_heads);
     const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
-    const bool keeper = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8) == 0;  // a state wave
+    const int role = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+    const bool keeper = role == 0;  // a state wave
     const int col0 = where.col0, col = col0 + c;
     const bool mine = col < s.dv;
     const SequenceAt at = sequence_at(s, n);
@@ -92,6 +94,8 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
     const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NS>; };
     const auto gate_of = [&](int64_t first) { return gate_at + ((first / kBlock) & 1) * 4 * kBlock; };
     const auto values_at = [&](int64_t first) { return Tile<NI, 16>(vt_at + ((first / kBlock) & 1) * Tile<NI, 16>::kBytes); };
+
+    const int64_t v_head = (int64_t)head * s.dv * kSize, copy0 = (seq_block * s.key_heads + key_head) * kBlock * DK;
 
     // An empty sequence has no table entry to read: its state is handed through.
     if (keeper) {
@@ -230,67 +234,34 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                     if (row < s.dk) final[state_at + (int64_t)row * s.dv] = S[t][r];
                 }
         }
-    } else if (seq_length > 0) {
-        Eight<E> k_raw[2][kCopies], v_raw[2], q_raw[2][kDepths];  // of the next two blocks
+    } else if (role == 1 && seq_length > 0) {
+        // The outputs.  Loads come back in the order of their issue, so all of them run more than a block ahead: one that
+        // did not would make its wait one for all before it.  Behind the last block loads repeat it or give zero and
+        // stores are dropped, so that no condition stands around them.
+        Eight<E> q_raw[2][kDepths];
         Operand<NS> pm[2][2];
-        float since[2], gate_raw[2];
-        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
-        static_assert(kMatrixBytes<NS> % (16 * 256) == 0, "pieces of a matrix to a thread");
-        fx4 t_raw[2][kPieces];
-        const int64_t v_head = (int64_t)head * s.dv * kSize, copy0 = (seq_block * s.key_heads + key_head) * kBlock * DK;
-        const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head), *q_p = reinterpret_cast<const char*>(q + copy0);
-        const char *p_p = p_in + entry0 * kMatrixBytes<NS>, *t_p = t_in + entry0 * kMatrixBytes<NS>, *out_p = start_of(out, v_step, v_head);
-        const char* load_gate_p = gate_p;
-        const auto load_block = [&](int64_t first, int set) {
-            const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
-#pragma unroll
-            for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
-            const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
-            v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
-            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
-            gate_raw[set] = fetch4(buffer_of(load_gate_p, kGateFloats * 4), tid * 4);
-            if (first + kBlock < seq_length) {
-                k_p += k_move;
-                v_p += v_move;
-                t_p += matrix_move;
-                load_gate_p += gate_move;
-            }
-        };
-        const auto stage_block = [&](int64_t first, int set) {
-            const Tile<NI, DK> kb = keys_at(first);
-#pragma unroll
-            for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
-            values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
-            gate_of(first)[tid] = gate_raw[set];
-        };
-        const auto load_outputs = [&](int64_t first, int set) {  // what the block's outputs take beside state and updates
+        float since[2];
+        const char *q_p = reinterpret_cast<const char*>(q + copy0), *p_p = p_in + entry0 * kMatrixBytes<NS>;
+        const char* out_p = start_of(out, v_step, v_head);
+        const auto load_q = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Buffer b = buffer_of(q_p, kKeyBytes);
 #pragma unroll
             for (int d = 0; d < kDepths; ++d) q_raw[set][d] = fetch8<E>(b, ((wave * kDepths + d) * 64 + lane) * 8 * kSize);
+            if (first + kBlock < seq_length) q_p += k_move;
+        };
+        const auto load_p = [&](int64_t first, int set) __attribute__((always_inline)) {
             load_matrix(p_p, pm[set]);
             since[set] = fetch4(gates_here(), kSince * 256 + token * 4);
             if (first + kBlock < seq_length) {
-                q_p += k_move;
                 p_p += matrix_move;
                 gate_p += gate_move;
             }
         };
-        // (in the order in which the loop goes on)
-        load_block(0, 0);
-        load_block(kBlock, 1);
-        load_outputs(0, 0);
-        stage_block(0, 0);
-        load_block(2 * kBlock, 0);
-        load_outputs(kBlock, 1);
+        load_q(0, 0);
+        load_p(0, 0);
+        load_q(kBlock, 1);
         lds_barrier();
-        // The block's own loads are in set `own`, the next one's in the other.  Loads come back in the order of their
-        // issue, so all of them run two blocks ahead: one that did not would make its wait one for all before it.
-        // Behind the last block loads give zero and stores are dropped, so no condition stands around either.
-        const auto block = [&](int64_t first, int own) {
+        const auto block = [&](int64_t first, int own) __attribute__((always_inline)) {
             lds_barrier();
             // (Q S0)^T (rows: state columns, columns: tokens)
             fx4 o = {0, 0, 0, 0}, o2 = {0, 0, 0, 0};
@@ -306,9 +277,8 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
                 }
             }
             lds_barrier();
-            // the tiles' last readers are behind the first barrier
-            stage_block(first + kBlock, own ^ 1);
-            load_block(first + 3 * kBlock, own ^ 1);
+            load_p(first + kBlock, own ^ 1);
+            load_q(first + 2 * kBlock, own);
             const float f = s.scale * since[own];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = f * (o[r] + o2[r]);
@@ -320,7 +290,6 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] += o2[r];
             }
-            load_outputs(first + 2 * kBlock, own);
             const int d = col0 + 4 * g;
             put4<E>(rows_of(out_p, first, v_step, s.dv * kSize), d < s.dv ? token * v_step + d * kSize : kOutside, o);
             out_p += v_move;
@@ -328,6 +297,57 @@ __global__ __launch_bounds__(512) void delta_chain(DeltaShape s, const typename 
         for (int64_t first = 0; first < seq_length; first += 2 * kBlock) {
             block(first, 0);
             block(first + kBlock, 1);
+        }
+    } else if (seq_length > 0) {
+        // Keys, values, T and gates to LDS, three blocks ahead.
+        Eight<E> k_raw[2][kCopies], v_raw[2];
+        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
+        static_assert(kMatrixBytes<NS> % (16 * 256) == 0, "pieces of a matrix to a thread");
+        fx4 t_raw[2][kPieces];
+        float gate_raw[2];
+        const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head);
+        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const auto load_block = [&](int64_t first, int set) __attribute__((always_inline)) {
+            const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
+            const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
+            v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            gate_raw[set] = fetch4(gates_here(), tid * 4);
+            v_p += v_move;
+            if (first + kBlock < seq_length) {
+                k_p += k_move;
+                t_p += matrix_move;
+                gate_p += gate_move;
+            }
+        };
+        const auto stage_block = [&](int64_t first, int set) __attribute__((always_inline)) {
+            const Tile<NI, DK> kb = keys_at(first);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
+            values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
+            gate_of(first)[tid] = gate_raw[set];
+        };
+        load_block(0, 0);
+        load_block(kBlock, 1);
+        stage_block(0, 0);
+        load_block(2 * kBlock, 0);
+        lds_barrier();
+        const auto block = [&](int64_t first, int other) __attribute__((always_inline)) {
+            lds_barrier();
+            lds_barrier();
+            stage_block(first + kBlock, other);  // the tiles' last readers are behind the first barrier
+            lds_barrier();
+            load_block(first + 3 * kBlock, other);
+        };
+        for (int64_t first = 0; first < seq_length; first += 2 * kBlock) {
+            block(first, 1);
+            block(first + kBlock, 0);
         }
     }
     // rows in front of the first and behind the last sequence are zero
