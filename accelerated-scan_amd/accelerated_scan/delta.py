@@ -30,7 +30,10 @@ def _fail(what):
 
 def _check_tensors(like, named):
     """All device tensors on one device, contiguous."""
+    device = like.device
     for name, t in named:
+        if t is None or (t.is_cuda and t.device == device and t.is_contiguous()):
+            continue
         if not t.is_cuda:
             _fail(f"expected {name} to be a device tensor")
         if t.device != like.device:
@@ -82,12 +85,8 @@ def _check_scan(queries, keys, values, log_gates, beta, initial, offsets):
         if initial.shape != shape or initial.dtype != torch.float32:
             _fail(f"expected initial of shape {shape} and dtype torch.float32, got {tuple(initial.shape)} and "
                   f"{initial.dtype}")
-    named = [("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("beta", beta)]
-    if initial is not None:
-        named.append(("initial", initial))
-    if offsets is not None:
-        named.append(("offsets", offsets))
-    _check_tensors(queries, named)
+    _check_tensors(queries, (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates),
+                             ("beta", beta), ("initial", initial), ("offsets", offsets)))
     return sequences
 
 
@@ -143,7 +142,11 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
     """
     _check_scan(queries, keys, values, log_gates, beta, initial, offsets)
     scale = float(scale) if scale is not None else queries.shape[-1] ** -0.5
-    return GatedDeltaScan.apply(queries, keys, values, log_gates, beta, initial, offsets, scale)
+    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad
+                                    or log_gates.requires_grad or beta.requires_grad
+                                    or (initial is not None and initial.requires_grad)):
+        return GatedDeltaScan.apply(queries, keys, values, log_gates, beta, initial, offsets, scale)
+    return _ops.delta_forward_run(queries, keys, values, log_gates, beta, initial, offsets, scale, False)[:2]
 
 
 def _check_step(queries, keys, values, log_gates, beta, states, slots):
@@ -155,16 +158,14 @@ def _check_step(queries, keys, values, log_gates, beta, states, slots):
     if states.dim() != 4 or states.shape[1:] != shape or states.dtype != torch.float32:
         _fail(f"expected states of shape (slots, {', '.join(map(str, shape))}) and dtype torch.float32, got "
               f"{tuple(states.shape)} and {states.dtype}")
-    named = [("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates), ("beta", beta),
-             ("states", states)]
     if slots is None:
         if states.shape[0] != queries.shape[0]:
             _fail(f"expected a state to each of {queries.shape[0]} rows, got {states.shape[0]}")
     else:
         if slots.shape != queries.shape[:1] or slots.dtype not in (torch.int32, torch.int64):
             _fail(f"expected slots of shape ({queries.shape[0]},), int32 or int64")
-        named.append(("slots", slots))
-    _check_tensors(queries, named)
+    _check_tensors(queries, (("queries", queries), ("keys", keys), ("values", values), ("log_gates", log_gates),
+                             ("beta", beta), ("states", states), ("slots", slots)))
 
 
 def gated_delta_step(queries, keys, values, log_gates, beta, states, slots=None, scale=None):

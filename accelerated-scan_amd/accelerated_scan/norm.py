@@ -15,6 +15,12 @@ _REAL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(x, gate, weight):
+    """The passing case builds no message."""
+    dtype, device, shape = x.dtype, x.device, x.shape
+    if (dtype in _REAL_DTYPES and gate.dtype == dtype and weight.dtype == dtype and gate.shape == shape
+            and weight.shape == shape[-1:] and len(shape) > 0 and x.is_cuda and gate.device == device
+            and weight.device == device and x.is_contiguous() and gate.is_contiguous() and weight.is_contiguous()):
+        return
     if x.dim() < 1 or gate.shape != x.shape or weight.shape != x.shape[-1:]:
         raise RuntimeError(
             f"accelerated_scan: expected x and gate of one shape and weight of its last axis, got {tuple(x.shape)}, "
@@ -32,6 +38,15 @@ def _check(x, gate, weight):
             raise RuntimeError(f"accelerated_scan: expected {name} to be contiguous")
 
 
+def _forward(x, gate, weight, eps):
+    if _ops.capturing():
+        return _ops.gated_norm(x, gate, weight, eps)
+    out = torch.empty_like(x)
+    if x.numel():
+        _abi.gated_norm(x, gate, weight, eps, out)
+    return out
+
+
 class GatedNorm(torch.autograd.Function):
     """Autograd node: saves the inputs, recomputes the norm."""
 
@@ -39,12 +54,7 @@ class GatedNorm(torch.autograd.Function):
     def forward(ctx, x, gate, weight, eps):
         ctx.save_for_backward(x, gate, weight)
         ctx.eps = eps
-        if _ops.capturing():
-            return _ops.gated_norm(x, gate, weight, eps)
-        out = torch.empty_like(x)
-        if x.numel():
-            _abi.gated_norm(x, gate, weight, eps, out)
-        return out
+        return _forward(x, gate, weight, eps)
 
     @staticmethod
     def backward(ctx, d_out):
@@ -65,4 +75,6 @@ def gated_norm(x, gate, weight, eps=1e-6):
         (torch.Tensor): the shape of x; differentiable in x, gate and weight.
     """
     _check(x, gate, weight)
-    return GatedNorm.apply(x, gate, weight, float(eps))
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or weight.requires_grad):
+        return GatedNorm.apply(x, gate, weight, float(eps))
+    return _forward(x, gate, weight, float(eps))

@@ -76,7 +76,7 @@ int norm_backward_any(const void* x, const void* gate, const void* weight, const
         return norm_status(hipGetLastError());
     });
     if (status != ASCAN_OK) return status;
-    hipLaunchKernelGGL((norm_fold<E>), dim3((unsigned)((width + 63) / 64)), dim3(1024), 0, stream, partial,
+    hipLaunchKernelGGL((norm_fold<E>), dim3((unsigned)((width + 15) / 16)), dim3(1024), 0, stream, partial,
                        static_cast<S*>(d_weight), (int)parts, (int)width);
     return norm_status(hipGetLastError());
 }
