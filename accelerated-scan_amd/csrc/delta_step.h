@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void delta_step(DeltaStep p, int groups) {
     for (int i = 0; i < N; ++i) {
         const int row = row0 + i * kRowStep;
         s[i] = fx4{0, 0, 0, 0};
-        if (there && mine && row < p.dk) s[i] = *reinterpret_cast<const fx4*>(state + (int64_t)row * p.dv);
+        if (there && mine && row < p.dk) s[i] = N > 4 ? __builtin_nontemporal_load(reinterpret_cast<const fx4*>(state + (int64_t)row * p.dv)) : *reinterpret_cast<const fx4*>(state + (int64_t)row * p.dv);
     }
     for (;;) {
         int64_t next = -1;
@@ -125,7 +125,10 @@ __global__ __launch_bounds__(256) void delta_step(DeltaStep p, int groups) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int row = row0 + i * kRowStep;
-        if (mine && row < p.dk) *reinterpret_cast<fx4*>(state + (int64_t)row * p.dv) = s[i];
+        if (mine && row < p.dk) {
+            if (N > 4) __builtin_nontemporal_store(s[i], reinterpret_cast<fx4*>(state + (int64_t)row * p.dv));
+            else *reinterpret_cast<fx4*>(state + (int64_t)row * p.dv) = s[i];
+        }
     }
 }
 

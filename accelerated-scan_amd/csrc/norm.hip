@@ -13,7 +13,7 @@ int norm_status(hipError_t e) {
 }
 
 // Workgroups of the backward kernel: four to a compute unit, so that one's loads cover another's sums.
-constexpr int64_t kNormParts = 1024;
+constexpr int64_t kNormParts = 2048;
 
 template <int L>
 int64_t norm_groups(int64_t rows) { return (rows + 256 / L - 1) / (256 / L); }
