@@ -256,26 +256,29 @@ constexpr int kGradientShared = Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColum
 template <int NI, int NS, int DK>
 constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS>;
 
-// A block of one key head and all value heads that share it.  A wave owns 16 features of keys and queries and dk/2
-// of the tokens, so that each row of the two states is read by one wave only (or two); the 64 x 64 products of
-// tokens with tokens are divided among the waves by tiles and go round through LDS.  What bounds it are the two fp32
-// states per block, 8 bytes per cell against 2 for an input; the next 64 value columns are requested while these are
-// computed.
-// q and k: the copies that delta_prepare made.  grid (blocks, key heads), 512 threads.
-template <class E, int NI, int NS, int DK>
+// A block of one head.  A wave owns 16 features of keys and queries and dk/2 of the tokens, so that each row of the two
+// states is read by one wave only (or two); the 64 x 64 products of tokens with tokens are divided among the waves by
+// tiles and go round through LDS.  A workgroup reads 230 KiB and computes for 3 us; with one resident to a compute unit
+// the two alternate, and a loop over heads or blocks around this body would only lift its address arithmetic in front,
+// where it does not fit the registers (bf16 (2, 4096, 16 heads of 128 x 128): 428 us with one, 218 us without).
+//
+// SHARED: dQ and dK go to `sums` in fp32, to be added over the heads that share the keys (delta_fold).
+// q and k: the copies that delta_prepare made.  grid (blocks, heads), 512 threads.
+template <class E, int NI, int NS, int DK, bool SHARED>
 __global__ __launch_bounds__(512) void delta_gradients(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ v, const typename E::S* __restrict__ d_out, const float* __restrict__ gates,
     const float* __restrict__ states, const float* __restrict__ updates, const float* __restrict__ d_states,
     const float* __restrict__ d_rows, typename E::S* __restrict__ d_q, typename E::S* __restrict__ d_k,
-    void* __restrict__ d_log_gates, void* __restrict__ d_beta, float* sums) {
+    void* __restrict__ d_log_gates, void* __restrict__ d_beta, float* __restrict__ sums) {
     using ES = typename E::S;
     constexpr int kFeatures = DK / 16, kTok = DK / 32;  // tiles of features, and of tokens that a wave owns
     extern __shared__ __align__(16) char smem[];
     __shared__ __align__(16) float gate[kGateFloats];
-    __shared__ float dots[8][3][16 * kTok], value_dots[kBlock], whole_terms[8];
+    __shared__ __align__(16) float dots[8][2][16 * kTok];
+    __shared__ float value_dots[kBlock], whole_terms[8];
     const int64_t block = blockIdx.x;
-    const int key_head = blockIdx.y, share = s.heads / s.key_heads;
+    const int head = blockIdx.y, share = s.heads / s.key_heads, key_head = head / share;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
 
     // rows in front of the first and behind the last sequence: zero gradients, 64 rows to a workgroup
@@ -285,12 +288,14 @@ __global__ __launch_bounds__(512) void delta_gradients(
         for (int i = 0; i < 2; ++i)
             for (int64_t row = spans[i][0] + block * kBlock + wave; row < spans[i][1] && row < spans[i][0] + (block + 1) * kBlock;
                  row += 8) {
-                for (int d = lane; d < s.dk; d += 64) {
-                    d_q[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
-                    d_k[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
+                if (head % share == 0) {
+                    for (int d = lane; d < s.dk; d += 64) {
+                        d_q[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
+                        d_k[(row * s.key_heads + key_head) * s.dk + d] = E::put(0.0f);
+                    }
                 }
-                for (int h = lane; h < share; h += 64) {
-                    const int64_t to = row * s.heads + key_head * share + h;
+                if (lane == 0) {
+                    const int64_t to = row * s.heads + head;
                     if (s.wide_gates) {
                         static_cast<float*>(d_log_gates)[to] = static_cast<float*>(d_beta)[to] = 0.0f;
                     } else {
@@ -301,7 +306,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
     }
     const BlockAt found = block_at(s, block);
     if (found.length <= 0) return;
-    const int64_t row0 = uniform(found.row);
+    const int64_t row0 = uniform(found.row), entry = block * s.heads + head;
     const int length = __builtin_amdgcn_readfirstlane(found.length);
 
     const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
@@ -318,271 +323,312 @@ __global__ __launch_bounds__(512) void delta_gradients(
     const auto rows_of = [&](const void* p, uint32_t step, int64_t at_head, uint32_t bytes) {
         return buffer_of(static_cast<const char*>(p) + row0 * step + at_head, (length - 1) * (int64_t)step + bytes);
     };
-    {
-        const int64_t copy = (block * s.key_heads + key_head) * kBlock * DK;
-        const Buffer kb = buffer_of(k + copy, kBlock * DK * kSize), qb = buffer_of(q + copy, kBlock * DK * kSize);
-#pragma unroll
-        for (int i = 0; i < DK / 64; ++i) {
-            const int row = (tid + 512 * i) / (DK / 8), d = (tid + 512 * i) % (DK / 8) * 8;
-            const uint32_t from = (tid + 512 * i) * 8 * kSize;
-            const Eight<E> kv = fetch8<E>(kb, from), qv = fetch8<E>(qb, from);
-            kt.template put8<E>(row, d, kv);
-            qt.template put8<E>(row, d, qv);
-        }
-    }
-
-    const int feature0 = 16 * (wave % kFeatures), tile0 = wave / kFeatures * kTok;  // own features, first own tile of tokens
+    const int feature0 = 16 * (wave & (kFeatures - 1)), tile0 = kFeatures == 8 ? 0 : (wave >> 2) * kTok;  // own features, first own tile of tokens
     const int groups = (s.dv + kColumns - 1) / kColumns;
-    // what comes from memory for 64 value columns of a head
+
+    // what comes from memory for 64 value columns
+    const int64_t cells = (int64_t)s.dk * s.dv;
+    const Buffer ob = d_out != nullptr ? rows_of(d_out, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize) : buffer_of(k, 0);
+    const Buffer vb = rows_of(v, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
+    const Buffer ub = rows_of(updates, r_step, (int64_t)head * s.dv * 4, s.dv * 4), rb = rows_of(d_rows, r_step, (int64_t)head * s.dv * 4, s.dv * 4);
+    const Buffer sb = buffer_of(states + entry * cells, cells * 4), db = buffer_of(d_states + entry * cells, cells * 4);
     Eight<E> o_raw, v_raw;
     Eight<ElemF32> u_raw, r_raw;
     fx4 s_raw[2][2], d_raw[2][2];
-    const auto load_rows = [&](int head, int group) {
-        const int64_t at_head = (int64_t)head * s.dv;
-        const int row = tid >> 3, d = group * kColumns + (tid & 7) * 8;
-        const uint32_t from = d < s.dv ? row * v_step + d * kSize : kOutside, from_r = d < s.dv ? row * r_step + d * 4 : kOutside;
-        o_raw = fetch8<E>(d_out != nullptr ? rows_of(d_out, v_step, at_head * kSize, s.dv * kSize) : buffer_of(k, 0), from);
-        v_raw = fetch8<E>(rows_of(v, v_step, at_head * kSize, s.dv * kSize), from);
-        u_raw = fetch8<ElemF32>(rows_of(updates, r_step, at_head * 4, s.dv * 4), from_r);
-        r_raw = fetch8<ElemF32>(rows_of(d_rows, r_step, at_head * 4, s.dv * 4), from_r);
+    const uint32_t row_at = (tid >> 3) * v_step + (tid & 7) * 8 * kSize, row_at_r = (tid >> 3) * r_step + (tid & 7) * 32;
+    const uint32_t cell_at = (feature0 + c) * (uint32_t)s.dv * 4 + 32 * g;
+    const auto load_rows = [&](int group) __attribute__((always_inline)) {
+        const bool in = group * kColumns + (tid & 7) * 8 < s.dv;
+        const uint32_t from = in ? row_at + group * kColumns * kSize : kOutside, from_r = in ? row_at_r + group * kColumns * 4 : kOutside;
+        o_raw = fetch8<E>(ob, from);
+        u_raw = fetch8<ElemF32>(ub, from_r);
+        r_raw = fetch8<ElemF32>(rb, from_r);
     };
-    const auto load_states = [&](int head, int group) {
-        const int64_t entry = block * s.heads + head, cells = (int64_t)s.dk * s.dv;
-        const Buffer sb = buffer_of(states + entry * cells, cells * 4), db = buffer_of(d_states + entry * cells, cells * 4);
+    const auto load_states = [&](int group) __attribute__((always_inline)) {
+        const bool in_v = group * kColumns + (tid & 7) * 8 < s.dv;
+        v_raw = fetch8<E>(vb, in_v ? row_at + group * kColumns * kSize : kOutside);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int e = group * kColumns + 32 * i + 8 * g;
+            const uint32_t cell = e < s.dv ? cell_at + (group * kColumns + 32 * i) * 4 : kOutside;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s_raw[i][h] = fetch16(sb, cell + 16 * h);
+                d_raw[i][h] = fetch16(db, cell + 16 * h);
+            }
+        }
+    };
+    const auto stage_rows = [&]() __attribute__((always_inline)) {
+        ot.template put8<E>(tid >> 3, (tid & 7) * 8, o_raw);
+        ut.template put8<ElemF32>(tid >> 3, (tid & 7) * 8, u_raw);
+        rt.template put8<ElemF32>(tid >> 3, (tid & 7) * 8, r_raw);
+    };
+
+    {
+        const int64_t copy = (block * s.key_heads + key_head) * kBlock * DK;
+        const Buffer kb = buffer_of(k + copy, kBlock * DK * kSize), qb = buffer_of(q + copy, kBlock * DK * kSize);
+        const Buffer gb = buffer_of(gates + entry * kGateFloats, kGateFloats * 4);
+        Eight<E> k_raw[DK / 64], q_raw[DK / 64];
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) {
+            k_raw[i] = fetch8<E>(kb, (tid + 512 * i) * 8 * kSize);
+            q_raw[i] = fetch8<E>(qb, (tid + 512 * i) * 8 * kSize);
+        }
+        const float gate_raw = fetch4(gb, tid * 4);
+        load_rows(0);
+        load_states(0);
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) {
+            const int row = (tid + 512 * i) / (DK / 8), d = (tid + 512 * i) % (DK / 8) * 8;
+            kt.template put8<E>(row, d, k_raw[i]);
+            qt.template put8<E>(row, d, q_raw[i]);
+        }
+        if (tid < kGateFloats) gate[tid] = gate_raw;
+    }
+
+    fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B: own tokens, own features
+    float value_dot = 0.0f, whole_term = 0.0f;
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
+#pragma unroll 1
+    for (int group = 0; group < groups; ++group) {
+        if (group > 0) lds_barrier();
+        stage_rows();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) value_dot += r_raw.v[i] * E::get(v_raw.v[i]);
+        Operand<NS> so[2], dd[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            so[i] = operand_of<NS>(s_raw[i][0], s_raw[i][1]);
+            dd[i] = operand_of<NS>(d_raw[i][0], d_raw[i][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) whole_term += s_raw[i][h][e] * d_raw[i][h][e];
+        }
+        lds_barrier();
+        // (behind the last group the one before it, which the products of tokens take next)
+        load_rows(group + 1 < groups ? group + 1 : (groups > 1 ? groups - 2 : 0));
+        if (group + 1 < groups) load_states(group + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int e = group * kColumns + 32 * i + 8 * g + 4 * h;
-                const uint32_t cell = e < s.dv ? ((feature0 + c) * s.dv + e) * 4 : kOutside;
-                s_raw[i][h] = fetch16(sb, cell);
-                d_raw[i][h] = fetch16(db, cell);
+            for (int t = 0; t < kTok; ++t) {
+                const int row = 16 * (tile0 + t) + c;
+                x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
+                a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
+                b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
             }
-    };
-    const auto stage_rows = [&]() {
-        const int row = tid >> 3, d = (tid & 7) * 8;
-        ot.template put8<E>(row, d, o_raw);
-        ut.template put8<ElemF32>(row, d, u_raw);
-        rt.template put8<ElemF32>(row, d, r_raw);
-    };
-    float* const mine = sums + (((block * s.key_heads + key_head) * 16 + wave) * kTok * 64 + lane) * 4;  // dK's half is 8 waves on
-
-#pragma unroll 1
-    for (int head = key_head * share; head < (key_head + 1) * share; ++head) {
-        const int64_t entry = block * s.heads + head;
-        fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B of the head: own tokens, own features
-        float value_dot = 0.0f, whole_term = 0.0f;
+    }
+    // Tokens against tokens, from the last group of columns back: tile `own` against all in dO U^T (waves 0 to 3) or
+    // dR U^T (4 to 7), with the own tokens as columns and earlier ones as rows, and with the own tokens as columns,
+    // where the other factor is U, and later ones as rows.
+    const int own = wave & 3;
+    const bool second = wave >= 4;
+    fx4 early[kTiles], late[kTiles];
 #pragma unroll
-        for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
-        load_rows(head, 0);
-        load_states(head, 0);
+    for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
 #pragma unroll 1
-        for (int group = 0; group < groups; ++group) {
+    for (int group = groups - 1; group >= 0; --group) {
+        if (group < groups - 1) {
             lds_barrier();
-            if (group == 0 && tid < kGateFloats) gate[tid] = gates[entry * kGateFloats + tid];
             stage_rows();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) value_dot += r_raw.v[i] * E::get(v_raw.v[i]);
-            Operand<NS> so[2], dd[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                so[i] = operand_of<NS>(s_raw[i][0], s_raw[i][1]);
-                dd[i] = operand_of<NS>(d_raw[i][0], d_raw[i][1]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) whole_term += s_raw[i][h][e] * d_raw[i][h][e];
-            }
             lds_barrier();
-            // (behind the last group the one before it, which the products of tokens take next)
-            const int next = group + 1 < groups ? group + 1 : (groups > 1 ? groups - 2 : 0);
-            load_rows(head, next);
-            load_states(head, next);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int t = 0; t < kTok; ++t) {
-                    const int row = 16 * (tile0 + t) + c;
-                    __builtin_amdgcn_sched_barrier(0);
-                    x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
-                    a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
-                    b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
-                }
-        }
-        // Tokens against tokens, from the last group of columns back: tile `own` against all in dO U^T (waves 0 to 3) or
-        // dR U^T (4 to 7), with the own tokens as columns and earlier ones as rows, and with the own tokens as columns,
-        // where the other factor is U, and later ones as rows.
-        const int own = wave & 3;
-        const bool second = wave >= 4;
-        fx4 early[kTiles], late[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
-#pragma unroll 1
-        for (int group = groups - 1; group >= 0; --group) {
-            if (group < groups - 1) {
-                lds_barrier();
-                stage_rows();
-                lds_barrier();
-                load_rows(head, group > 0 ? group - 1 : 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                __builtin_amdgcn_sched_barrier(0);
-                const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
-                if (!second) {
-                    const Operand<NI> o = ot.along(16 * own + c, 32 * i, g);
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
-                        if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
-                    }
-                } else {
-                    const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
-                        if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
-                    }
-                }
-            }
-        }
-
-        // weighted, the products of tokens go to all waves
-        lds_barrier();
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int there = 16 * t + 4 * g + r, here = 16 * own + c;
-                const float far = (gate[kSumHigh * kBlock + here] - gate[kSumHigh * kBlock + there]) +
-                                  (gate[kSumLow * kBlock + here] - gate[kSumLow * kBlock + there]);
-                if (!second) {
-                    early[t][r] = there <= here ? s.scale * exp_of(far) * early[t][r] : 0.0f;
-                    late[t][r] = there >= here ? s.scale * exp_of(-far) * late[t][r] : 0.0f;
-                } else {
-                    early[t][r] = there < here ? -exp_of(far) * early[t][r] : 0.0f;
-                    late[t][r] = there > here ? -gate[kBeta * kBlock + there] * exp_of(-far) * late[t][r] : 0.0f;
-                }
-            }
-            const Exchange<NS, kPairs>&rows = second ? l_rows : f_rows, &cols = second ? l_cols : f_cols;
-            if (t <= (own | 1)) Exchange<NS, kPairs>(rows).put(2 * pair_lower(own, t >> 1) + (t & 1), lane, early[t]);
-            if (t >= (own & 2)) Exchange<NS, kPairs>(cols).put(2 * pair_upper(own, t >> 1) + (t & 1), lane, late[t]);
-        }
-        lds_barrier();
-        fx4 carried = {0, 0, 0, 0};
-        Operand<NI> ko[2], qo[2];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            ko[p] = kt.down(32 * p, feature0, lane);
-            qo[p] = qt.down(32 * p, feature0, lane);
+            load_rows(group > 0 ? group - 1 : 0);
         }
 #pragma unroll
-        for (int t = 0; t < kTok; ++t) {
-            const int tile = tile0 + t;
-            __builtin_amdgcn_sched_barrier(0);  // (a tile at a time: the registers of two would not fit)
-            // factors of the parts that went through the state
-            const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * tile + 4 * g);
-            const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * tile + 4 * g);
-            const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * tile + 4 * g);
-            const fx4 kv = kt.tile(16 * tile, feature0, lane), qv = qt.tile(16 * tile, feature0, lane);
+        for (int i = 0; i < 2; ++i) {
+            const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
+            if (!second) {
+                const Operand<NI> o = ot.along(16 * own + c, 32 * i, g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                x[t][r] *= s.scale * since[r];
-                a[t][r] *= -since[r];
-                b[t][r] *= until[r];
-                carried[r] += kv[r] * b[t][r];
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                if (p <= (tile >> 1)) {
-                    x[t] = mma<NS, NI>(f_rows.get(pair_lower(tile, p), lane), ko[p], x[t]);
-                    a[t] = mma<NS, NI>(l_rows.get(pair_lower(tile, p), lane), ko[p], a[t]);
+                for (int t = 0; t < kTiles; ++t) {
+                    if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
+                    if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
                 }
-                if (p >= (tile >> 1)) {
-                    b[t] = mma<NS, NI>(f_cols.get(pair_upper(tile, p), lane), qo[p], b[t]);
-                    b[t] = mma<NS, NI>(l_cols.get(pair_upper(tile, p), lane), ko[p], b[t]);
-                }
-            }
+            } else {
+                const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float dq = sum16(qv[r] * x[t][r]), da = sum16(kv[r] * a[t][r]), db = sum16(kv[r] * b[t][r]);
-                if (c == 0) {
-                    dots[wave][0][16 * t + 4 * g + r] = dq;
-                    dots[wave][1][16 * t + 4 * g + r] = da;
-                    dots[wave][2][16 * t + 4 * g + r] = db;
-                }
-                b[t][r] += beta[r] * a[t][r];  // dK
-            }
-        }
-        // over the heads that share the keys: by way of memory, where this wave alone reads what it wrote
-        if (head > key_head * share) {
-#pragma unroll
-            for (int t = 0; t < kTok; ++t) {
-                x[t] += *reinterpret_cast<const fx4*>(mine + t * 256);
-                b[t] += *reinterpret_cast<const fx4*>(mine + (8 * kTok + t) * 256);
-            }
-        }
-        if (head + 1 < (key_head + 1) * share) {
-#pragma unroll
-            for (int t = 0; t < kTok; ++t) {
-                *reinterpret_cast<fx4*>(mine + t * 256) = x[t];
-                *reinterpret_cast<fx4*>(mine + (8 * kTok + t) * 256) = b[t];
-            }
-        } else {
-            const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-            const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
-#pragma unroll
-            for (int t = 0; t < kTok; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t to = feature0 + c < s.dk ? (16 * (tile0 + t) + 4 * g + r) * k_step + (feature0 + c) * kSize : kOutside;
-                    put1<E>(qb, to, x[t][r]);
-                    put1<E>(kb, to, b[t][r]);
-                }
-        }
-        whole_term = tile0 == 0 ? whole_term * gate[kSince * kBlock + kBlock - 1] : 0.0f;  // a cell counts once
-#pragma unroll
-        for (int r = 0; r < 4; ++r) whole_term += carried[r];
-        whole_term = sum16(whole_term);
-        whole_term += __shfl_xor(whole_term, 16);
-        whole_term += __shfl_xor(whole_term, 32);
-        if (lane == 0) whole_terms[wave] = whole_term;
-        value_dot += __shfl_xor(value_dot, 1);
-        value_dot += __shfl_xor(value_dot, 2);
-        value_dot += __shfl_xor(value_dot, 4);
-        if ((tid & 7) == 0) value_dots[tid >> 3] = value_dot;
-        lds_barrier();
-        if (wave == 0) {
-            // token `lane`: over the tiles of features, then the sums from it on
-            float dq = 0.0f, da = 0.0f, db = 0.0f, whole = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kFeatures; ++i) {
-                const int w = lane / (16 * kTok) * kFeatures + i;
-                dq += dots[w][0][lane % (16 * kTok)];
-                da += dots[w][1][lane % (16 * kTok)];
-                db += dots[w][2][lane % (16 * kTok)];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) whole += whole_terms[i];
-            float sum = dq + gate[kBeta * kBlock + lane] * da - db;
-#pragma unroll
-            for (int d = 1; d < 64; d *= 2) {
-                const float y = __shfl_down(sum, d);
-                if (lane + d < 64) sum += y;
-            }
-            sum += whole;
-            if (lane < length) {
-                const int64_t to = (row0 + lane) * s.heads + head;
-                if (s.wide_gates) {
-                    static_cast<float*>(d_log_gates)[to] = sum;
-                    static_cast<float*>(d_beta)[to] = value_dots[lane] + da;
-                } else {
-                    static_cast<ES*>(d_log_gates)[to] = E::put(sum);
-                    static_cast<ES*>(d_beta)[to] = E::put(value_dots[lane] + da);
+                for (int t = 0; t < kTiles; ++t) {
+                    if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
+                    if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
                 }
             }
         }
     }
+
+    // weighted, the products of tokens go to all waves
+    lds_barrier();
+    {
+        const int here = 16 * own + c;
+        const float high = gate[kSumHigh * kBlock + here], low = gate[kSumLow * kBlock + here];
+        Exchange<NS, kPairs> rows = second ? l_rows : f_rows, cols = second ? l_cols : f_cols;
+        const float factor = second ? -1.0f : s.scale;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            const int there0 = 16 * t + 4 * g;
+            const fx4 h = *reinterpret_cast<const fx4*>(gate + kSumHigh * kBlock + there0);
+            const fx4 l = *reinterpret_cast<const fx4*>(gate + kSumLow * kBlock + there0);
+            if (t <= (own | 1)) {
+                fx4 e = {0, 0, 0, 0};
+                if (t <= own) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w = factor * exp_of((high - h[r]) + (low - l[r]));
+                        e[r] = there0 + r < here + (second ? 0 : 1) ? w * early[t][r] : 0.0f;
+                    }
+                }
+                rows.put(2 * pair_lower(own, t >> 1) + (t & 1), lane, e);
+            }
+            if (t >= (own & 2)) {
+                fx4 e = {0, 0, 0, 0};
+                if (t >= own) {
+                    const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + there0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w = factor * (second ? beta[r] : 1.0f) * exp_of((h[r] - high) + (l[r] - low));
+                        e[r] = there0 + r > here - (second ? 0 : 1) ? w * late[t][r] : 0.0f;
+                    }
+                }
+                cols.put(2 * pair_upper(own, t >> 1) + (t & 1), lane, e);
+            }
+        }
+    }
+    lds_barrier();
+    float carried = 0.0f;
+    Operand<NI> ko[2], qo[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        ko[p] = kt.down(32 * p, feature0, lane);
+        qo[p] = qt.down(32 * p, feature0, lane);
+    }
+    const uint32_t to0 = feature0 + c < s.dk ? (16 * tile0 + 4 * g) * k_step + (feature0 + c) * kSize : kOutside;
+    const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+    const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
+    float* const mine = sums + ((entry * 16 + wave) * kTok * 64 + lane) * 4;  // dK's half is 8 waves on
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {
+        const int tile = tile0 + t;
+        // factors of the parts that went through the state
+        const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * tile + 4 * g);
+        const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * tile + 4 * g);
+        const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * tile + 4 * g);
+        const fx4 kv = kt.tile(16 * tile, feature0, lane), qv = qt.tile(16 * tile, feature0, lane);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            x[t][r] *= s.scale * since[r];
+            a[t][r] *= -since[r];
+            b[t][r] *= until[r];
+            carried += kv[r] * b[t][r];
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            if (p <= (tile >> 1)) {
+                x[t] = mma<NS, NI>(f_rows.get(pair_lower(tile, p), lane), ko[p], x[t]);
+                a[t] = mma<NS, NI>(l_rows.get(pair_lower(tile, p), lane), ko[p], a[t]);
+            }
+            if (p >= (tile >> 1)) {
+                b[t] = mma<NS, NI>(f_cols.get(pair_upper(tile, p), lane), qo[p], b[t]);
+                b[t] = mma<NS, NI>(l_cols.get(pair_upper(tile, p), lane), ko[p], b[t]);
+            }
+        }
+        fx4 dc, da;  // of the own features: q.dQ + beta k.A - k.B and k.A
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float ka = kv[r] * a[t][r];
+            dc[r] = sum16(qv[r] * x[t][r] + (beta[r] * ka - kv[r] * b[t][r]));
+            da[r] = sum16(ka);
+            b[t][r] += beta[r] * a[t][r];  // dK
+        }
+        if (c == 0) {
+            *reinterpret_cast<fx4*>(&dots[wave][0][16 * t + 4 * g]) = dc;
+            *reinterpret_cast<fx4*>(&dots[wave][1][16 * t + 4 * g]) = da;
+        }
+        if constexpr (SHARED) {
+            *reinterpret_cast<fx4*>(mine + t * 256) = x[t];
+            *reinterpret_cast<fx4*>(mine + (8 * kTok + t) * 256) = b[t];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                put1<E>(qb, to0 + (16 * t + r) * k_step, x[t][r]);
+                put1<E>(kb, to0 + (16 * t + r) * k_step, b[t][r]);
+            }
+        }
+    }
+    whole_term = tile0 == 0 ? whole_term * gate[kSince * kBlock + kBlock - 1] : 0.0f;  // a cell counts once
+    whole_term = sum16(whole_term + carried);
+    whole_term += __shfl_xor(whole_term, 16);
+    whole_term += __shfl_xor(whole_term, 32);
+    if (lane == 0) whole_terms[wave] = whole_term;
+    value_dot += __shfl_xor(value_dot, 1);
+    value_dot += __shfl_xor(value_dot, 2);
+    value_dot += __shfl_xor(value_dot, 4);
+    if ((tid & 7) == 0) value_dots[tid >> 3] = value_dot;
+    lds_barrier();
+    if (wave == 0) {
+        // token `lane`: over the tiles of features, then the sums from it on
+        float dc = 0.0f, da = 0.0f, whole = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFeatures; ++i) {
+            const int w = lane / (16 * kTok) * kFeatures + i;
+            dc += dots[w][0][lane % (16 * kTok)];
+            da += dots[w][1][lane % (16 * kTok)];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) whole += whole_terms[i];
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const float y = __shfl_down(dc, d);
+            if (lane + d < 64) dc += y;
+        }
+        dc += whole;
+        if (lane < length) {
+            const int64_t to = (row0 + lane) * s.heads + head;
+            if (s.wide_gates) {
+                static_cast<float*>(d_log_gates)[to] = dc;
+                static_cast<float*>(d_beta)[to] = value_dots[lane] + da;
+            } else {
+                static_cast<ES*>(d_log_gates)[to] = E::put(dc);
+                static_cast<ES*>(d_beta)[to] = E::put(value_dots[lane] + da);
+            }
+        }
+    }
+}
+
+// dQ and dK of a block and key head: the sums of the heads that share it, in their order.
+// grid (blocks, key heads), 512 threads, which hold what the ones of delta_gradients do.
+template <class E, int DK>
+__global__ __launch_bounds__(512) void delta_fold(DeltaShape s, const float* __restrict__ sums,
+                                                  typename E::S* __restrict__ d_q, typename E::S* __restrict__ d_k) {
+    constexpr int kFeatures = DK / 16, kTok = DK / 32;
+    const int64_t block = blockIdx.x;
+    const int key_head = blockIdx.y, share = s.heads / s.key_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const BlockAt found = block_at(s, block);
+    if (found.length <= 0) return;
+    const int feature = 16 * (wave & (kFeatures - 1)) + c, tile0 = kFeatures == 8 ? 0 : (wave >> 2) * kTok;
+    const float* from = sums + (((block * s.heads + key_head * share) * 16 + wave) * kTok * 64 + lane) * 4;
+    fx4 x[kTok], b[kTok];
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) x[t] = b[t] = fx4{0, 0, 0, 0};
+    for (int h = 0; h < share; ++h, from += 16 * kTok * 256) {
+#pragma unroll
+        for (int t = 0; t < kTok; ++t) {
+            x[t] += *reinterpret_cast<const fx4*>(from + t * 256);
+            b[t] += *reinterpret_cast<const fx4*>(from + (8 * kTok + t) * 256);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kTok; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * (tile0 + t) + 4 * g + r;
+            if (row < found.length && feature < s.dk) {
+                const int64_t to = ((found.row + row) * s.key_heads + key_head) * s.dk + feature;
+                d_q[to] = E::put(x[t][r]);
+                d_k[to] = E::put(b[t][r]);
+            }
+        }
 }
 
 }  // namespace

@@ -34,7 +34,7 @@ struct DeltaParts {
         d_states = round_up(q + copy);
         d_rows = round_up(d_states + (backward ? entries * s.dk * s.dv * 4 : 0));
         sums = round_up(d_rows + (backward ? (size_t)s.rows * s.heads * s.dv * 4 : 0));
-        end = round_up(sums + (backward && s.heads > s.key_heads ? (size_t)s.blocks * s.key_heads * 2 * kBlock * (s.dk <= 64 ? 64 : 128) * 4 : 0));
+        end = round_up(sums + (backward && s.heads > s.key_heads ? entries * 2 * kBlock * (s.dk <= 64 ? 64 : 128) * 4 : 0));
     }
 };
 
@@ -88,12 +88,18 @@ int delta_backward_dk(const DeltaBackward& f) {
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows);
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
-    return delta_status(delta_launch(
-        delta_gradients<E, NI, NS, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), 512, kGradientBytes<NI, NS, DK>,
-        f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k), static_cast<const S*>(f.v),
-        static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
-        static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates, f.d_beta,
-        reinterpret_cast<float*>(ws + at.sums)));
+    const bool shared = s.heads > s.key_heads;
+    const auto kernel = shared ? delta_gradients<E, NI, NS, DK, true> : delta_gradients<E, NI, NS, DK, false>;
+    float* sums = reinterpret_cast<float*>(ws + at.sums);
+    e = delta_launch(kernel, dim3((unsigned)s.blocks, (unsigned)s.heads), 512, kGradientBytes<NI, NS, DK>, f.stream, s,
+                     reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k), static_cast<const S*>(f.v),
+                     static_cast<const S*>(f.d_out), gates, f.states, f.updates, static_cast<const float*>(d_states),
+                     static_cast<const float*>(d_rows), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k), f.d_log_gates,
+                     f.d_beta, sums);
+    if (e == hipSuccess && shared)
+        e = delta_launch(delta_fold<E, DK>, dim3((unsigned)s.blocks, (unsigned)s.key_heads), 512, 0, f.stream, s,
+                         static_cast<const float*>(sums), static_cast<S*>(f.d_q), static_cast<S*>(f.d_k));
+    return delta_status(e);
 }
 
 template <class E, int Q, int N>
