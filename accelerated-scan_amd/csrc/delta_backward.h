@@ -21,14 +21,15 @@ namespace {
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
 template <int NI, int NS, int DK>
-constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                              3 * Exchange<NS, 2>::kBytes;
+constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
+                              2 * Exchange<NS, 2>::kBytes + (8 + DK / 16) * 1024 + kMatrixBytes<NS> + 4 * kBlock * 4;
 
-// The chain, last block first, divided like the forward one: 16 columns of D to a workgroup, wave w keeps rows
-// dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.
-// q and k: the copies that delta_prepare made.  grid chain_grid(), 256 threads.
+// The chain, last block first, divided like the forward one: 16 columns of D to a workgroup; state wave w keeps rows
+// dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.  Four waves
+// compute what does not wait for D (P^T dO and Q^T diag(scale e^c) dO) and write what leaves the chain, four load.
+// q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.
 template <class E, int NI, int NS, int DK>
-__global__ __launch_bounds__(256, 2) void delta_reverse_chain(
+__global__ __launch_bounds__(768) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
     const char* __restrict__ p_in, const float* __restrict__ d_final, typename E::S* __restrict__ d_v,
@@ -40,206 +41,297 @@ __global__ __launch_bounds__(256, 2) void delta_reverse_chain(
     if (!where.there) return;
     const int64_t n = where.sequence;
     const int head = where.head, key_head = head / (s.heads / s.key_heads);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
+    const int role = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
     const int col0 = where.col0, col = col0 + c;
     const bool mine = col < s.dv;
     const SequenceAt at = sequence_at(s, n);
 
-    // (queries are read between the second and the third barrier only: one tile is enough)
+    // Keys, values' gradients: two blocks' room.  Queries are wanted between the second and the third barrier, T and the
+    // gates in front of the second one only: room for one block.
     char* m = smem + 2 * Tile<NI, DK>::kBytes;
     const Tile<NI, DK> qt(m);
     m += Tile<NI, DK>::kBytes;
-    const Tile<NI, 16> ot(m);
-    m += Tile<NI, 16>::kBytes;
+    char* const ot_at = m;
+    m += 2 * Tile<NI, 16>::kBytes;
     Exchange<NS, kDepths> xs(m);
     m += Exchange<NS, kDepths>::kBytes;
-    Exchange<NS, 2> xr(m), xw(m + Exchange<NS, 2>::kBytes), xu(m + 2 * Exchange<NS, 2>::kBytes);
-
-    fx4 D[kOwn];
-    const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
-#pragma unroll
-    for (int t = 0; t < kOwn; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = feature_row(kOwn * wave + t, g, r);
-            D[t][r] = d_final != nullptr && mine && row < s.dk ? d_final[state_at + (int64_t)row * s.dv] : 0.0f;
-        }
+    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes);
+    m += 2 * Exchange<NS, 2>::kBytes;
+    fx4* const po_at = reinterpret_cast<fx4*>(m) + lane;  // accumulator tiles from wave to wave, a KiB each
+    fx4* const qw_at = po_at + 4 * 64;
+    fx4* const dr_at = qw_at + 4 * kOwn * 64;
+    m += (8 + DK / 16) * 1024;
+    char* const matrix_at = m;
+    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NS>);
 
     constexpr uint32_t kSize = sizeof(ES);
+    constexpr int kKeyBytes = kBlock * DK * kSize;
     const uint32_t v_step = s.heads * s.dv * kSize, r_step = s.heads * s.dv * 4;
     const int64_t seq_row = uniform(at.row), seq_length = uniform(at.length), seq_block = uniform(at.block);
+    const int64_t last = (seq_length - 1) / kBlock;  // number of the last block
     const int token = 16 * wave + c;
-    const auto rows_of = [&](const void* p, int64_t first, uint32_t step, int64_t at_head, uint32_t bytes) {
-        const int64_t left = seq_length - first < kBlock ? seq_length - first : kBlock;
-        return buffer_of(static_cast<const char*>(p) + (seq_row + first) * step + at_head, (left - 1) * (int64_t)step + bytes);
+    const auto rows_of = [&](const char* p, int64_t n_block, uint32_t step, uint32_t bytes) {
+        const int64_t left = seq_length - n_block * kBlock;
+        return buffer_of(p, n_block < 0 ? 0 : ((left < kBlock ? (int)left : kBlock) - 1) * (int)step + (int)bytes);
     };
-    const auto entry_of = [&](int64_t first) { return (seq_block + first / kBlock) * s.heads + head; };
-    Eight<E> k_raw[kCopies], q_raw[kCopies], o_raw;
-    Operand<NS> tm[2], pm[2];
-    fx4 beta, beta_since, until, since;
-    float whole;
-    const auto load_rows = [&](int64_t first) {
-        const int64_t copy = ((seq_block + first / kBlock) * s.key_heads + key_head) * kBlock * DK;
-        const Buffer kb = buffer_of(k + copy, kBlock * DK * kSize), qb = buffer_of(q + copy, kBlock * DK * kSize);
-        const Buffer ob = d_out != nullptr ? rows_of(d_out, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize) : buffer_of(k, 0);
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            k_raw[i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
-            q_raw[i] = fetch8<E>(qb, (tid + 256 * i) * 8 * kSize);
-        }
-        const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
-        o_raw = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+    const auto start_of = [&](const void* p, uint32_t step, int64_t at_head) {
+        return static_cast<const char*>(p) + (seq_row + last * kBlock) * step + at_head;
     };
-    // (waves 2 and 3 have one operand to a row of tiles: their first load repeats the second)
-    const auto load_matrix = [&](const char* from, int64_t first, Operand<NS>(&o)[2]) {
-        const Buffer b = buffer_of(from + entry_of(first) * kMatrixBytes<NS>, kMatrixBytes<NS>);
-        o[0] = matrix_operand<NS>(b, pair_upper(wave, wave < 2 ? 0 : 1), lane);
-        o[1] = matrix_operand<NS>(b, pair_upper(wave, 1), lane);
-    };
-    const auto gates_of = [&](int64_t first) { return buffer_of(gates + entry_of(first) * kGateFloats, kGateFloats * 4); };
-    const uint32_t gate_rows = (16 * wave + 4 * g) * 4;
+    const int64_t entry0 = (seq_block + last) * s.heads + head;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
+    const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
+    const auto keys_at = [&](int64_t n_block) { return Tile<NI, DK>(smem + (n_block & 1) * Tile<NI, DK>::kBytes); };
+    const auto outs_at = [&](int64_t n_block) { return Tile<NI, 16>(ot_at + (n_block & 1) * Tile<NI, 16>::kBytes); };
+    const auto gate_rows = [&](int row) { return *reinterpret_cast<const fx4*>(gate + row * kBlock + 16 * wave + 4 * g); };
 
-    const int64_t last = (seq_length - 1) / kBlock * kBlock;
-    if (seq_length > 0) {  // (an empty sequence has no table entry to read)
-        load_rows(last);
-        load_matrix(p_in, last, pm);
-        const Buffer b = gates_of(last);
-        until = fetch16(b, kUntil * 256 + gate_rows);
-        since = fetch16(b, kSince * 256 + gate_rows);
-        load_matrix(t_in, last, tm);
-        beta = fetch16(b, kBeta * 256 + gate_rows);
-        beta_since = fetch16(b, kBetaSince * 256 + gate_rows);
-        whole = fetch4(b, kSince * 256 + (c | 63) * 4);
-    }
-    for (int64_t first = last; first >= 0 && seq_length > 0; first -= kBlock) {
-        const int64_t ahead = first > 0 ? first - kBlock : 0;
-        const Buffer gb = gates_of(ahead);
-        const Tile<NI, DK> kb(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes);
-        {
-            const Buffer to = buffer_of(d_states + entry_of(first) * s.dk * s.dv, (int64_t)s.dk * s.dv * 4);
-#pragma unroll
-            for (int t = 0; t < kOwn; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, D[t][r]);
-        }
-#pragma unroll
-        for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, D[t]);
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int row = (tid + 256 * i) / (DK / 8), d = (tid + 256 * i) % (DK / 8) * 8;
-            kb.template put8<E>(row, d, k_raw[i]);
-            qt.template put8<E>(row, d, q_raw[i]);
-        }
-        ot.template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw);
-        lds_barrier();
-
-        // dU = diag(e^(c[63]-c)) K D1 + P^T dO
-        fx4 u = {0, 0, 0, 0}, w;
-        {
-            Operand<NS> so[kDepths];
-            Operand<NI> ko[kDepths];
-#pragma unroll
-            for (int d = 0; d < kDepths; ++d) {
-                so[d] = xs.get(d, lane);
-                ko[d] = kb.along(token, 32 * d, g);
-            }
-            const Operand<NI> o_low = ot.down(0, 0, lane), o_high = ot.down(32, 0, lane);
-            w = ot.tile(16 * wave, 0, lane);
-            load_rows(ahead);
-            __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
-            fx4 po = {0, 0, 0, 0};
-            if (wave < 2) po = mma<NS, NI>(pm[0], o_low, po);
-            po = mma<NS, NI>(pm[1], o_high, po);
-            fx4 u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-#pragma unroll
-            for (int d = 0; d < kDepths; d += 2) {
-                u = mma<NI, NS>(ko[d], so[d], u);
-                u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
-            }
-            load_matrix(p_in, ahead, pm);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                u[r] = until[r] * (u[r] + u2[r]) + po[r];
-                w[r] *= s.scale * since[r];
-            }
-        }
-        xr.put(wave, lane, u);
-        xw.put(wave, lane, w);
-        until = fetch16(gb, kUntil * 256 + gate_rows);
-        since = fetch16(gb, kSince * 256 + gate_rows);
-        lds_barrier();
-
-        // dR = dU + T^T dU;  D0 = e^c[63] D1 + Q^T diag(scale e^c) dO while it waits
-        fx4 x;
-        {
-            const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane), w_low = xw.get(0, lane), w_high = xw.get(1, lane);
-            Operand<NI> q_low[kOwn], q_high[kOwn];
-#pragma unroll
-            for (int t = 0; t < kOwn; ++t) {
-                q_low[t] = qt.down_features(0, kOwn * wave + t, lane);
-                q_high[t] = qt.down_features(32, kOwn * wave + t, lane);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            u = mma<NS, NS>(tm[1], high, u);
-            if (wave < 2) {
-                const fx4 more = mma<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
-#pragma unroll
-                for (int r = 0; r < 4; ++r) u[r] += more[r];
-            }
-#pragma unroll
-            for (int t = 0; t < kOwn; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) D[t][r] *= whole;
-                D[t] = mma<NI, NS>(q_low[t], w_low, D[t]);
-                D[t] = mma<NI, NS>(q_high[t], w_high, D[t]);
-            }
-        }
-        load_matrix(t_in, ahead, tm);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = -beta_since[r] * u[r];
-        xu.put(wave, lane, x);
-        beta_since = fetch16(gb, kBetaSince * 256 + gate_rows);
-        whole = fetch4(gb, kSince * 256 + (c | 63) * 4);
-        lds_barrier();
-
-        // D0 -= K^T diag(beta e^c) dR
-        {
-            const Operand<NS> low = xu.get(0, lane), high = xu.get(1, lane);
-            Operand<NI> k_low[kOwn], k_high[kOwn];
-#pragma unroll
-            for (int t = 0; t < kOwn; ++t) {
-                k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
-                k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int t = 0; t < kOwn; ++t) {
-                D[t] = mma<NI, NS>(k_low[t], low, D[t]);
-                D[t] = mma<NI, NS>(k_high[t], high, D[t]);
-            }
-        }
-        {
-            const Buffer to = rows_of(d_v, first, v_step, (int64_t)head * s.dv * kSize, s.dv * kSize);
-            const Buffer rows = rows_of(d_rows, first, r_step, (int64_t)head * s.dv * 4, s.dv * 4);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                put1<E>(to, mine ? (16 * wave + 4 * g + r) * v_step + col * kSize : kOutside, beta[r] * u[r]);
-                put1<ElemF32>(rows, mine ? (16 * wave + 4 * g + r) * r_step + col * 4 : kOutside, u[r]);
-            }
-        }
-        beta = fetch16(gb, kBeta * 256 + gate_rows);
-    }
-    if (d_initial != nullptr && mine) {
+    if (role == 0) {
+        fx4 D[kOwn];
+        const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
 #pragma unroll
         for (int t = 0; t < kOwn; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int row = feature_row(kOwn * wave + t, g, r);
-                if (row < s.dk) d_initial[state_at + (int64_t)row * s.dv] = D[t][r];
+                D[t][r] = d_final != nullptr && mine && row < s.dk ? d_final[state_at + (int64_t)row * s.dv] : 0.0f;
             }
+        __builtin_amdgcn_s_setprio(3);
+        Operand<NI> ko[kDepths];
+        const auto read_block = [&](int64_t n_block) {
+#pragma unroll
+            for (int d = 0; d < kDepths; ++d) ko[d] = keys_at(n_block).along(token, 32 * d, g);
+        };
+        if (seq_length > 0) {
+            lds_barrier();  // the last block is there
+            read_block(last);
+        }
+        for (int64_t now = last; now >= 0 && seq_length > 0; --now) {
+            const Tile<NI, DK> kb = keys_at(now);
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) xs.put(kOwn * wave + t, lane, D[t]);
+            lds_barrier();
+
+            // dU = diag(e^(c[63]-c)) K D1 + P^T dO
+            fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
+            Operand<NS> tm[2];
+            fx4 beta_since;
+            float whole;
+            {
+                Operand<NS> so[kDepths];
+#pragma unroll
+                for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
+                const fx4 po = po_at[wave * 64], until = gate_rows(kUntil);
+                tm[0] = matrix_operand<NS>(matrix_at, pair_upper(wave, wave >> 1), lane);
+                tm[1] = matrix_operand<NS>(matrix_at, pair_upper(wave, 1), lane);
+                beta_since = gate_rows(kBetaSince);
+                whole = gate[kSince * kBlock + kBlock - 1];
+                __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
+#pragma unroll
+                for (int d = 0; d < kDepths; d += 2) {
+                    u = mma<NI, NS>(ko[d], so[d], u);
+                    u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] = until[r] * (u[r] + u2[r]) + po[r];
+            }
+            xr.put(wave, lane, u);
+            lds_barrier();
+
+            // dR = dU + T^T dU; what the next products take of the keys is read on the way
+            Operand<NI> k_low[kOwn], k_high[kOwn];
+            {
+                const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
+#pragma unroll
+                for (int t = 0; t < kOwn; ++t) {
+                    k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
+                    k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                u = mma<NS, NS>(tm[1], high, u);
+                if (wave < 2) {
+                    u2 = mma<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) u[r] += u2[r];
+                }
+            }
+            {
+                fx4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = -beta_since[r] * u[r];
+                xu.put(wave, lane, y);
+            }
+            dr_at[wave * 64] = u;
+            lds_barrier();
+
+            // D0 = e^c[63] D1 + Q^T diag(scale e^c) dO - K^T diag(beta e^c) dR
+            {
+                const Operand<NS> low = xu.get(0, lane), high = xu.get(1, lane);
+                fx4 qw[kOwn], D2[kOwn];
+#pragma unroll
+                for (int t = 0; t < kOwn; ++t) qw[t] = qw_at[(kOwn * wave + t) * 64];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < kOwn; ++t) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) D[t][r] *= whole;
+                    D[t] = mma<NI, NS>(k_low[t], low, D[t]);
+                    D2[t] = mma<NI, NS>(k_high[t], high, qw[t]);
+                }
+                read_block(now > 0 ? now - 1 : now);
+#pragma unroll
+                for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) D[t][r] += D2[t][r];
+            }
+        }
+        if (seq_length > 0 && (last & 1) == 0) {  // the other waves go on by two blocks
+            lds_barrier();
+            lds_barrier();
+            lds_barrier();
+        }
+        if (d_initial != nullptr && mine) {
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = feature_row(kOwn * wave + t, g, r);
+                    if (row < s.dk) d_initial[state_at + (int64_t)row * s.dv] = D[t][r];
+                }
+        }
+    } else if (role == 1 && seq_length > 0) {
+        // In front of the first block loads repeat it or give zero and stores are dropped: no condition stands around them.
+        Operand<NS> pm[2][2];
+        const char* p_p = p_in + entry0 * kMatrixBytes<NS>;
+        char* state_p = reinterpret_cast<char*>(d_states + entry0 * s.dk * s.dv);
+        const int quad = col0 + 4 * g;
+        char *v_p = const_cast<char*>(start_of(d_v, v_step, (int64_t)head * s.dv * kSize));
+        char *r_p = const_cast<char*>(start_of(d_rows, r_step, (int64_t)head * s.dv * 4));
+        const auto load_p = [&](int64_t n_block, int set) __attribute__((always_inline)) {
+            const Buffer b = buffer_of(p_p, kMatrixBytes<NS>);
+            pm[set][0] = matrix_operand<NS>(b, wave < 2 ? pair_upper(wave, 0) : (int)(kOutside >> 12), lane);
+            pm[set][1] = matrix_operand<NS>(b, pair_upper(wave, 1), lane);
+            if (n_block > 0) p_p -= matrix_move;
+        };
+        const auto outputs = [&](int64_t n_block, int set) __attribute__((always_inline)) {  // P^T dO
+            const Tile<NI, 16> ot = outs_at(n_block);
+            fx4 po = mma<NS, NI>(pm[set][1], ot.down(32, 0, lane), fx4{0, 0, 0, 0});
+            if (wave < 2) po = mma<NS, NI>(pm[set][0], ot.down(0, 0, lane), po);
+            po_at[wave * 64] = po;
+        };
+        load_p(last, 0);
+        load_p(last - 1, 1);
+        lds_barrier();
+        outputs(last, 0);
+        load_p(last - 2, 0);
+        const auto block = [&](int64_t now, int other) __attribute__((always_inline)) {  // the next block's P is in `other`
+            lds_barrier();
+            // W = diag(scale e^c) dO as the right operand, and the state behind the block for the kernel that follows
+            fx4 w[kTiles];
+            const Tile<NI, 16> ot = outs_at(now);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                const fx4 f = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * t + 4 * g);
+                w[t] = ot.tile(16 * t, 0, lane);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[t][r] *= s.scale * f[r];
+            }
+            const float beta = gate[kBeta * kBlock + token];
+            const Operand<NS> w_low = operand_of<NS>(w[0], w[1]), w_high = operand_of<NS>(w[2], w[3]);
+            {
+                const Buffer to = buffer_of(state_p, now >= 0 ? (int64_t)s.dk * s.dv * 4 : 0);
+#pragma unroll
+                for (int t = kOwn * wave; t < kOwn * wave + kOwn; ++t)
+                    put4<ElemF32>(to, quad < s.dv ? (feature_row(t, c >> 2, c & 3) * s.dv + quad) * 4 : kOutside, exchanged_row(xs, t, lane));
+                state_p -= (int64_t)s.heads * s.dk * s.dv * 4;
+            }
+            lds_barrier();
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+                fx4 qw = mma<NI, NS>(qt.down_features(0, kOwn * wave + t, lane), w_low, fx4{0, 0, 0, 0});
+                qw = mma<NI, NS>(qt.down_features(32, kOwn * wave + t, lane), w_high, qw);
+                qw_at[(kOwn * wave + t) * 64] = qw;
+            }
+            lds_barrier();
+            outputs(now - 1, other);
+            load_p(now - 3, other);
+            // row `token` of dR, four columns, from the accumulators' order
+            const float* from = reinterpret_cast<const float*>(dr_at - lane + wave * 64 + (c >> 2) * 16 + 4 * g) + (c & 3);
+            const fx4 u = {from[0], from[4], from[8], from[12]};
+            put4<ElemF32>(rows_of(r_p, now, r_step, s.dv * 4), quad < s.dv ? token * r_step + quad * 4 : kOutside, u);
+            put4<E>(rows_of(v_p, now, v_step, s.dv * kSize), quad < s.dv ? token * v_step + quad * kSize : kOutside,
+                    fx4{beta * u[0], beta * u[1], beta * u[2], beta * u[3]});
+            v_p -= v_move;
+            r_p -= (int64_t)r_step * kBlock;
+        };
+        for (int64_t now = last; now >= 0; now -= 2) {
+            block(now, 1);
+            block(now - 1, 0);
+        }
+    } else if (seq_length > 0) {
+        // Keys, queries, dO, T and gates to LDS.
+        Eight<E> k_raw[2][kCopies], q_raw[2][kCopies], o_raw[2];
+        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
+        fx4 t_raw[2][kPieces];
+        float gate_raw[2];
+        const int64_t copy0 = ((seq_block + last) * s.key_heads + key_head) * kBlock * DK;
+        const char *k_p = reinterpret_cast<const char*>(k + copy0), *q_p = reinterpret_cast<const char*>(q + copy0);
+        const char* o_p = start_of(d_out, v_step, (int64_t)head * s.dv * kSize);
+        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const auto load_block = [&](int64_t n_block, int set) __attribute__((always_inline)) {
+            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NS>);
+            const Buffer ob = d_out != nullptr ? rows_of(o_p, n_block, v_step, s.dv * kSize) : buffer_of(k_p, 0);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
+                q_raw[set][i] = fetch8<E>(qb, (tid + 256 * i) * 8 * kSize);
+            }
+            const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
+            o_raw[set] = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            gate_raw[set] = fetch4(buffer_of(gate_p, kGateFloats * 4), tid * 4);
+            o_p -= v_move;
+            if (n_block > 0) {
+                k_p -= k_move;
+                q_p -= k_move;
+                t_p -= matrix_move;
+                gate_p -= gate_move;
+            }
+        };
+        const auto stage_block = [&](int64_t n_block, int set) __attribute__((always_inline)) {
+            const Tile<NI, DK> kb = keys_at(n_block);
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
+            outs_at(n_block).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw[set]);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
+            gate[tid] = gate_raw[set];
+        };
+        const auto stage_queries = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) qt.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, q_raw[set][i]);
+        };
+        load_block(last, 0);
+        load_block(last - 1, 1);
+        stage_block(last, 0);
+        stage_queries(0);
+        load_block(last - 2, 0);
+        lds_barrier();
+        const auto block = [&](int64_t now, int other) __attribute__((always_inline)) {
+            lds_barrier();
+            lds_barrier();
+            stage_block(now - 1, other);  // the readers of all but the queries are behind the second barrier
+            lds_barrier();
+            stage_queries(other);
+            load_block(now - 3, other);
+        };
+        for (int64_t now = last; now >= 0; now -= 2) {
+            block(now, 1);
+            block(now - 1, 0);
+        }
     }
-    if (s.offsets != nullptr && mine) {
+    if (s.offsets != nullptr && mine && role == 0) {
         const int own = 4 * wave + g;
         if (n == 0)
             for (int64_t row = own; row < offset_at(s, 0); row += 16) d_v[(row * s.heads + head) * s.dv + col] = E::put(0.0f);

@@ -84,7 +84,7 @@ int delta_backward_dk(const DeltaBackward& f) {
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 256, kReverseBytes<NI, NS, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NS, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows);
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);

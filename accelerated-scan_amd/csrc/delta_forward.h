@@ -101,8 +101,6 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     if (keeper) {
         fx4 S[kOwn];
         const int64_t state_at = (n * s.heads + head) * s.dk * s.dv + col;
-        [[maybe_unused]] char* state_p = reinterpret_cast<char*>(states + entry0 * s.dk * s.dv);
-        [[maybe_unused]] char* update_p = reinterpret_cast<char*>(updates + (seq_row * s.heads + head) * s.dv);
 #pragma unroll
         for (int t = 0; t < kOwn; ++t)
 #pragma unroll
@@ -187,14 +185,6 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
             {
                 const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
-                if constexpr (KEEP) {  // (the state in front of the block, while these come)
-                    const Buffer to = buffer_of(state_p, (int64_t)s.dk * s.dv * 4);
-#pragma unroll
-                    for (int t = 0; t < kOwn; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            put1<ElemF32>(to, mine ? (feature_row(kOwn * wave + t, g, r) * s.dv + col) * 4 : kOutside, S[t][r]);
-                }
                 __builtin_amdgcn_sched_barrier(0);
                 fx4 S2[kOwn];
 #pragma unroll
@@ -205,15 +195,6 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                     S2[t] = mma<NI, NS>(k_high[t], high, fx4{0, 0, 0, 0});
                 }
                 read_block(more ? first + kBlock : first);
-                if constexpr (KEEP) {
-                    const uint32_t step = s.heads * s.dv * 4;
-                    const Buffer to = rows_of(update_p, first, step, s.dv * 4);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        put1<ElemF32>(to, mine ? (16 * wave + 4 * g + r) * step + col * 4 : kOutside, u[r]);
-                    state_p += (int64_t)s.heads * s.dk * s.dv * 4;
-                    update_p += (int64_t)step * kBlock;
-                }
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t)
 #pragma unroll
@@ -243,6 +224,11 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         float since[2];
         const char *q_p = reinterpret_cast<const char*>(q + copy0), *p_p = p_in + entry0 * kMatrixBytes<NS>;
         const char* out_p = start_of(out, v_step, v_head);
+        // KEEP: state and updates leave from their parts in LDS, to 2^-16 like all that is computed from them (fp32: exact)
+        const uint32_t u_step = s.heads * s.dv * 4;
+        [[maybe_unused]] char* state_p = reinterpret_cast<char*>(states + entry0 * s.dk * s.dv);
+        [[maybe_unused]] char* update_p = reinterpret_cast<char*>(updates + (seq_row * s.heads + head) * s.dv);
+        const int quad = col0 + 4 * g;
         const auto load_q = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Buffer b = buffer_of(q_p, kKeyBytes);
 #pragma unroll
@@ -276,6 +262,13 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                     o2 = mma<NS, NI>(so[d + 1], operand_from<NI, E>(q_raw[own][d + 1]), o2);
                 }
             }
+            if constexpr (KEEP) {
+                const Buffer to = buffer_of(state_p, first < seq_length ? (int64_t)s.dk * s.dv * 4 : 0);
+#pragma unroll
+                for (int t = kOwn * wave; t < kOwn * wave + kOwn; ++t)
+                    put4<ElemF32>(to, quad < s.dv ? (feature_row(t, c >> 2, c & 3) * s.dv + quad) * 4 : kOutside, exchanged_row(xs, t, lane));
+                state_p += (int64_t)s.heads * s.dk * s.dv * 4;
+            }
             lds_barrier();
             load_p(first + kBlock, own ^ 1);
             load_q(first + 2 * kBlock, own);
@@ -290,9 +283,13 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] += o2[r];
             }
-            const int d = col0 + 4 * g;
-            put4<E>(rows_of(out_p, first, v_step, s.dv * kSize), d < s.dv ? token * v_step + d * kSize : kOutside, o);
+            put4<E>(rows_of(out_p, first, v_step, s.dv * kSize), quad < s.dv ? token * v_step + quad * kSize : kOutside, o);
             out_p += v_move;
+            if constexpr (KEEP) {
+                put4<ElemF32>(rows_of(update_p, first, u_step, s.dv * 4), quad < s.dv ? token * u_step + quad * 4 : kOutside,
+                              exchanged_row(xu, wave, lane));
+                update_p += (int64_t)u_step * kBlock;
+            }
         };
         for (int64_t first = 0; first < seq_length; first += 2 * kBlock) {
             block(first, 0);

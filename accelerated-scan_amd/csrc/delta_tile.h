@@ -446,6 +446,29 @@ struct Exchange {
     }
 };
 
+// Row lane % 16 of an exchanged tile, columns 4 (lane / 16) .. + 3: what goes to memory as 16 bytes of a row.  (From
+// the accumulator itself a store would be four bytes to a lane: four times the instructions.)
+template <int P, int N>
+__device__ __forceinline__ fx4 exchanged_row(const Exchange<P, N>& x, int tile, int lane) {
+    const int i = lane & 15, c0 = 4 * (lane >> 4);
+    fx4 y;
+    if constexpr (P == 0) {
+        const char* at = x.base + (tile * 64 + (i >> 2) * 16 + c0) * 16 + (i & 3) * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = *reinterpret_cast<const float*>(at + r * 16);
+    } else {
+#pragma unroll
+        for (int n = P - 1; n >= 0; --n) {
+            char* at = x.base + ((n * N + (tile >> 1)) * 64 + (i & 3) * 16 + c0 + (i >> 2)) * 16 + (tile & 1) * 8;
+            const bx4 part = __builtin_bit_cast(
+                bx4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) sx4*)at));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = n == P - 1 ? (float)part[r] : y[r] + (float)part[r];
+        }
+    }
+    return y;
+}
+
 // Workgroup barrier for data in LDS: loads from memory stay in flight across it, which __syncthreads() does not
 // promise.
 __device__ __forceinline__ void lds_barrier() {
