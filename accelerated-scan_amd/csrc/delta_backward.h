@@ -33,7 +33,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
     const char* __restrict__ p_in, const float* __restrict__ d_final, typename E::S* __restrict__ d_v,
-    float* __restrict__ d_initial, float* __restrict__ d_states, float* __restrict__ d_rows) {
+    float* __restrict__ d_initial, float* __restrict__ d_states, float* __restrict__ d_rows, bool ahead) {
     using ES = typename E::S;
     constexpr int kDepths = DK / 32, kOwn = DK / 64, kCopies = DK / 32;
     extern __shared__ __align__(16) char smem[];
@@ -312,11 +312,30 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) qt.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, q_raw[set][i]);
         };
+        const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
+        int touched = 0;
+        const auto touch_block = [&](int64_t n_block) __attribute__((always_inline)) {
+            asm volatile("" ::"v"(touched));
+            if (ahead && n_block >= 0) {
+                const int64_t back = last - n_block, rows = seq_length - n_block * kBlock < kBlock ? seq_length - n_block * kBlock : kBlock;
+                const char* at_k = reinterpret_cast<const char*>(k + copy0) - back * k_move;
+                const char* at_q = reinterpret_cast<const char*>(q + copy0) - back * k_move;
+                const int64_t at_matrix = entry0 * kMatrixBytes<NS> - back * matrix_move;
+                const Lines lines{{at_k, at_q, t_in + at_matrix, p_in + at_matrix,
+                                   start_of(d_out, v_step, (int64_t)head * s.dv * kSize) - back * v_move},
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
+                                   d_out != nullptr ? (int)rows * ((row_bytes + 127) / 128) : 0},
+                                  (row_bytes + 127) / 128, (int64_t)v_step};
+                touched = touch(lines, tid * groups + col0 / 16);
+            }
+        };
         load_block(last, 0);
         load_block(last - 1, 1);
         stage_block(last, 0);
         stage_queries(0);
         load_block(last - 2, 0);
+        touch_block(last - 3);
+        touch_block(last - 4);
         lds_barrier();
         const auto block = [&](int64_t now, int other) __attribute__((always_inline)) {
             lds_barrier();
@@ -325,6 +344,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             lds_barrier();
             stage_queries(other);
             load_block(now - 3, other);
+            touch_block(now - 5);
         };
         for (int64_t now = last; now >= 0; now -= 2) {
             block(now, 1);

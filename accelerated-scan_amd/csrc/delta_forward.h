@@ -30,6 +30,34 @@ __device__ __forceinline__ ChainAt chain_at(const DeltaShape& s) {
 }
 inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads + 7) / 8 * 8 * ((s.dv + 15) / 16); }
 
+// Whether a chain kernel asks for its blocks ahead (touch below).  It gains where a compute unit runs one long chain
+// of large blocks: bf16 (1, 16384, 32 heads of 128 x 128) 379 -> 341 us; and loses where workgroups follow each other, whose
+// starts it delays (fp16, 16 packed sequences, 2048 workgroups: 226 -> 239 us), where blocks are small (key size 64:
+// 51 -> 57 us) and where fp32 products take longer than the loads (69 -> 72 us).
+template <int NS, int DK>
+inline bool chain_touches(const DeltaShape& s) { return NS > 0 && DK == 128 && chain_grid(s) <= 512; }
+
+// A chain's workgroup may have as many lines of 128 bytes on their way as its compute unit's cache holds, 256.  At the
+// latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 66 (and nobody else uses the
+// bandwidth); at that of the die's second cache it is three times as much.  So every line is asked for blocks ahead by
+// one of the workgroups that will read it: line `id` of up to five pieces of memory, one after the other.
+struct Lines {
+    const char* at[5];
+    int count[5];  // of 128 bytes
+    int row_lines;   // of the last piece: lines of a row, which are `step` bytes apart
+    int64_t step;
+};
+__device__ __forceinline__ int touch(const Lines& l, int id) {
+    const char* p = nullptr;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const char* here = i < 4 ? l.at[i] + id * 128 : l.at[4] + (int64_t)(id / l.row_lines) * l.step + id % l.row_lines * 128;
+        if (id >= 0 && id < l.count[i]) p = here;
+        id -= l.count[i];
+    }
+    return p != nullptr ? *reinterpret_cast<const int*>(p) : 0;
+}
+
 template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
                             3 * Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
@@ -42,7 +70,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                                                    const float* __restrict__ gates, const char* __restrict__ t_in,
                                                    const char* __restrict__ p_in, const float* __restrict__ initial,
                                                    typename E::S* __restrict__ out, float* __restrict__ final,
-                                                   float* __restrict__ states, float* __restrict__ updates) {
+                                                   float* __restrict__ states, float* __restrict__ updates, bool ahead) {
     using ES = typename E::S;
     constexpr int kDepths = DK / 32, kOwn = DK / 64, kCopies = DK / 32;  // operands of a row, state tiles of a wave, loads of a thread
     extern __shared__ __align__(16) char smem[];
@@ -330,10 +358,28 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
             gate_of(first)[tid] = gate_raw[set];
         };
+        const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
+        int touched = 0;
+        const auto touch_block = [&](int64_t first) __attribute__((always_inline)) {
+            asm volatile("" ::"v"(touched));  // (what the last call asked for has to have come by now: it keeps it in the program)
+            if (ahead && first < seq_length) {
+                const int64_t n_block = first / kBlock, rows = seq_length - first < kBlock ? seq_length - first : kBlock;
+                const char* at_k = reinterpret_cast<const char*>(k + copy0) + n_block * k_move;
+                const char* at_q = reinterpret_cast<const char*>(q + copy0) + n_block * k_move;
+                const int64_t at_matrix = entry0 * kMatrixBytes<NS> + n_block * matrix_move;
+                const Lines lines{{at_k, at_q, t_in + at_matrix, p_in + at_matrix, start_of(v, v_step, v_head) + n_block * v_move},
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
+                                   (int)rows * ((row_bytes + 127) / 128)},
+                                  (row_bytes + 127) / 128, (int64_t)v_step};
+                touched = touch(lines, tid * groups + col0 / 16);
+            }
+        };
         load_block(0, 0);
         load_block(kBlock, 1);
         stage_block(0, 0);
         load_block(2 * kBlock, 0);
+        touch_block(3 * kBlock);
+        touch_block(4 * kBlock);
         lds_barrier();
         const auto block = [&](int64_t first, int other) __attribute__((always_inline)) {
             lds_barrier();
@@ -341,6 +387,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             stage_block(first + kBlock, other);  // the tiles' last readers are behind the first barrier
             lds_barrier();
             load_block(first + 3 * kBlock, other);
+            touch_block(first + 5 * kBlock);
         };
         for (int64_t first = 0; first < seq_length; first += 2 * kBlock) {
             block(first, 1);
