@@ -20,15 +20,15 @@ namespace {
 
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
-template <int NI, int NS, int DK>
-constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                              2 * Exchange<NS, 2>::kBytes + (8 + DK / 16) * 1024 + kMatrixBytes<NS> + 4 * kBlock * 4;
+template <int NI, int NC, int DK>
+constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NC, DK / 32>::kBytes +
+                              2 * Exchange<NC, 2>::kBytes + (4 + DK / 16) * 1024 + kMatrixBytes<NC> + 4 * kBlock * 4;
 
 // The chain, last block first, divided like the forward one: 16 columns of D to a workgroup; state wave w keeps rows
 // dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.  Four waves
 // compute what does not wait for D (P^T dO and Q^T diag(scale e^c) dO) and write what leaves the chain, four load.
 // q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.
-template <class E, int NI, int NS, int DK>
+template <class E, int NI, int NC, int DK>
 __global__ __launch_bounds__(768) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
@@ -54,16 +54,16 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     m += Tile<NI, DK>::kBytes;
     char* const ot_at = m;
     m += 2 * Tile<NI, 16>::kBytes;
-    Exchange<NS, kDepths> xs(m);
-    m += Exchange<NS, kDepths>::kBytes;
-    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes);
-    m += 2 * Exchange<NS, 2>::kBytes;
+    Exchange<NC, kDepths> xs(m);
+    m += Exchange<NC, kDepths>::kBytes;
+    Exchange<NC, 2> xr(m), xu(m + Exchange<NC, 2>::kBytes);
+    m += 2 * Exchange<NC, 2>::kBytes;
     fx4* const po_at = reinterpret_cast<fx4*>(m) + lane;  // accumulator tiles from wave to wave, a KiB each
+    fx4* const dr_at = po_at;  // (P^T dO is read in front of the second barrier, dR written behind it)
     fx4* const qw_at = po_at + 4 * 64;
-    fx4* const dr_at = qw_at + 4 * kOwn * 64;
-    m += (8 + DK / 16) * 1024;
+    m += (4 + DK / 16) * 1024;
     char* const matrix_at = m;
-    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NS>);
+    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NC>);
 
     constexpr uint32_t kSize = sizeof(ES);
     constexpr int kKeyBytes = kBlock * DK * kSize;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         return static_cast<const char*>(p) + (seq_row + last * kBlock) * step + at_head;
     };
     const int64_t entry0 = (seq_block + last) * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NC>;
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
     const auto keys_at = [&](int64_t n_block) { return Tile<NI, DK>(smem + (n_block & 1) * Tile<NI, DK>::kBytes); };
@@ -114,23 +114,23 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 
             // dU = diag(e^(c[63]-c)) K D1 + P^T dO
             fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-            Operand<NS> tm[2];
+            Operand<NC> tm[2];
             fx4 beta_since;
             float whole;
             {
-                Operand<NS> so[kDepths];
+                Operand<NC> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
                 const fx4 po = po_at[wave * 64], until = gate_rows(kUntil);
-                tm[0] = matrix_operand<NS>(matrix_at, pair_upper(wave, wave >> 1), lane);
-                tm[1] = matrix_operand<NS>(matrix_at, pair_upper(wave, 1), lane);
+                tm[0] = matrix_operand<NC>(matrix_at, pair_upper(wave, wave >> 1), lane);
+                tm[1] = matrix_operand<NC>(matrix_at, pair_upper(wave, 1), lane);
                 beta_since = gate_rows(kBetaSince);
                 whole = gate[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
-                    u = mma<NI, NS>(ko[d], so[d], u);
-                    u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
+                    u = mma<NI, NC>(ko[d], so[d], u);
+                    u2 = mma<NI, NC>(ko[d + 1], so[d + 1], u2);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u[r] = until[r] * (u[r] + u2[r]) + po[r];
@@ -141,16 +141,16 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             // dR = dU + T^T dU; what the next products take of the keys is read on the way
             Operand<NI> k_low[kOwn], k_high[kOwn];
             {
-                const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
+                const Operand<NC> low = xr.get(0, lane), high = xr.get(1, lane);
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
                     k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma<NS, NS>(tm[1], high, u);
+                u = mma<NC, NC>(tm[1], high, u);
                 if (wave < 2) {
-                    u2 = mma<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
+                    u2 = mma<NC, NC>(tm[0], low, fx4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 }
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 
             // D0 = e^c[63] D1 + Q^T diag(scale e^c) dO - K^T diag(beta e^c) dR
             {
-                const Operand<NS> low = xu.get(0, lane), high = xu.get(1, lane);
+                const Operand<NC> low = xu.get(0, lane), high = xu.get(1, lane);
                 fx4 qw[kOwn], D2[kOwn];
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) qw[t] = qw_at[(kOwn * wave + t) * 64];
@@ -175,8 +175,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) D[t][r] *= whole;
-                    D[t] = mma<NI, NS>(k_low[t], low, D[t]);
-                    D2[t] = mma<NI, NS>(k_high[t], high, qw[t]);
+                    D[t] = mma<NI, NC>(k_low[t], low, D[t]);
+                    D2[t] = mma<NI, NC>(k_high[t], high, qw[t]);
                 }
                 read_block(now > 0 ? now - 1 : now);
 #pragma unroll
@@ -201,22 +201,22 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         }
     } else if (role == 1 && seq_length > 0) {
         // In front of the first block loads repeat it or give zero and stores are dropped: no condition stands around them.
-        Operand<NS> pm[2][2];
-        const char* p_p = p_in + entry0 * kMatrixBytes<NS>;
+        Operand<NC> pm[2][2];
+        const char* p_p = p_in + entry0 * kMatrixBytes<NC>;
         char* state_p = reinterpret_cast<char*>(d_states + entry0 * s.dk * s.dv);
         const int quad = col0 + 4 * g;
         char *v_p = const_cast<char*>(start_of(d_v, v_step, (int64_t)head * s.dv * kSize));
         char *r_p = const_cast<char*>(start_of(d_rows, r_step, (int64_t)head * s.dv * 4));
         const auto load_p = [&](int64_t n_block, int set) __attribute__((always_inline)) {
-            const Buffer b = buffer_of(p_p, kMatrixBytes<NS>);
-            pm[set][0] = matrix_operand<NS>(b, wave < 2 ? pair_upper(wave, 0) : (int)(kOutside >> 12), lane);
-            pm[set][1] = matrix_operand<NS>(b, pair_upper(wave, 1), lane);
+            const Buffer b = buffer_of(p_p, kMatrixBytes<NC>);
+            pm[set][0] = matrix_operand<NC>(b, wave < 2 ? pair_upper(wave, 0) : (int)(kOutside >> 12), lane);
+            pm[set][1] = matrix_operand<NC>(b, pair_upper(wave, 1), lane);
             if (n_block > 0) p_p -= matrix_move;
         };
         const auto outputs = [&](int64_t n_block, int set) __attribute__((always_inline)) {  // P^T dO
             const Tile<NI, 16> ot = outs_at(n_block);
-            fx4 po = mma<NS, NI>(pm[set][1], ot.down(32, 0, lane), fx4{0, 0, 0, 0});
-            if (wave < 2) po = mma<NS, NI>(pm[set][0], ot.down(0, 0, lane), po);
+            fx4 po = mma<NC, NI>(pm[set][1], ot.down(32, 0, lane), fx4{0, 0, 0, 0});
+            if (wave < 2) po = mma<NC, NI>(pm[set][0], ot.down(0, 0, lane), po);
             po_at[wave * 64] = po;
         };
         load_p(last, 0);
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 for (int r = 0; r < 4; ++r) w[t][r] *= s.scale * f[r];
             }
             const float beta = gate[kBeta * kBlock + token];
-            const Operand<NS> w_low = operand_of<NS>(w[0], w[1]), w_high = operand_of<NS>(w[2], w[3]);
+            const Operand<NC> w_low = operand_of<NC>(w[0], w[1]), w_high = operand_of<NC>(w[2], w[3]);
             {
                 const Buffer to = buffer_of(state_p, now >= 0 ? (int64_t)s.dk * s.dv * 4 : 0);
 #pragma unroll
@@ -248,16 +248,17 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < kOwn; ++t) {
-                fx4 qw = mma<NI, NS>(qt.down_features(0, kOwn * wave + t, lane), w_low, fx4{0, 0, 0, 0});
-                qw = mma<NI, NS>(qt.down_features(32, kOwn * wave + t, lane), w_high, qw);
+                fx4 qw = mma<NI, NC>(qt.down_features(0, kOwn * wave + t, lane), w_low, fx4{0, 0, 0, 0});
+                qw = mma<NI, NC>(qt.down_features(32, kOwn * wave + t, lane), w_high, qw);
                 qw_at[(kOwn * wave + t) * 64] = qw;
             }
             lds_barrier();
-            outputs(now - 1, other);
-            load_p(now - 3, other);
             // row `token` of dR, four columns, from the accumulators' order
             const float* from = reinterpret_cast<const float*>(dr_at - lane + wave * 64 + (c >> 2) * 16 + 4 * g) + (c & 3);
             const fx4 u = {from[0], from[4], from[8], from[12]};
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");  // the same place takes the next P^T dO
+            outputs(now - 1, other);
+            load_p(now - 3, other);
             put4<ElemF32>(rows_of(r_p, now, r_step, s.dv * 4), quad < s.dv ? token * r_step + quad * 4 : kOutside, u);
             put4<E>(rows_of(v_p, now, v_step, s.dv * kSize), quad < s.dv ? token * v_step + quad * kSize : kOutside,
                     fx4{beta * u[0], beta * u[1], beta * u[2], beta * u[3]});
@@ -271,15 +272,14 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     } else if (seq_length > 0) {
         // Keys, queries, dO, T and gates to LDS.
         Eight<E> k_raw[2][kCopies], q_raw[2][kCopies], o_raw[2];
-        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
-        fx4 t_raw[2][kPieces];
+        fx4 t_raw[2][kPieces<NC>];
         float gate_raw[2];
         const int64_t copy0 = ((seq_block + last) * s.key_heads + key_head) * kBlock * DK;
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *q_p = reinterpret_cast<const char*>(q + copy0);
         const char* o_p = start_of(d_out, v_step, (int64_t)head * s.dv * kSize);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const char* t_p = t_in + entry0 * kMatrixBytes<NC>;
         const auto load_block = [&](int64_t n_block, int set) __attribute__((always_inline)) {
-            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NS>);
+            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NC>);
             const Buffer ob = d_out != nullptr ? rows_of(o_p, n_block, v_step, s.dv * kSize) : buffer_of(k_p, 0);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             o_raw[set] = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces<NC>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(buffer_of(gate_p, kGateFloats * 4), tid * 4);
             o_p -= v_move;
             if (n_block > 0) {
@@ -305,7 +305,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             outs_at(n_block).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces<NC>; ++i)
+                if ((tid + 256 * i) * 16 < kMatrixBytes<NC>) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
             gate[tid] = gate_raw[set];
         };
         const auto stage_queries = [&](int set) __attribute__((always_inline)) {
@@ -320,10 +321,10 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 const int64_t back = last - n_block, rows = seq_length - n_block * kBlock < kBlock ? seq_length - n_block * kBlock : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) - back * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) - back * k_move;
-                const int64_t at_matrix = entry0 * kMatrixBytes<NS> - back * matrix_move;
+                const int64_t at_matrix = entry0 * kMatrixBytes<NC> - back * matrix_move;
                 const Lines lines{{at_k, at_q, t_in + at_matrix, p_in + at_matrix,
                                    start_of(d_out, v_step, (int64_t)head * s.dv * kSize) - back * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NC> / 128, kMatrixBytes<NC> / 128,
                                    d_out != nullptr ? (int)rows * ((row_bytes + 127) / 128) : 0},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);

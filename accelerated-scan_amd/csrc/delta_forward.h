@@ -34,8 +34,8 @@ inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads +
 // of large blocks: bf16 (1, 16384, 32 heads of 128 x 128) 379 -> 341 us; and loses where workgroups follow each other, whose
 // starts it delays (fp16, 16 packed sequences, 2048 workgroups: 226 -> 239 us), where blocks are small (key size 64:
 // 51 -> 57 us) and where fp32 products take longer than the loads (69 -> 72 us).
-template <int NS, int DK>
-inline bool chain_touches(const DeltaShape& s) { return NS > 0 && DK == 128 && chain_grid(s) <= 512; }
+template <int NC, int DK>
+inline bool chain_touches(const DeltaShape& s) { return NC > 0 && DK == 128 && chain_grid(s) <= 512; }
 
 // A chain's workgroup may have as many lines of 128 bytes on their way as its compute unit's cache holds, 256.  At the
 // latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 66 (and nobody else uses the
@@ -58,12 +58,17 @@ __device__ __forceinline__ int touch(const Lines& l, int id) {
     return p != nullptr ? *reinterpret_cast<const int*>(p) : 0;
 }
 
-template <int NI, int NS, int DK>
-constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                            3 * Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
+template <int NI, int NS, int NC, int DK>
+constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NC, DK / 32>::kBytes +
+                            2 * Exchange<NC, 2>::kBytes + Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NC> + 2 * 4 * kBlock * 4;
 
-// q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.  KEEP: write the states in front of the blocks and the rows U.
-template <class E, int NI, int NS, int DK, bool KEEP>
+// Pieces of 16 bytes of T that each of 256 threads carries to LDS.
+template <int NC>
+constexpr int kPieces = (kMatrixBytes<NC> / 16 + 255) / 256;
+
+// q and k: the copies that delta_prepare made.  NC: parts of what the chain hands on, NS: of what only
+// the outputs see.  grid chain_grid(), 768 threads.  KEEP: write the states in front of the blocks and the rows U.
+template <class E, int NI, int NS, int NC, int DK, bool KEEP>
 __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
                                                    const typename E::S* __restrict__ v,
@@ -89,12 +94,14 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     m += 2 * Tile<NI, DK>::kBytes;
     char* const vt_at = m;
     m += 2 * Tile<NI, 16>::kBytes;
-    Exchange<NS, kDepths> xs(m);
-    m += Exchange<NS, kDepths>::kBytes;
-    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes), xd(m + 2 * Exchange<NS, 2>::kBytes);
-    m += 3 * Exchange<NS, 2>::kBytes;
+    Exchange<NC, kDepths> xs(m);
+    m += Exchange<NC, kDepths>::kBytes;
+    Exchange<NC, 2> xr(m), xd(m + Exchange<NC, 2>::kBytes);
+    m += 2 * Exchange<NC, 2>::kBytes;
+    Exchange<NS, 2> xu(m);
+    m += Exchange<NS, 2>::kBytes;
     char* const matrix_at = m;
-    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NS>);
+    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NC>);
 
     constexpr uint32_t kSize = sizeof(ES);
     const uint32_t v_step = s.heads * s.dv * kSize;
@@ -107,7 +114,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     };
     const auto start_of = [&](const void* p, uint32_t step, int64_t at_head) { return static_cast<const char*>(p) + seq_row * step + at_head; };
     const int64_t entry0 = seq_block * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, t_move = (int64_t)s.heads * kMatrixBytes<NC>, p_move = (int64_t)s.heads * kMatrixBytes<NS>;
     constexpr int kKeyBytes = kBlock * DK * kSize;  // of a block, in the copies
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         o[1] = matrix_operand<NS>(b, wave >= 2 ? pair_lower(wave, 1) : (int)(kOutside >> 12), lane);
     };
     const auto keys_at = [&](int64_t first) { return Tile<NI, DK>(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes); };
-    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NS>; };
+    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NC>; };
     const auto gate_of = [&](int64_t first) { return gate_at + ((first / kBlock) & 1) * 4 * kBlock; };
     const auto values_at = [&](int64_t first) { return Tile<NI, 16>(vt_at + ((first / kBlock) & 1) * Tile<NI, 16>::kBytes); };
 
@@ -160,22 +167,22 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 
             // K S0 (rows: tokens, columns: state columns)
             fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-            Operand<NS> tm[2];
+            Operand<NC> tm[2];
             fx4 until;
             float whole;
             {
-                Operand<NS> so[kDepths];
+                Operand<NC> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
-                tm[0] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane);
-                tm[1] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
+                tm[0] = matrix_operand<NC>(matrix_of(first), pair_lower(wave, 0), lane);
+                tm[1] = matrix_operand<NC>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
                 until = gate_rows(first, kUntil);
                 whole = gate_of(first)[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
-                    u = mma<NI, NS>(ko[d], so[d], u);
-                    u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
+                    u = mma<NI, NC>(ko[d], so[d], u);
+                    u2 = mma<NI, NC>(ko[d + 1], so[d + 1], u2);
                 }
             }
             // R = diag(beta) V - diag(beta e^c) K S0
@@ -187,16 +194,16 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             // U = R + T R; what the next products take of the keys is read on the way
             Operand<NI> k_low[kOwn], k_high[kOwn];
             {
-                const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
+                const Operand<NC> low = xr.get(0, lane), high = xr.get(1, lane);
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
                     k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma<NS, NS>(tm[0], low, u);
+                u = mma<NC, NC>(tm[0], low, u);
                 if (wave >= 2) {
-                    u2 = mma<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
+                    u2 = mma<NC, NC>(tm[1], high, fx4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 }
@@ -212,15 +219,15 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 
             // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
             {
-                const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
+                const Operand<NC> low = xd.get(0, lane), high = xd.get(1, lane);
                 __builtin_amdgcn_sched_barrier(0);
                 fx4 S2[kOwn];
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) S[t][r] *= whole;
-                    S[t] = mma<NI, NS>(k_low[t], low, S[t]);
-                    S2[t] = mma<NI, NS>(k_high[t], high, fx4{0, 0, 0, 0});
+                    S[t] = mma<NI, NC>(k_low[t], low, S[t]);
+                    S2[t] = mma<NI, NC>(k_high[t], high, fx4{0, 0, 0, 0});
                 }
                 read_block(more ? first + kBlock : first);
 #pragma unroll
@@ -267,7 +274,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             load_matrix(p_p, pm[set]);
             since[set] = fetch4(gates_here(), kSince * 256 + token * 4);
             if (first + kBlock < seq_length) {
-                p_p += matrix_move;
+                p_p += p_move;
                 gate_p += gate_move;
             }
         };
@@ -282,7 +289,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             {
                 Operand<NS> so[kDepths];
 #pragma unroll
-                for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
+                for (int d = 0; d < kDepths; ++d) so[d] = leading<NS>(xs.get(d, lane));
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
@@ -326,26 +333,24 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     } else if (seq_length > 0) {
         // Keys, values, T and gates to LDS, three blocks ahead.
         Eight<E> k_raw[2][kCopies], v_raw[2];
-        constexpr int kPieces = kMatrixBytes<NS> / 16 / 256;
-        static_assert(kMatrixBytes<NS> % (16 * 256) == 0, "pieces of a matrix to a thread");
-        fx4 t_raw[2][kPieces];
+        fx4 t_raw[2][kPieces<NC>];
         float gate_raw[2];
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const char* t_p = t_in + entry0 * kMatrixBytes<NC>;
         const auto load_block = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
-            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
+            const Buffer tb = buffer_of(t_p, kMatrixBytes<NC>);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces<NC>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(gates_here(), tid * 4);
             v_p += v_move;
             if (first + kBlock < seq_length) {
                 k_p += k_move;
-                t_p += matrix_move;
+                t_p += t_move;
                 gate_p += gate_move;
             }
         };
@@ -355,7 +360,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces<NC>; ++i)
+                if ((tid + 256 * i) * 16 < kMatrixBytes<NC>) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
             gate_of(first)[tid] = gate_raw[set];
         };
         const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
@@ -366,9 +372,9 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 const int64_t n_block = first / kBlock, rows = seq_length - first < kBlock ? seq_length - first : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) + n_block * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) + n_block * k_move;
-                const int64_t at_matrix = entry0 * kMatrixBytes<NS> + n_block * matrix_move;
-                const Lines lines{{at_k, at_q, t_in + at_matrix, p_in + at_matrix, start_of(v, v_step, v_head) + n_block * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
+                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NC> + n_block * t_move,
+                                   p_in + entry0 * kMatrixBytes<NS> + n_block * p_move, start_of(v, v_step, v_head) + n_block * v_move},
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NC> / 128, kMatrixBytes<NS> / 128,
                                    (int)rows * ((row_bytes + 127) / 128)},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);

@@ -91,6 +91,20 @@ __device__ __forceinline__ Operand<P> operand_of(const fx4& a, const fx4& b) {
     return o;
 }
 
+// The first N parts of an operand.
+template <int N, int P>
+__device__ __forceinline__ Operand<N> leading(const Operand<P>& o) {
+    static_assert(N <= P && (N > 0 || P == 0), "parts that are there");
+    Operand<N> r;
+    if constexpr (P == 0) {
+        r = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.p[i] = o.p[i];
+    }
+    return r;
+}
+
 // c + a * b over 32 depths.  Pairs of parts below the last bit kept of the product are left out:
 // part i of a has weight 2^-8i.
 template <int PA, int PB>
@@ -280,7 +294,7 @@ __device__ __forceinline__ constexpr int feature_row(int t, int g, int r) { retu
 // ---------------------------------------------------------------------------
 template <int P, int W>
 struct Tile {
-    static constexpr int kStride = W < 64 ? W + 8 : W;
+    static constexpr int kStride = W;  // (rows of 16 values: four of them are the 128 bytes of a transposing read)
     static constexpr int kPlane = kBlock * kStride;
     static constexpr int kBytes = P * kPlane * 2;
     __bf16* base;
