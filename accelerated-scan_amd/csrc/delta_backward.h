@@ -20,15 +20,16 @@ namespace {
 
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
-template <int NI, int NC, int DK>
-constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NC, DK / 32>::kBytes +
-                              2 * Exchange<NC, 2>::kBytes + (4 + DK / 16) * 1024 + kMatrixBytes<NC> + 4 * kBlock * 4;
+template <int NI, int NS, int NC, int DK>
+constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
+                              Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + (4 + DK / 16) * 1024 + kMatrixBytes<NS> + 4 * kBlock * 4;
 
 // The chain, last block first, divided like the forward one: 16 columns of D to a workgroup; state wave w keeps rows
 // dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.  Four waves
 // compute what does not wait for D (P^T dO and Q^T diag(scale e^c) dO) and write what leaves the chain, four load.
+// What enters D for good (P^T dO, W and the rows from dR) is in NC parts, the rest in NS, as in the forward chain.
 // q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.
-template <class E, int NI, int NC, int DK>
+template <class E, int NI, int NS, int NC, int DK>
 __global__ __launch_bounds__(768) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
@@ -54,16 +55,18 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     m += Tile<NI, DK>::kBytes;
     char* const ot_at = m;
     m += 2 * Tile<NI, 16>::kBytes;
-    Exchange<NC, kDepths> xs(m);
-    m += Exchange<NC, kDepths>::kBytes;
-    Exchange<NC, 2> xr(m), xu(m + Exchange<NC, 2>::kBytes);
-    m += 2 * Exchange<NC, 2>::kBytes;
+    Exchange<NS, kDepths> xs(m);
+    m += Exchange<NS, kDepths>::kBytes;
+    Exchange<NS, 2> xr(m);
+    m += Exchange<NS, 2>::kBytes;
+    Exchange<NC, 2> xu(m);
+    m += Exchange<NC, 2>::kBytes;
     fx4* const po_at = reinterpret_cast<fx4*>(m) + lane;  // accumulator tiles from wave to wave, a KiB each
     fx4* const dr_at = po_at;  // (P^T dO is read in front of the second barrier, dR written behind it)
     fx4* const qw_at = po_at + 4 * 64;
     m += (4 + DK / 16) * 1024;
     char* const matrix_at = m;
-    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NC>);
+    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NS>);
 
     constexpr uint32_t kSize = sizeof(ES);
     constexpr int kKeyBytes = kBlock * DK * kSize;
@@ -79,7 +82,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         return static_cast<const char*>(p) + (seq_row + last * kBlock) * step + at_head;
     };
     const int64_t entry0 = (seq_block + last) * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NC>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, t_move = (int64_t)s.heads * kMatrixBytes<NS>, p_move = (int64_t)s.heads * kMatrixBytes<NC>;
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
     const auto keys_at = [&](int64_t n_block) { return Tile<NI, DK>(smem + (n_block & 1) * Tile<NI, DK>::kBytes); };
@@ -114,23 +117,23 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 
             // dU = diag(e^(c[63]-c)) K D1 + P^T dO
             fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-            Operand<NC> tm[2];
+            Operand<NS> tm[2];
             fx4 beta_since;
             float whole;
             {
-                Operand<NC> so[kDepths];
+                Operand<NS> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
                 const fx4 po = po_at[wave * 64], until = gate_rows(kUntil);
-                tm[0] = matrix_operand<NC>(matrix_at, pair_upper(wave, wave >> 1), lane);
-                tm[1] = matrix_operand<NC>(matrix_at, pair_upper(wave, 1), lane);
+                tm[0] = matrix_operand<NS>(matrix_at, pair_upper(wave, wave >> 1), lane);
+                tm[1] = matrix_operand<NS>(matrix_at, pair_upper(wave, 1), lane);
                 beta_since = gate_rows(kBetaSince);
                 whole = gate[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
-                    u = mma<NI, NC>(ko[d], so[d], u);
-                    u2 = mma<NI, NC>(ko[d + 1], so[d + 1], u2);
+                    u = mma<NI, NS>(ko[d], so[d], u);
+                    u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u[r] = until[r] * (u[r] + u2[r]) + po[r];
@@ -141,16 +144,16 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             // dR = dU + T^T dU; what the next products take of the keys is read on the way
             Operand<NI> k_low[kOwn], k_high[kOwn];
             {
-                const Operand<NC> low = xr.get(0, lane), high = xr.get(1, lane);
+                const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
                     k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma<NC, NC>(tm[1], high, u);
+                u = mma_all<NS, NS>(tm[1], high, u);
                 if (wave < 2) {
-                    u2 = mma<NC, NC>(tm[0], low, fx4{0, 0, 0, 0});
+                    u2 = mma_all<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 }
@@ -211,7 +214,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             const Buffer b = buffer_of(p_p, kMatrixBytes<NC>);
             pm[set][0] = matrix_operand<NC>(b, wave < 2 ? pair_upper(wave, 0) : (int)(kOutside >> 12), lane);
             pm[set][1] = matrix_operand<NC>(b, pair_upper(wave, 1), lane);
-            if (n_block > 0) p_p -= matrix_move;
+            if (n_block > 0) p_p -= p_move;
         };
         const auto outputs = [&](int64_t n_block, int set) __attribute__((always_inline)) {  // P^T dO
             const Tile<NI, 16> ot = outs_at(n_block);
@@ -272,14 +275,14 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     } else if (seq_length > 0) {
         // Keys, queries, dO, T and gates to LDS.
         Eight<E> k_raw[2][kCopies], q_raw[2][kCopies], o_raw[2];
-        fx4 t_raw[2][kPieces<NC>];
+        fx4 t_raw[2][kPieces<NS>];
         float gate_raw[2];
         const int64_t copy0 = ((seq_block + last) * s.key_heads + key_head) * kBlock * DK;
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *q_p = reinterpret_cast<const char*>(q + copy0);
         const char* o_p = start_of(d_out, v_step, (int64_t)head * s.dv * kSize);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NC>;
+        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
         const auto load_block = [&](int64_t n_block, int set) __attribute__((always_inline)) {
-            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NC>);
+            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NS>);
             const Buffer ob = d_out != nullptr ? rows_of(o_p, n_block, v_step, s.dv * kSize) : buffer_of(k_p, 0);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
@@ -289,13 +292,13 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             o_raw[set] = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
 #pragma unroll
-            for (int i = 0; i < kPieces<NC>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces<NS>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(buffer_of(gate_p, kGateFloats * 4), tid * 4);
             o_p -= v_move;
             if (n_block > 0) {
                 k_p -= k_move;
                 q_p -= k_move;
-                t_p -= matrix_move;
+                t_p -= t_move;
                 gate_p -= gate_move;
             }
         };
@@ -305,8 +308,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             outs_at(n_block).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces<NC>; ++i)
-                if ((tid + 256 * i) * 16 < kMatrixBytes<NC>) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces<NS>; ++i)
+                if ((tid + 256 * i) * 16 < kMatrixBytes<NS>) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
             gate[tid] = gate_raw[set];
         };
         const auto stage_queries = [&](int set) __attribute__((always_inline)) {
@@ -321,10 +324,9 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 const int64_t back = last - n_block, rows = seq_length - n_block * kBlock < kBlock ? seq_length - n_block * kBlock : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) - back * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) - back * k_move;
-                const int64_t at_matrix = entry0 * kMatrixBytes<NC> - back * matrix_move;
-                const Lines lines{{at_k, at_q, t_in + at_matrix, p_in + at_matrix,
+                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NS> - back * t_move, p_in + entry0 * kMatrixBytes<NC> - back * p_move,
                                    start_of(d_out, v_step, (int64_t)head * s.dv * kSize) - back * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NC> / 128, kMatrixBytes<NC> / 128,
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NC> / 128,
                                    d_out != nullptr ? (int)rows * ((row_bytes + 127) / 128) : 0},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);

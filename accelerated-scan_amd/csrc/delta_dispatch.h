@@ -28,7 +28,7 @@ struct DeltaParts {
         const size_t copy = (size_t)s.blocks * s.key_heads * kBlock * (s.dk <= 64 ? 64 : 128) * element;
         gates = 0;
         t = round_up(gates + entries * kGateFloats * 4);
-        p = round_up(t + entries * kMatrixBytes<NC>);
+        p = round_up(t + entries * kMatrixBytes<NS>);
         k = round_up(p + entries * (backward ? kMatrixBytes<NC> : kMatrixBytes<NS>));
         q = round_up(k + copy);
         d_states = round_up(q + copy);
@@ -48,7 +48,7 @@ template <class E, int NI, int NS, int NC, int DK>
 hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void* log_gates, const void* beta,
                    char* ws, const DeltaParts<NS, NC>& at, bool upper, hipStream_t stream) {
     using S = typename E::S;
-    const auto kernel = upper ? delta_prepare<E, NI, NC, NC, DK, true> : delta_prepare<E, NI, NS, NC, DK, false>;
+    const auto kernel = upper ? delta_prepare<E, NI, NC, NS, DK, true> : delta_prepare<E, NI, NS, NS, DK, false>;
     return delta_launch(kernel, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
                         kPrepareBytes<NI, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
                         log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p,
@@ -77,7 +77,7 @@ int delta_forward_dk(const DeltaForward& f) {
 
 template <class E, int NI, int NS, int NC, int DK>
 int delta_backward_dk(const DeltaBackward& f) {
-    static_assert(kReverseBytes<NI, NC, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + 8 * 1024 <= kLdsBytes, "fits a compute unit");
+    static_assert(kReverseBytes<NI, NS, NC, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + 8 * 1024 <= kLdsBytes, "fits a compute unit");
     using S = typename E::S;
     const DeltaShape& s = f.shape;
     const DeltaParts<NS, NC> at(s, true, sizeof(S));
@@ -88,7 +88,7 @@ int delta_backward_dk(const DeltaBackward& f) {
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NC, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NC, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, NC, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NS, NC, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
                      f.d_initial, d_states, d_rows, chain_touches<NC, DK>(s));
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);

@@ -59,15 +59,19 @@ __device__ __forceinline__ int touch(const Lines& l, int id) {
 }
 
 template <int NI, int NS, int NC, int DK>
-constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NC, DK / 32>::kBytes +
-                            2 * Exchange<NC, 2>::kBytes + Exchange<NS, 2>::kBytes + 2 * kMatrixBytes<NC> + 2 * 4 * kBlock * 4;
+constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
+                            2 * Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
 
 // Pieces of 16 bytes of T that each of 256 threads carries to LDS.
 template <int NC>
 constexpr int kPieces = (kMatrixBytes<NC> / 16 + 255) / 256;
 
-// q and k: the copies that delta_prepare made.  NC: parts of what the chain hands on, NS: of what only
-// the outputs see.  grid chain_grid(), 768 threads.  KEEP: write the states in front of the blocks and the rows U.
+// q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.  KEEP: write the states in front
+// of the blocks and the rows U.
+// U goes into the state in NC parts, all else is in NS: the rounding of U stays in a state for good, where the
+// delta rule corrects in the next block what it read and solved inexactly.  With NS = 2 and bf16 a state after 16384 tokens is
+// off by 2.8e-6 of its norm with NC = 2 (341 us), by 7.0e-7 with NC = 3 and all pairs of parts in T R (348 us),
+// by 1.4e-7 with three parts throughout, where the longer exchanges and matrices cost 478 us.
 template <class E, int NI, int NS, int NC, int DK, bool KEEP>
 __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
@@ -94,14 +98,14 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     m += 2 * Tile<NI, DK>::kBytes;
     char* const vt_at = m;
     m += 2 * Tile<NI, 16>::kBytes;
-    Exchange<NC, kDepths> xs(m);
-    m += Exchange<NC, kDepths>::kBytes;
-    Exchange<NC, 2> xr(m), xd(m + Exchange<NC, 2>::kBytes);
-    m += 2 * Exchange<NC, 2>::kBytes;
-    Exchange<NS, 2> xu(m);
-    m += Exchange<NS, 2>::kBytes;
+    Exchange<NS, kDepths> xs(m);
+    m += Exchange<NS, kDepths>::kBytes;
+    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes);
+    m += 2 * Exchange<NS, 2>::kBytes;
+    Exchange<NC, 2> xd(m);
+    m += Exchange<NC, 2>::kBytes;
     char* const matrix_at = m;
-    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NC>);
+    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NS>);
 
     constexpr uint32_t kSize = sizeof(ES);
     const uint32_t v_step = s.heads * s.dv * kSize;
@@ -114,7 +118,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     };
     const auto start_of = [&](const void* p, uint32_t step, int64_t at_head) { return static_cast<const char*>(p) + seq_row * step + at_head; };
     const int64_t entry0 = seq_block * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, t_move = (int64_t)s.heads * kMatrixBytes<NC>, p_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
     constexpr int kKeyBytes = kBlock * DK * kSize;  // of a block, in the copies
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
@@ -126,7 +130,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         o[1] = matrix_operand<NS>(b, wave >= 2 ? pair_lower(wave, 1) : (int)(kOutside >> 12), lane);
     };
     const auto keys_at = [&](int64_t first) { return Tile<NI, DK>(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes); };
-    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NC>; };
+    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NS>; };
     const auto gate_of = [&](int64_t first) { return gate_at + ((first / kBlock) & 1) * 4 * kBlock; };
     const auto values_at = [&](int64_t first) { return Tile<NI, 16>(vt_at + ((first / kBlock) & 1) * Tile<NI, 16>::kBytes); };
 
@@ -167,22 +171,22 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 
             // K S0 (rows: tokens, columns: state columns)
             fx4 u = {0, 0, 0, 0}, u2 = {0, 0, 0, 0};  // (two sums: half as many products that wait for each other)
-            Operand<NC> tm[2];
+            Operand<NS> tm[2];
             fx4 until;
             float whole;
             {
-                Operand<NC> so[kDepths];
+                Operand<NS> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
-                tm[0] = matrix_operand<NC>(matrix_of(first), pair_lower(wave, 0), lane);
-                tm[1] = matrix_operand<NC>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
+                tm[0] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane);
+                tm[1] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
                 until = gate_rows(first, kUntil);
                 whole = gate_of(first)[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
-                    u = mma<NI, NC>(ko[d], so[d], u);
-                    u2 = mma<NI, NC>(ko[d + 1], so[d + 1], u2);
+                    u = mma<NI, NS>(ko[d], so[d], u);
+                    u2 = mma<NI, NS>(ko[d + 1], so[d + 1], u2);
                 }
             }
             // R = diag(beta) V - diag(beta e^c) K S0
@@ -194,16 +198,16 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             // U = R + T R; what the next products take of the keys is read on the way
             Operand<NI> k_low[kOwn], k_high[kOwn];
             {
-                const Operand<NC> low = xr.get(0, lane), high = xr.get(1, lane);
+                const Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
                     k_low[t] = kb.down_features(0, kOwn * wave + t, lane);
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma<NC, NC>(tm[0], low, u);
+                u = mma_all<NS, NS>(tm[0], low, u);
                 if (wave >= 2) {
-                    u2 = mma<NC, NC>(tm[1], high, fx4{0, 0, 0, 0});
+                    u2 = mma_all<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 }
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             load_matrix(p_p, pm[set]);
             since[set] = fetch4(gates_here(), kSince * 256 + token * 4);
             if (first + kBlock < seq_length) {
-                p_p += p_move;
+                p_p += matrix_move;
                 gate_p += gate_move;
             }
         };
@@ -289,7 +293,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             {
                 Operand<NS> so[kDepths];
 #pragma unroll
-                for (int d = 0; d < kDepths; ++d) so[d] = leading<NS>(xs.get(d, lane));
+                for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
@@ -333,24 +337,24 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     } else if (seq_length > 0) {
         // Keys, values, T and gates to LDS, three blocks ahead.
         Eight<E> k_raw[2][kCopies], v_raw[2];
-        fx4 t_raw[2][kPieces<NC>];
+        fx4 t_raw[2][kPieces<NS>];
         float gate_raw[2];
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NC>;
+        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
         const auto load_block = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
-            const Buffer tb = buffer_of(t_p, kMatrixBytes<NC>);
+            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
 #pragma unroll
-            for (int i = 0; i < kPieces<NC>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces<NS>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(gates_here(), tid * 4);
             v_p += v_move;
             if (first + kBlock < seq_length) {
                 k_p += k_move;
-                t_p += t_move;
+                t_p += matrix_move;
                 gate_p += gate_move;
             }
         };
@@ -360,8 +364,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces<NC>; ++i)
-                if ((tid + 256 * i) * 16 < kMatrixBytes<NC>) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces<NS>; ++i)
+                if ((tid + 256 * i) * 16 < kMatrixBytes<NS>) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
             gate_of(first)[tid] = gate_raw[set];
         };
         const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
@@ -372,9 +376,9 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 const int64_t n_block = first / kBlock, rows = seq_length - first < kBlock ? seq_length - first : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) + n_block * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) + n_block * k_move;
-                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NC> + n_block * t_move,
-                                   p_in + entry0 * kMatrixBytes<NS> + n_block * p_move, start_of(v, v_step, v_head) + n_block * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NC> / 128, kMatrixBytes<NS> / 128,
+                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NS> + n_block * matrix_move,
+                                   p_in + entry0 * kMatrixBytes<NS> + n_block * matrix_move, start_of(v, v_step, v_head) + n_block * v_move},
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
                                    (int)rows * ((row_bytes + 127) / 128)},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);

@@ -114,7 +114,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
     return (((row >> 4) * (DK / 32) + (d >> 5)) * 64 + ((d >> 3) & 3) * 16 + (row & 15)) * 8;
 }
 
-// grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.  T is written in NC
+// grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.  T is written in NT
 // parts, P in NP.
 //
 // P leaves from the accumulators: the tile K_j Q_i^T has token i in a lane's column and its rows j along the depth, as
@@ -125,7 +125,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
 // The block's keys and queries are copied to where they stand without gaps, missing rows and features as zeros: in the
 // tensors the rows of a head are a power of two apart as a rule, so that one channel of the cache holds them all, and the
 // chain's workgroups, which all want the same rows at the same time, waited for it (1.9 us a block, 1.2 us with copies).
-template <class E, int NI, int NP, int NC, int DK, bool upper>
+template <class E, int NI, int NP, int NT, int DK, bool upper>
 __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
                                                      const typename E::S* __restrict__ k,
                                                      const void* __restrict__ log_gates, const void* __restrict__ beta,
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
     }
     __syncthreads();
 
-    char* to = t_out + (block * s.heads + head) * kMatrixBytes<NC>;
+    char* to = t_out + (block * s.heads + head) * kMatrixBytes<NT>;
     for (int i = tid; i < kPairs * 64; i += 256) {
         const int pair = i >> 6;
         const int m = upper ? (pair < 4 ? pair >> 1 : pair - 2) : (pair < 2 ? pair : (pair + 2) >> 1);
@@ -345,13 +345,13 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
             a[r] -= row == col + r ? 1.0f : 0.0f;
             b[r] -= row == col + 16 + r ? 1.0f : 0.0f;
         }
-        const Operand<NC> o = operand_of<NC>(a, b);
-        if constexpr (NC == 0) {
+        const Operand<NT> o = operand_of<NT>(a, b);
+        if constexpr (NT == 0) {
             reinterpret_cast<fx4*>(to + i * 32)[0] = o.t[0];
             reinterpret_cast<fx4*>(to + i * 32)[1] = o.t[1];
         } else {
 #pragma unroll
-            for (int n = 0; n < NC; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
+            for (int n = 0; n < NT; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
         }
     }
 }

@@ -91,20 +91,6 @@ __device__ __forceinline__ Operand<P> operand_of(const fx4& a, const fx4& b) {
     return o;
 }
 
-// The first N parts of an operand.
-template <int N, int P>
-__device__ __forceinline__ Operand<N> leading(const Operand<P>& o) {
-    static_assert(N <= P && (N > 0 || P == 0), "parts that are there");
-    Operand<N> r;
-    if constexpr (P == 0) {
-        r = o;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.p[i] = o.p[i];
-    }
-    return r;
-}
-
 // c + a * b over 32 depths.  Pairs of parts below the last bit kept of the product are left out:
 // part i of a has weight 2^-8i.
 template <int PA, int PB>
@@ -125,6 +111,22 @@ __device__ __forceinline__ fx4 mma(const Operand<PA>& a, const Operand<PB>& b, f
                     c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], c, 0, 0, 0);
     }
     return c;
+}
+
+// The same over all pairs of parts, for a product in which the last ones are as large as the parts' own rounding.
+template <int PA, int PB>
+__device__ __forceinline__ fx4 mma_all(const Operand<PA>& a, const Operand<PB>& b, fx4 c) {
+    if constexpr (PA == 0) {
+        return mma<PA, PB>(a, b, c);
+    } else {
+#pragma unroll
+        for (int s = PA + PB - 2; s >= 0; --s)
+#pragma unroll
+            for (int i = 0; i < PA; ++i)
+                if (s - i >= 0 && s - i < PB)
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], c, 0, 0, 0);
+        return c;
+    }
 }
 
 // ---------------------------------------------------------------------------
