@@ -339,14 +339,19 @@ def _delta_gradients(queries, keys, values, log_gates, beta, states, started, of
     return (*(torch.empty_like(t) for t in (queries, keys, values, log_gates, beta)), d_initial)
 
 
+def _on_16_bytes(t):
+    """A gradient can be a piece of a larger tensor, from where the kernels do not read."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final, started):
     grads = _delta_gradients(queries, keys, values, log_gates, beta, states, started, offsets)
     if offsets is not None and offsets.shape[0] == 1:
         for g in grads:
             g.zero_()
     else:
-        _abi.delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final,
-                            *grads[:5], grads[5] if started else None)
+        _abi.delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale,
+                            _on_16_bytes(d_out), _on_16_bytes(d_final), *grads[:5], grads[5] if started else None)
     return grads
 
 

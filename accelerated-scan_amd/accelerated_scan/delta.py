@@ -18,6 +18,7 @@ diagonal (accelerated_scan/warp.cuh:49-223).
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _abi, _ops
 
@@ -108,13 +109,19 @@ class GatedDeltaScan(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out, d_final):
-        if d_out is None and d_final is None:
-            return (None,) * 8
-        *inputs, states, updates, offsets = ctx.saved_tensors
-        grads = _ops.delta_backward_run(*inputs, states, updates, offsets, ctx.scale,
-                                        d_out.contiguous() if d_out is not None else None,
-                                        d_final.contiguous() if d_final is not None else None, ctx.started)
-        return (*grads[:5], grads[5] if ctx.started else None, None, None)
+        if torch.is_grad_enabled() and not _ops.capturing():  # create_graph: no second derivatives
+            return once_differentiable(_scan_gradients)(ctx, d_out, d_final)
+        return _scan_gradients(ctx, d_out, d_final)
+
+
+def _scan_gradients(ctx, d_out, d_final):
+    if d_out is None and d_final is None:
+        return (None,) * 8
+    *inputs, states, updates, offsets = ctx.saved_tensors
+    grads = _ops.delta_backward_run(*inputs, states, updates, offsets, ctx.scale,
+                                    d_out.contiguous() if d_out is not None else None,
+                                    d_final.contiguous() if d_final is not None else None, ctx.started)
+    return (*grads[:5], grads[5] if ctx.started else None, None, None)
 
 
 def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale=None, offsets=None):
@@ -126,7 +133,7 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
         values (torch.Tensor): shape (B, T, heads, value_dim), contiguous, same dtype; ``heads`` a multiple of
             ``key_heads``.
         log_gates, beta (torch.Tensor): shape (B, T, heads), contiguous, the same dtype or fp32.  A log gate of
-            ``-inf`` starts the state anew.
+            ``-inf`` starts the state anew; where they are positive, 64 of them sum to less than 88.
         initial (torch.Tensor, optional): shape (B, heads, key_dim, value_dim), fp32: the states to start from
             (zero if absent); with ``offsets`` one per sequence.
         scale (float, optional): factor of the outputs, ``key_dim ** -0.5`` if absent.
@@ -138,7 +145,8 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
     Returns:
         (torch.Tensor, torch.Tensor): the outputs, shape (B, T, heads, value_dim), and the states behind the last
         tokens, fp32, as ``initial`` has them: hand them to the next chunk or to ``gated_delta_step``.
-        Differentiable in all tensors but ``offsets``.
+        Differentiable once in all tensors but ``offsets``.  A token that is not finite leaves the outputs of the
+        tokens before it as they are.
     """
     _check_scan(queries, keys, values, log_gates, beta, initial, offsets)
     scale = float(scale) if scale is not None else queries.shape[-1] ** -0.5
@@ -192,4 +200,6 @@ def gated_delta_step(queries, keys, values, log_gates, beta, states, slots=None,
         return _ops.delta_step(queries, keys, values, log_gates, beta, states, slots, scale)
     out = torch.empty_like(values)
     _abi.delta_step(queries, keys, values, log_gates, beta, states, slots, scale, out)
+    if not states.is_inference():
+        torch.autograd.graph.increment_version(states)
     return out

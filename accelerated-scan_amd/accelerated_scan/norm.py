@@ -8,6 +8,7 @@ The reference has no operator of this kind.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _abi, _ops
 
@@ -58,8 +59,14 @@ class GatedNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_out):
-        x, gate, weight = ctx.saved_tensors
-        return (*_ops.gated_norm_backward_run(x, gate, weight, d_out.contiguous(), ctx.eps), None)
+        if torch.is_grad_enabled() and not _ops.capturing():  # create_graph: no second derivatives
+            return once_differentiable(_gradients)(ctx, d_out)
+        return _gradients(ctx, d_out)
+
+
+def _gradients(ctx, d_out):
+    x, gate, weight = ctx.saved_tensors
+    return (*_ops.gated_norm_backward_run(x, gate, weight, d_out.contiguous(), ctx.eps), None)
 
 
 def gated_norm(x, gate, weight, eps=1e-6):
@@ -72,7 +79,7 @@ def gated_norm(x, gate, weight, eps=1e-6):
         eps (float): added to the mean of the squares.
 
     Returns:
-        (torch.Tensor): the shape of x; differentiable in x, gate and weight.
+        (torch.Tensor): the shape of x; differentiable once in x, gate and weight.
     """
     _check(x, gate, weight)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or weight.requires_grad):

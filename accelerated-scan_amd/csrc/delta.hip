@@ -12,6 +12,7 @@ int element_bytes(int dtype) { return dtype == ASCAN_F32 ? 4 : (dtype == ASCAN_B
 constexpr int64_t kMaxHeads = 65535, kMaxRows = INT64_C(1) << 40, kMaxSequences = 65535;
 constexpr int64_t kMaxKeyDim = 128, kMaxValueDim = 4096;
 constexpr int64_t kMaxRowElements = INT64_C(1) << 22;  // of a token: 64 tokens stay below 2^31 bytes
+constexpr int64_t kMaxThreads = INT64_C(4294967295);   // of an axis of a launch
 
 bool heads_ok(int64_t heads, int64_t key_heads, int64_t dk, int64_t dv) {
     return heads > 0 && heads <= kMaxHeads && key_heads > 0 && heads % key_heads == 0 && dk > 0 && dk <= kMaxKeyDim &&
@@ -22,7 +23,11 @@ bool heads_ok(int64_t heads, int64_t key_heads, int64_t dk, int64_t dv) {
 bool rows_ok(int64_t rows, int64_t sequences, bool packed) {
     if (rows < 0 || sequences < 0 || rows > kMaxRows || sequences > kMaxSequences) return false;
     if (!packed && (sequences == 0 ? rows != 0 : rows % sequences != 0)) return false;
-    return delta_blocks(rows, sequences, packed) <= INT64_C(2147483647);
+    return delta_blocks(rows, sequences, packed) <= kMaxThreads / 512;
+}
+// Workgroups of the chains: one to 16 columns of every sequence's every head, in whole rounds of eight.
+bool chains_ok(int64_t sequences, int64_t heads, int64_t dv) {
+    return ((sequences * heads + 7) / 8 * 8) * ((dv + 15) / 16) <= kMaxThreads / 768;
 }
 
 bool misaligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
@@ -77,7 +82,7 @@ int check_scan(const void* const* inputs, size_t count, int64_t rows, int64_t se
                int64_t dk, int64_t dv, int dtype, int flags, const void* offsets, int gate_bytes) {
     if (element_bytes(dtype) == 0) return ASCAN_ERR_BAD_DTYPE;
     if (!heads_ok(heads, key_heads, dk, dv)) return ASCAN_ERR_BAD_HEADS;
-    if (!rows_ok(rows, sequences, offsets != nullptr)) return ASCAN_ERR_BAD_SHAPE;
+    if (!rows_ok(rows, sequences, offsets != nullptr) || !chains_ok(sequences, heads, dv)) return ASCAN_ERR_BAD_SHAPE;
     if (misaligned(offsets, flags & ASCAN_DELTA_OFFSETS_I64 ? 8 : 4)) return ASCAN_ERR_MISALIGNED;
     if (rows > 0 && sequences > 0) {
         for (size_t i = 0; i < count; ++i) {
@@ -99,7 +104,9 @@ int64_t ascan_delta_blocks(int64_t rows, int64_t sequences, int packed) {
 
 size_t ascan_delta_workspace_bytes(int64_t rows, int64_t sequences, int64_t heads, int64_t key_heads, int64_t dk,
                                    int64_t dv, int dtype, int packed, int backward) {
-    if (element_bytes(dtype) == 0 || !heads_ok(heads, key_heads, dk, dv) || !rows_ok(rows, sequences, packed != 0)) return 0;
+    if (element_bytes(dtype) == 0 || !heads_ok(heads, key_heads, dk, dv) || !rows_ok(rows, sequences, packed != 0) ||
+        !chains_ok(sequences, heads, dv))
+        return 0;
     static const int32_t some = 0;  // only whether there are offsets counts here
     return workspace_of(shape_of(packed ? &some : nullptr, rows, sequences, heads, key_heads, dk, dv, 1.0f, 0), dtype, backward != 0);
 }
@@ -180,7 +187,8 @@ int ascan_delta_step(const void* q, const void* k, const void* v, const void* lo
     const int es = element_bytes(dtype), gs = flags & ASCAN_DELTA_GATES_F32 ? 4 : es;
     if (es == 0) return ASCAN_ERR_BAD_DTYPE;
     if (!heads_ok(heads, key_heads, dk, dv)) return ASCAN_ERR_BAD_HEADS;
-    if (batch < 0 || state_count < 0 || state_count > kMaxRows || batch > 2147483647 / (heads * ((dv + 31) / 32)))
+    if (batch < 0 || state_count < 0 || state_count > INT64_MAX / 4 / (heads * dk * dv) ||
+        batch > kMaxThreads / 256 / (heads * ((dv + 31) / 32)))
         return ASCAN_ERR_BAD_SHAPE;
     if (slots == nullptr && batch > state_count) return ASCAN_ERR_BAD_SHAPE;
     if (batch == 0) return ASCAN_OK;

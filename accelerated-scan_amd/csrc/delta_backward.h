@@ -151,11 +151,13 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma_all<NS, NS>(tm[1], high, u);
                 if (wave < 2) {
                     u2 = mma_all<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
+                    u = mma_all<NS, NS>(tm[1], high, u);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
+                } else {
+                    u = mma_all<NS, NS>(tm[1], high, u);
                 }
             }
             {
@@ -218,9 +220,9 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         };
         const auto outputs = [&](int64_t n_block, int set) __attribute__((always_inline)) {  // P^T dO
             const Tile<NI, 16> ot = outs_at(n_block);
-            fx4 po = mma<NC, NI>(pm[set][1], ot.down(32, 0, lane), fx4{0, 0, 0, 0});
+            fx4 po = {0, 0, 0, 0};
             if (wave < 2) po = mma<NC, NI>(pm[set][0], ot.down(0, 0, lane), po);
-            po_at[wave * 64] = po;
+            po_at[wave * 64] = mma<NC, NI>(pm[set][1], ot.down(32, 0, lane), po);
         };
         load_p(last, 0);
         load_p(last - 1, 1);
@@ -559,14 +561,20 @@ __global__ __launch_bounds__(512) void delta_gradients(
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     if (t <= own) early[t] = mma<NS, NI>(ut.along(16 * t + c, 32 * i, g), o, early[t]);
-                    if (t >= own) late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
+                    if (t >= own) {
+                        late[t] = mma<NI, NS>(ot.along(16 * t + c, 32 * i, g), u, late[t]);
+                        asm volatile("s_nop 1" : "+v"(late[t]));  // (behind the branches that follow the compiler waits too little)
+                    }
                 }
             } else {
                 const Operand<NS> r = rt.along(16 * own + c, 32 * i, g);
 #pragma unroll
                 for (int t = 0; t < kTiles; ++t) {
                     if (t <= own) early[t] = mma<NS, NS>(ut.along(16 * t + c, 32 * i, g), r, early[t]);
-                    if (t >= own) late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
+                    if (t >= own) {
+                        late[t] = mma<NS, NS>(rt.along(16 * t + c, 32 * i, g), u, late[t]);
+                        asm volatile("s_nop 1" : "+v"(late[t]));
+                    }
                 }
             }
         }

@@ -60,11 +60,32 @@ __device__ __forceinline__ int touch(const Lines& l, int id) {
 
 template <int NI, int NS, int NC, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                            2 * Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4;
+                            2 * Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4 + 64;
 
 // Pieces of 16 bytes of T that each of 256 threads carries to LDS.
 template <int NC>
 constexpr int kPieces = (kMatrixBytes<NC> / 16 + 255) / 256;
+
+// Zeros for what is not finite in an operand of tokens; the first such token, where its first four are row0 ..
+template <int P>
+__device__ __forceinline__ int zero_odd(Operand<P>& o, int row0) {
+    int odd = kBlock;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+        bool is;
+        if constexpr (P == 0) {
+            is = is_odd(o.t[e >> 2][e & 3]);
+            if (is) o.t[e >> 2][e & 3] = 0.0f;
+        } else {
+            is = is_odd((float)o.p[0][e]);
+#pragma unroll
+            for (int n = 0; n < P; ++n)
+                if (is) o.p[n][e] = (__bf16)0.0f;
+        }
+        if (is) odd = row0 + (e >> 2) * 16 + (e & 3);
+    }
+    return odd;
+}
 
 // q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.  KEEP: write the states in front
 // of the blocks and the rows U.
@@ -106,6 +127,10 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     m += Exchange<NC, 2>::kBytes;
     char* const matrix_at = m;
     float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NS>);
+    // Per column the first token of the block at hand from which its state is not finite.  A NaN in R meets the zeros of T
+    // and would meet those of P and reach earlier tokens: U, which shows it, is computed again with a zero in its place,
+    // and state and outputs get the NaN by this number.  (A test of R itself stands on every block's way.)
+    int* const odd_at = reinterpret_cast<int*>(gate_at + 2 * 4 * kBlock);
 
     constexpr uint32_t kSize = sizeof(ES);
     const uint32_t v_step = s.heads * s.dv * kSize;
@@ -157,6 +182,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             beta = gate_rows(first, kBeta);
             beta_since = gate_rows(first, kBetaSince);
         };
+        if (tid < 16) odd_at[tid] = kBlock;
         __builtin_amdgcn_s_setprio(3);
         if (seq_length > 0) {
             lds_barrier();  // the first block's keys and values are there
@@ -192,6 +218,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             // R = diag(beta) V - diag(beta e^c) K S0
 #pragma unroll
             for (int r = 0; r < 4; ++r) u[r] = beta[r] * x[r] - beta_since[r] * (u[r] + u2[r]);
+            const fx4 own = u;
             xr.put(wave, lane, u);
             lds_barrier();
 
@@ -205,11 +232,15 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                     k_high[t] = kb.down_features(32, kOwn * wave + t, lane);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-                u = mma_all<NS, NS>(tm[0], low, u);
+                // (one branch around all of it: where a branch stands between a matrix instruction and the first use of its
+                // result, the compiler has left out the wait)
                 if (wave >= 2) {
                     u2 = mma_all<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
+                    u = mma_all<NS, NS>(tm[0], low, u);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
+                } else {
+                    u = mma_all<NS, NS>(tm[0], low, u);
                 }
             }
             {
@@ -219,6 +250,31 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 xd.put(wave, lane, y);
             }
             xu.put(wave, lane, u);
+            if (__any(is_odd(u[0]) || is_odd(u[1]) || is_odd(u[2]) || is_odd(u[3]))) {
+                // again without what is not finite
+                Operand<NS> low = xr.get(0, lane), high = xr.get(1, lane);
+                int odd = wave >= 2 ? zero_odd(high, 32 + 4 * g) : kBlock;
+                odd = min(odd, zero_odd(low, 4 * g));
+                odd = min(odd, __shfl_xor(odd, 16));
+                odd = min(odd, __shfl_xor(odd, 32));
+                u = mma_all<NS, NS>(matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane), low, fx4{0, 0, 0, 0});
+                u2 = mma_all<NS, NS>(matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane), high, fx4{0, 0, 0, 0});
+                fx4 y;
+#pragma unroll
+                for (int r = 3; r >= 0; --r) {
+                    u[r] += own[r] + (wave >= 2 ? u2[r] : 0.0f);
+                    if (is_odd(u[r])) odd = min(odd, 16 * wave + 4 * g + r);
+                }
+                atomicMin(odd_at + c, odd);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool gone = 16 * wave + 4 * g + r >= odd;
+                    y[r] = gone ? __builtin_nanf("") : until[r] * u[r];
+                    u[r] = gone ? 0.0f : u[r];
+                }
+                xd.put(wave, lane, y);
+                xu.put(wave, lane, u);
+            }
             lds_barrier();
 
             // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
@@ -316,11 +372,19 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             for (int r = 0; r < 4; ++r) o[r] = f * (o[r] + o2[r]);
             lds_barrier();
             // out^T = scale (Q S0)^T diag(e^c) + U^T P^T
-            o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
+            int odd[4];
+            __builtin_memcpy(odd, odd_at + 4 * g, 16);
             if (wave >= 2) {
                 o2 = mma<NS, NS>(xu.get(1, lane), pm[own][1], fx4{0, 0, 0, 0});
+                o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] += o2[r];
+            } else {
+                o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
+            }
+            if (__any(odd[0] < kBlock || odd[1] < kBlock || odd[2] < kBlock || odd[3] < kBlock)) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] = token >= odd[r] ? __builtin_nanf("") : o[r];
             }
             put4<E>(rows_of(out_p, first, v_step, s.dv * kSize), quad < s.dv ? token * v_step + quad * kSize : kOutside, o);
             out_p += v_move;

@@ -60,7 +60,7 @@ __device__ __forceinline__ BlockAt block_at(const DeltaShape& s, int64_t block) 
     }
     const SequenceAt q = sequence_at(s, n);
     const int64_t first = (block - q.block) * kBlock;
-    const int64_t left = q.length - first;
+    const int64_t left = first < 0 ? 0 : q.length - first;  // (first entries of a table that does not ascend do not either)
     return BlockAt{q.row + first, (int)(left < 0 ? 0 : (left > kBlock ? kBlock : left)), n};
 }
 
@@ -134,6 +134,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
                                                      typename E::S* __restrict__ q_out) {
     extern __shared__ __align__(16) char smem[];
     __shared__ float high[kBlock], low[kBlock], rate[kBlock];
+    __shared__ int odd_at;
     const int64_t block = blockIdx.x;
     const int head = blockIdx.y, key_head = head / (s.heads / s.key_heads);
     const BlockAt at = block_at(s, block);
@@ -142,6 +143,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
 
     const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
     float b = 0.0f, x = 0.0f;
+    if (tid == 0) odd_at = kBlock;
     {
         constexpr uint32_t kSize = sizeof(typename E::S);
         const int64_t row0 = uniform(at.row);
@@ -194,6 +196,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
         to[kUntil * kBlock] = exp_of((float)(whole - sum));
         to[kSumHigh * kBlock] = h;
         to[kSumLow * kBlock] = l;
+        if (is_odd(h) || is_odd(b)) atomicMin(&odd_at, lane);
     }
 
     // kk: K_j K_i^T with i the own tile and j up to it.  pq: K_j Q_i^T, or with `upper` Q_i K_j^T for j the own tile and
@@ -215,7 +218,18 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
         }
     }
     const int here = 16 * wave + c;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+        if (j == wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (4 * g + r == c && is_odd(kk[j][r])) atomicMin(&odd_at, here);
+        }
     __syncthreads();  // the tiles' memory is taken over by L^T and the inverse
+    // T and P have zeros from the first token on whose key (by its product with itself), beta or gate is not finite; the chain
+    // finds that token by its R, which its beta makes NaN.
+    const int odd = odd_at, here_up_to = here < odd ? here : -1;
+    if (tid == odd && odd < kBlock) gates[(block * s.heads + head) * kGateFloats + kBeta * kBlock + tid] = __builtin_nanf("");
     const float high_here = high[here], low_here = low[here], rate_here = rate[here];
 
     float *lt = reinterpret_cast<float*>(smem), *xm = lt + kBlock * kMatrixRow;
@@ -232,7 +246,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
         if (j <= wave) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                lt[(row0 + r) * kMatrixRow + here] = row0 + r < here ? rate_here * e[r] * kk[j][r] : 0.0f;
+                lt[(row0 + r) * kMatrixRow + here] = row0 + r < here_up_to ? rate_here * e[r] * kk[j][r] : 0.0f;
         }
         if (upper && j == wave) {
 #pragma unroll
@@ -240,7 +254,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            pq[j][r] = (upper ? row0 + r >= here : row0 + r <= here) ? s.scale * e[r] * pq[j][r] : 0.0f;
+            pq[j][r] = (upper ? row0 + r >= here && row0 + r < odd : row0 + r <= here_up_to) ? s.scale * e[r] * pq[j][r] : 0.0f;
     }
     {
         char* to = p_out + (block * s.heads + head) * kMatrixBytes<NP>;

@@ -507,10 +507,13 @@ __device__ __forceinline__ float sum16(float x) {
     return x;
 }
 
+// NaN or infinite.
+__device__ __forceinline__ bool is_odd(float x) { return __builtin_amdgcn_classf(x, 0x207); }
+
 // e^x to 2^-22 of its value: 2^(x log2 e) from the hardware, with the product's rounding error put back.
 __device__ __forceinline__ float exp_of(float x) {
     constexpr float kHigh = 1.44269502f, kLow = 1.92596299e-8f;  // log2 e
-    x = fmaxf(x, -200.0f);  // (0 from there on, and -inf has no product with a rounding error)
+    x = x < -200.0f ? -200.0f : x;  // (0 from there on, and -inf has no product with a rounding error; NaN stays)
     const float t = x * kHigh;
     const float rest = fmaf(x, kHigh, -t) + x * kLow;
     const float p = __builtin_amdgcn_exp2f(t);

@@ -412,8 +412,9 @@ ASCAN_API int ascan_backward_gated_values(const void* gate_inputs, const void* v
  *   - the workspace has the size that ascan_delta_workspace_bytes gives, and belongs to the call until it has run.
  *     Its contents on entry do not matter;
  *   - a log gate below -1000, -inf among them, is a gate of zero: the state starts anew there;
- *   - tokens are taken in blocks of 64 from the start of each sequence: a NaN or an infinity in a token can reach
- *     the outputs of earlier tokens of its block, never those of earlier blocks or of other sequences.
+ *   - a NaN or an infinity in a token reaches no output of an earlier token.  Gradients are taken in blocks of 64
+ *     tokens from the start of each sequence, and it can reach those of its whole block and of all earlier ones;
+ *   - the log gates of a block sum to less than 88 from any token to a later one (e^88 is the end of fp32).
  *
  * ascan_delta_step advances the states of `batch` conversations by one token (q and k (batch, key_heads, dk), ...) in
  * place.  Row b uses states[slots[b]] (slots: int32, or int64 with ASCAN_DELTA_OFFSETS_I64), states[b] where slots is

@@ -25,7 +25,7 @@ def forward(p, **change):
     """Arguments of a valid call on 2 x 70 tokens with buffers 64 KiB apart, with some of them changed."""
     a = dict(q=p, k=p + 0x10000, v=p + 0x20000, log_gates=p + 0x30000, beta=p + 0x31000, initial=None, offsets=None,
              out=p + 0x40000, final=None, states=None, updates=None, rows=140, sequences=2, heads=2, key_heads=1, dk=16,
-             dv=16, scale=1.0, dtype=0, flags=0, workspace=p + 0x80000, bytes=1 << 18, stream=None)
+             dv=16, scale=1.0, dtype=0, flags=0, workspace=p + 0x80000, bytes=1 << 19, stream=None)
     a.update(change)
     return _abi.load().ascan_delta_forward(*a.values())
 
@@ -34,7 +34,7 @@ def backward(p, **change):
     a = dict(q=p, k=p + 0x4000, v=p + 0x8000, log_gates=p + 0x10000, beta=p + 0x11000, states=p + 0x14000,
              updates=p + 0x20000, offsets=None, d_out=p + 0x28000, d_final=None, d_q=p + 0x30000, d_k=p + 0x34000,
              d_v=p + 0x38000, d_log_gates=p + 0x40000, d_beta=p + 0x41000, d_initial=None, rows=140, sequences=2, heads=2,
-             key_heads=1, dk=16, dv=16, scale=1.0, dtype=0, flags=0, workspace=p + 0x60000, bytes=1 << 19, stream=None)
+             key_heads=1, dk=16, dv=16, scale=1.0, dtype=0, flags=0, workspace=p + 0x60000, bytes=0xa0000, stream=None)
     a.update(change)
     return _abi.load().ascan_delta_backward(*a.values())
 
@@ -233,3 +233,13 @@ def test_the_definition_itself():
             o = 0.5 * sum(S[i][j] * q[0, t, 0, i].item() for i in range(8))
             assert abs(o - want[0, t, 0, j].item()) < 1e-12
     assert all(abs(S[i][j] - final[0, 0, i, j].item()) < 1e-12 for i in range(8) for j in range(8))
+
+
+def test_launches_beyond_the_hardware_are_refused(room):
+    wide = dict(rows=0, sequences=65535, heads=64, key_heads=64, dk=128, dv=128)  # 33 million workgroups of 768 threads
+    assert forward(room, **wide, final=room) == SHAPE and backward(room, **wide, d_initial=room) == SHAPE
+    assert _abi.load().ascan_delta_workspace_bytes(0, 65535, 64, 64, 128, 128, 0, 0, 0) == 0
+    many = dict(heads=1, key_heads=1, dk=8, dv=8)
+    assert forward(room, rows=1 << 30, sequences=1, **many) == SHAPE  # 2^24 blocks
+    assert step(room, batch=1 << 24, count=1 << 24, **many) == SHAPE
+    assert step(room, count=1 << 62) == SHAPE

@@ -462,3 +462,210 @@ def test_empty_inputs():
     assert not out.any() and final.shape == (0, 2, 16, 16)
     step = delta.gated_delta_step(new(0, 1, 16), new(0, 1, 16), new(0, 2, 16), new(0, 2), new(0, 2), new(0, 2, 16, 16))
     assert step.shape == (0, 2, 16)
+
+
+@pytest.mark.parametrize("t", [0, 37, 64, 149])
+@pytest.mark.parametrize("what", ["queries", "keys", "values", "log_gates", "beta"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_tokens_that_are_not_finite_leave_earlier_ones_alone(dtype, what, t):
+    """As in a padded batch whose padding holds anything."""
+    from accelerated_scan import delta
+
+    for dk, bad in ((64, float("nan")), (128, float("inf"))):
+        data = ref.inputs(1, 150, 2, 2, dk, 40, dtype, seed=31)
+        want, state = ref.delta_scan(*as_exact(data))
+        broken = [x.clone() for x in data]
+        x = broken[NAMES.index(what)]
+        if x.dim() == 4:
+            x[0, t, 1, 5] = bad
+        else:
+            x[0, t, 1] = bad
+        got, final = delta.gated_delta_scan(*on_gpu(broken))
+        got, final = got.cpu(), final.cpu()
+        ref.close(got[:, :, :1], want[:, :, :1], dtype, what="the other head")
+        ref.close(final[:, :1], state[:, :1], dtype, what="the other head's state")
+        if t:
+            ref.close(got[:, :t], want[:, :t], dtype, what="earlier tokens")
+        if what == "queries":
+            assert not torch.isfinite(got[0, t, 1]).any()
+            if t < 149:
+                ref.close(got[:, t + 1:], want[:, t + 1:], dtype, what="later tokens")
+            ref.close(final, state, dtype, what="final")
+            continue
+        if what == "values":
+            others = [c for c in range(40) if c != 5]
+            ref.close(got[..., others], want[..., others], dtype, what="other columns")
+            ref.close(final[..., others], state[..., others], dtype, what="other columns of the state")
+            got, final = got[..., 5:6], final[..., 5:6]
+        assert not torch.isfinite(got[0, t:, 1]).any()
+        assert not torch.isfinite(final[0, 1]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_gradients_beside_padding_that_is_not_finite(dtype):
+    """Values that are NaN behind the end of each sequence of a batch, where no gradient comes from."""
+    from accelerated_scan import delta
+
+    T, ends = 150, (81, 130)
+    data = ref.inputs(2, T, 1, 2, 64, 40, dtype, seed=32)
+    d_out = torch.randn(2, T, 2, 40, generator=torch.Generator().manual_seed(33)).to(dtype)
+    for b, end in enumerate(ends):
+        d_out[b, end:] = 0
+    exact = as_exact(data, grad=True)
+    want = torch.autograd.grad(ref.delta_scan(*exact)[0], exact, d_out.double())
+    for b, end in enumerate(ends):
+        data[2][b, end:] = float("nan")
+    leaves = on_gpu(data, grad=True)
+    got = torch.autograd.grad(delta.gated_delta_scan(*leaves)[0], leaves, d_out.to(DEVICE))
+    for name, a, b in zip(NAMES, got, want):
+        for n, end in enumerate(ends):
+            rows = slice(None) if name == "initial" else slice(0, end)
+            ref.close(a[n][rows], b[n][rows], dtype, backward=True, what=name)
+
+
+@pytest.mark.parametrize("packed", [False, True], ids=["one", "packed"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_many_blocks(dtype, packed):
+    """Long enough that every block of a chain is asked for ahead by another one; four heads to a key head."""
+    from accelerated_scan import delta
+
+    T, ends = 64 * 11 + 17, [0, 64 * 9 + 1, 64 * 11 + 17]
+    data = ref.inputs(1, T, 1, 4, 128, 32, dtype, seed=34, sequences=2 if packed else None)
+    exact = as_exact(data, grad=True)
+    d_out = torch.randn(1, T, 4, 32, generator=torch.Generator().manual_seed(35)).to(dtype)
+    if packed:
+        parts = [ref.delta_scan(*(x[:, a:b] for x in exact[:5]), exact[5][n:n + 1]) for n, (a, b) in enumerate(zip(ends, ends[1:]))]
+        out, final = (torch.cat(x, d) for x, d in zip(zip(*parts), (1, 0)))
+    else:
+        out, final = ref.delta_scan(*exact)
+    d_final = torch.randn(final.shape, generator=torch.Generator().manual_seed(36))
+    want = torch.autograd.grad([out, final], exact, [d_out.double(), d_final.double()])
+    leaves = on_gpu(data, grad=True)
+    offsets = torch.tensor(ends, dtype=torch.int32, device=DEVICE) if packed else None
+    results = delta.gated_delta_scan(*leaves, offsets=offsets)
+    ref.close(results[0], out, dtype, what="out")
+    ref.close(results[1], final, dtype, what="final")
+    for name, a, b in zip(NAMES, torch.autograd.grad(results, leaves, on_gpu([d_out, d_final])), want):
+        ref.close(a, b, dtype, backward=True, what=name)
+
+
+def test_gradients_that_are_pieces_of_larger_tensors():
+    from accelerated_scan import delta, norm
+
+    data = on_gpu(ref.inputs(1, 70, 1, 2, 16, 16, torch.bfloat16, seed=37), grad=True)
+    weight = torch.ones(16, device=DEVICE, dtype=torch.bfloat16, requires_grad=True)
+    out, final = delta.gated_delta_scan(*data)
+    gated = norm.gated_norm(out, data[2], weight)
+    gen = torch.Generator(DEVICE).manual_seed(38)
+    pieces = [torch.randn(t.numel() + 1, generator=gen, device=DEVICE).to(t.dtype) for t in (out, final, gated)]
+    odd = [p[1:].view(t.shape) for p, t in zip(pieces, (out, final, gated))]
+    assert all(t.data_ptr() % 16 for t in odd)
+    inputs = [*data, weight]
+    got = torch.autograd.grad([out, final, gated], inputs, odd, retain_graph=True)
+    want = torch.autograd.grad([out, final, gated], inputs, [t.clone() for t in odd])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_second_derivatives_are_refused():
+    from accelerated_scan import delta, norm
+
+    data = on_gpu(ref.inputs(1, 70, 1, 2, 16, 16, torch.float32, seed=39), grad=True)
+    weight = torch.ones(16, device=DEVICE, requires_grad=True)
+    out, _ = delta.gated_delta_scan(*data)
+    for result, leaf in ((out, data[0]), (norm.gated_norm(data[2], data[2], weight), weight)):
+        (first,) = torch.autograd.grad(result.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+
+
+def test_step_marks_its_states_as_changed():
+    from accelerated_scan import delta
+
+    q, k, v, g, b, states = on_gpu(ref.inputs(2, 1, 1, 2, 16, 16, torch.float32, seed=40))
+    factor = torch.ones((), device=DEVICE, requires_grad=True)
+    kept = factor * states  # keeps the states for its gradient
+    with torch.no_grad():
+        delta.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], b[:, 0], states)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
+    with torch.inference_mode():
+        held = states.clone()
+        out = delta.gated_delta_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], b[:, 0], held)
+        assert torch.isfinite(out).all()
+
+
+def test_offsets_that_do_not_ascend():
+    """Unspecified values, and no access outside: what follows is right."""
+    from accelerated_scan import delta
+
+    data = on_gpu(ref.inputs(1, 300, 1, 2, 32, 32, torch.bfloat16, seed=41, sequences=5), grad=True)
+    good = torch.tensor([0, 40, 40, 150, 299, 300], device=DEVICE)
+    want = delta.gated_delta_scan(*data, offsets=good)
+    for table in ([130, 10, 200, 70, 300, 0], [-5, 600, -1, 64, 128, 1 << 40], [300, 200, 100, 50, 20, 0]):
+        out, final = delta.gated_delta_scan(*data, offsets=torch.tensor(table, device=DEVICE))
+        torch.autograd.grad([out, final], data, [torch.ones_like(out), torch.ones_like(final)])
+    got = delta.gated_delta_scan(*data, offsets=good)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tensors_beyond_two_to_the_31():
+    """The last tokens of a sequence whose values have more elements than 32 bits count, and a slot behind as many
+    state elements."""
+    from accelerated_scan import delta
+
+    heads, dv, T, cut = 32, 128, (1 << 19) + 200, (1 << 19) - 64 * 3
+    gen = torch.Generator(DEVICE).manual_seed(42)
+    new = lambda *s: torch.randn(s, generator=gen, device=DEVICE, dtype=torch.bfloat16)  # noqa: E731
+    q, k = (torch.nn.functional.normalize(new(1, T, 1, 8), dim=-1) for _ in range(2))
+    v = new(1, T, heads, dv)
+    g, b = -new(1, T, heads).abs(), new(1, T, heads).sigmoid()
+    out, final = delta.gated_delta_scan(q, k, v, g, b)
+    head, state = delta.gated_delta_scan(*(t[:, :cut].contiguous() for t in (q, k, v, g, b)))
+    tail, last = delta.gated_delta_scan(*(t[:, cut:].contiguous() for t in (q, k, v, g, b)), state)
+    assert torch.equal(out[:, :cut], head) and torch.equal(out[:, cut:], tail) and torch.equal(final, last)
+    del head, tail, out
+    part = [t[:, cut:].contiguous().requires_grad_() for t in (q, k, v, g, b)]
+    out, _ = delta.gated_delta_scan(*part, state)
+    want = torch.autograd.grad(out, part, torch.ones_like(out))
+    whole = [t.requires_grad_() for t in (q, k, v, g, b)]
+    out, _ = delta.gated_delta_scan(*whole)
+    got = torch.autograd.grad(out, whole, torch.ones_like(out))
+    for a, w in zip(got, want):
+        assert torch.equal(a[:, cut:], w)
+    del got, out, whole, v
+    states = torch.zeros(4100, 32, 128, 128, device=DEVICE)
+    token = [new(2, 1, 128), new(2, 1, 128), new(2, 32, 128), -new(2, 32).abs(), new(2, 32).sigmoid()]
+    small = states[:2].clone()
+    out = delta.gated_delta_step(*token, states, slots=torch.tensor([4099, 0], device=DEVICE))
+    assert torch.equal(out, delta.gated_delta_step(*token, small))
+    assert torch.equal(states[4099], small[0]) and torch.equal(states[0], small[1]) and not states[1:4099].any()
+
+
+def test_captured_training_step():
+    from accelerated_scan import delta, norm
+
+    data = on_gpu(ref.inputs(2, 150, 1, 2, 64, 64, torch.bfloat16, seed=43), grad=True)
+    weight = torch.ones(64, device=DEVICE, dtype=torch.bfloat16, requires_grad=True)
+    d_out = torch.randn(2, 150, 2, 64, generator=torch.Generator().manual_seed(44)).to(DEVICE, torch.bfloat16)
+    inputs = [*data, weight]
+
+    def gradients():
+        out, _ = delta.gated_delta_scan(*data)
+        return torch.autograd.grad(norm.gated_norm(out, data[2], weight), inputs, d_out)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = gradients()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = gradients()
+    for turn in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        gradients()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
