@@ -314,6 +314,19 @@ def _delta_forward(queries, keys, values, log_gates, beta, initial, offsets, sca
     return out, final, states, updates
 
 
+def delta_outputs(queries, keys, values, log_gates, beta, initial, offsets, scale):
+    """(out, final) alone, by the direct call."""
+    sequences = queries.shape[0] if offsets is None else offsets.shape[0] - 1
+    out = torch.empty_like(values)
+    final = torch.empty((sequences, values.shape[2], queries.shape[3], values.shape[3]), dtype=torch.float32,
+                        device=values.device)
+    if sequences == 0:
+        out.zero_()  # rows outside all sequences
+    else:
+        _abi.delta_forward(queries, keys, values, log_gates, beta, initial, offsets, scale, out, final)
+    return out, final
+
+
 @torch.library.custom_op("accelerated_scan::delta_forward", mutates_args=())
 def delta_forward(
     queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, log_gates: torch.Tensor, beta: torch.Tensor,

@@ -69,7 +69,25 @@ def _check_heads(queries, keys, values, log_gates, beta):
               f"{value_dim}")
 
 
+def _plainly_right(queries, keys, values, log_gates, beta):
+    """Whether a call passes the checks of what both operators have in common (no message is built)."""
+    lead_heads, dtype, device = values.shape[:-1], queries.dtype, queries.device
+    *lead, key_heads, key_dim = queries.shape
+    heads, value_dim = lead_heads[-1], values.shape[-1]
+    return (dtype in _REAL_DTYPES and keys.dtype == dtype and values.dtype == dtype and beta.dtype == log_gates.dtype
+            and (log_gates.dtype == dtype or log_gates.dtype == torch.float32) and keys.shape == queries.shape
+            and log_gates.shape == lead_heads and beta.shape == lead_heads and (*lead, heads) == lead_heads
+            and key_heads and heads and heads % key_heads == 0 and 0 < key_dim <= 128 and key_dim % 8 == 0
+            and 0 < value_dim <= 4096 and value_dim % 8 == 0
+            and queries.is_cuda and keys.device == device and values.device == device and log_gates.device == device
+            and beta.device == device and queries.is_contiguous() and keys.is_contiguous() and values.is_contiguous()
+            and log_gates.is_contiguous() and beta.is_contiguous())
+
+
 def _check_scan(queries, keys, values, log_gates, beta, initial, offsets):
+    if (initial is None and offsets is None and queries.dim() == 4 and values.dim() == 4
+            and _plainly_right(queries, keys, values, log_gates, beta)):
+        return queries.shape[0]
     if queries.dim() != 4 or values.dim() != 4:
         _fail("expected queries, keys and values of shape (B, T, heads, dim)")
     _check_types(queries, keys, values, log_gates, beta)
@@ -154,10 +172,20 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
                                     or log_gates.requires_grad or beta.requires_grad
                                     or (initial is not None and initial.requires_grad)):
         return GatedDeltaScan.apply(queries, keys, values, log_gates, beta, initial, offsets, scale)
-    return _ops.delta_forward_run(queries, keys, values, log_gates, beta, initial, offsets, scale, False)[:2]
+    if _ops.capturing():
+        return _ops.delta_forward(queries, keys, values, log_gates, beta, initial, offsets, scale, False)[:2]
+    return _ops.delta_outputs(queries, keys, values, log_gates, beta, initial, offsets, scale)
 
 
 def _check_step(queries, keys, values, log_gates, beta, states, slots):
+    if (queries.dim() == 3 and values.dim() == 3 and states.dtype == torch.float32 and states.dim() == 4
+            and states.shape[1:] == (values.shape[1], queries.shape[2], values.shape[2]) and states.device == queries.device
+            and states.is_contiguous()
+            and (states.shape[0] == queries.shape[0] if slots is None else
+                 slots.shape == queries.shape[:1] and slots.dtype in (torch.int32, torch.int64)
+                 and slots.device == queries.device and slots.is_contiguous())
+            and _plainly_right(queries, keys, values, log_gates, beta)):
+        return
     if queries.dim() != 3 or values.dim() != 3:
         _fail("expected queries, keys and values of shape (B, heads, dim)")
     _check_types(queries, keys, values, log_gates, beta)
@@ -193,7 +221,8 @@ def gated_delta_step(queries, keys, values, log_gates, beta, states, slots=None,
         (torch.Tensor): the outputs, shape (B, heads, value_dim).
     """
     _check_step(queries, keys, values, log_gates, beta, states, slots)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (queries, keys, values, log_gates, beta, states)):
+    if torch.is_grad_enabled() and (queries.requires_grad or keys.requires_grad or values.requires_grad
+                                    or log_gates.requires_grad or beta.requires_grad or states.requires_grad):
         _fail("gated_delta_step is not differentiable: use gated_delta_scan, or torch.no_grad()")
     scale = float(scale) if scale is not None else queries.shape[-1] ** -0.5
     if _ops.capturing():
