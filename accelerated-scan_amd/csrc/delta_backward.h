@@ -18,6 +18,7 @@
 namespace ascan {
 namespace {
 
+constexpr int kAhead = 256;   // workgroups from one to that which takes its place: one to a compute unit
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
 template <int NI, int NS, int NC, int DK>
@@ -366,12 +367,18 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     }
 }
 
+// dO, U and dR of kColumns columns in LDS.  The second pass over the columns goes back: with room for two such sets it finds
+// the last two where the first pass has left them.
 template <int NI, int NS>
-constexpr int kGradientShared = Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes > 4 * Exchange<NS, kPairs>::kBytes
-                                    ? Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes
+constexpr int kRowsBytes = Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes;
+template <int NI, int NS, int DK>
+constexpr int kRowSets = 2 * Tile<NI, DK>::kBytes + 2 * kRowsBytes<NI, NS> + 8 * 1024 <= 160 * 1024 ? 2 : 1;
+template <int NI, int NS, int DK>
+constexpr int kGradientShared = kRowSets<NI, NS, DK> * kRowsBytes<NI, NS> > 4 * Exchange<NS, kPairs>::kBytes
+                                    ? kRowSets<NI, NS, DK> * kRowsBytes<NI, NS>
                                     : 4 * Exchange<NS, kPairs>::kBytes;
 template <int NI, int NS, int DK>
-constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS>;
+constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS, DK>;
 
 // A block of one head.  A wave owns 16 features of keys and queries and dk/2 of the tokens, so that each row of the two
 // states is read by one wave only (or two); the 64 x 64 products of tokens with tokens are divided among the waves by
@@ -428,10 +435,12 @@ __global__ __launch_bounds__(512) void delta_gradients(
 
     const Tile<NI, DK> kt(smem), qt(smem + Tile<NI, DK>::kBytes);
     char* more = smem + 2 * Tile<NI, DK>::kBytes;
-    const Tile<NI, kColumns> ot(more);
-    const Tile<NS, kColumns> ut(more + Tile<NI, kColumns>::kBytes);
-    const Tile<NS, kColumns> rt(more + Tile<NI, kColumns>::kBytes + Tile<NS, kColumns>::kBytes);
-    // the products of tokens take the place of the three tiles once those are done with
+    constexpr int kSets = kRowSets<NI, NS, DK>;
+    const auto set_of = [&](int group) { return more + (kSets > 1 ? (group & 1) * kRowsBytes<NI, NS> : 0); };
+    const auto ot_of = [&](int group) { return Tile<NI, kColumns>(set_of(group)); };
+    const auto ut_of = [&](int group) { return Tile<NS, kColumns>(set_of(group) + Tile<NI, kColumns>::kBytes); };
+    const auto rt_of = [&](int group) { return Tile<NS, kColumns>(set_of(group) + Tile<NI, kColumns>::kBytes + Tile<NS, kColumns>::kBytes); };
+    // the products of tokens take the place of the rows once those are done with
     Exchange<NS, kPairs> f_rows(more), l_rows(more + Exchange<NS, kPairs>::kBytes), f_cols(more + 2 * Exchange<NS, kPairs>::kBytes),
         l_cols(more + 3 * Exchange<NS, kPairs>::kBytes);
 
@@ -475,10 +484,10 @@ __global__ __launch_bounds__(512) void delta_gradients(
             }
         }
     };
-    const auto stage_rows = [&]() __attribute__((always_inline)) {
-        ot.template put8<E>(tid >> 3, (tid & 7) * 8, o_raw);
-        ut.template put8<ElemF32>(tid >> 3, (tid & 7) * 8, u_raw);
-        rt.template put8<ElemF32>(tid >> 3, (tid & 7) * 8, r_raw);
+    const auto stage_rows = [&](int group) __attribute__((always_inline)) {
+        ot_of(group).template put8<E>(tid >> 3, (tid & 7) * 8, o_raw);
+        ut_of(group).template put8<ElemF32>(tid >> 3, (tid & 7) * 8, u_raw);
+        rt_of(group).template put8<ElemF32>(tid >> 3, (tid & 7) * 8, r_raw);
     };
 
     {
@@ -509,8 +518,8 @@ __global__ __launch_bounds__(512) void delta_gradients(
     for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
 #pragma unroll 1
     for (int group = 0; group < groups; ++group) {
-        if (group > 0) lds_barrier();
-        stage_rows();
+        if (kSets == 1 && group > 0) lds_barrier();  // (of two sets the last readers are behind the other's barrier)
+        stage_rows(group);
 #pragma unroll
         for (int i = 0; i < 8; ++i) value_dot += r_raw.v[i] * E::get(v_raw.v[i]);
         Operand<NS> so[2], dd[2];
@@ -524,17 +533,17 @@ __global__ __launch_bounds__(512) void delta_gradients(
                 for (int e = 0; e < 4; ++e) whole_term += s_raw[i][h][e] * d_raw[i][h][e];
         }
         lds_barrier();
-        // (behind the last group the one before it, which the products of tokens take next)
-        load_rows(group + 1 < groups ? group + 1 : (groups > 1 ? groups - 2 : 0));
+        // (behind the last group the one that the products of tokens load first, or one that is not there)
+        load_rows(group + 1 < groups ? group + 1 : (groups > kSets ? groups - 1 - kSets : groups));
         if (group + 1 < groups) load_states(group + 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int t = 0; t < kTok; ++t) {
                 const int row = 16 * (tile0 + t) + c;
-                x[t] = mma<NI, NS>(ot.along(row, 32 * i, g), so[i], x[t]);
-                a[t] = mma<NS, NS>(rt.along(row, 32 * i, g), so[i], a[t]);
-                b[t] = mma<NS, NS>(ut.along(row, 32 * i, g), dd[i], b[t]);
+                x[t] = mma<NI, NS>(ot_of(group).along(row, 32 * i, g), so[i], x[t]);
+                a[t] = mma<NS, NS>(rt_of(group).along(row, 32 * i, g), so[i], a[t]);
+                b[t] = mma<NS, NS>(ut_of(group).along(row, 32 * i, g), dd[i], b[t]);
             }
     }
     // Tokens against tokens, from the last group of columns back: tile `own` against all in dO U^T (waves 0 to 3) or
@@ -547,12 +556,14 @@ __global__ __launch_bounds__(512) void delta_gradients(
     for (int t = 0; t < kTiles; ++t) early[t] = late[t] = fx4{0, 0, 0, 0};
 #pragma unroll 1
     for (int group = groups - 1; group >= 0; --group) {
-        if (group < groups - 1) {
+        if (group < groups - kSets) {
             lds_barrier();
-            stage_rows();
+            stage_rows(group);
             lds_barrier();
-            load_rows(group > 0 ? group - 1 : 0);
+            load_rows(group > 0 ? group - 1 : groups);
         }
+        const Tile<NI, kColumns> ot = ot_of(group);
+        const Tile<NS, kColumns> ut = ut_of(group), rt = rt_of(group);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const Operand<NS> u = ut.along(16 * own + c, 32 * i, g);
@@ -577,6 +588,24 @@ __global__ __launch_bounds__(512) void delta_gradients(
                     }
                 }
             }
+        }
+    }
+
+    // No load of this block is left to come.  What the workgroup that follows on this die wants first is asked for
+    // meanwhile: its states' first 64 columns, and keys and queries, which it finds in the second cache then.
+    int touched[2] = {0, 0};
+    {
+        const int64_t follow = (int64_t)blockIdx.y * gridDim.x + blockIdx.x + kAhead;
+        const int64_t its_head = follow / gridDim.x, its_block = follow % gridDim.x;
+        if (its_head < s.heads) {
+            const int64_t its = its_block * s.heads + its_head;
+            const char* from = reinterpret_cast<const char*>((tid < 256 ? states : d_states) + its * cells);
+            const int row = (tid & 255) >> 1, at = (tid & 1) * 128;
+            if (row < s.dk && at < s.dv * 4) touched[0] = *reinterpret_cast<const int*>(from + (int64_t)row * s.dv * 4 + at);
+            constexpr int kLines = kBlock * DK * kSize / 128;
+            const int64_t copy = (its_block * s.key_heads + its_head / share) * kBlock * DK;
+            if (tid < 2 * kLines)
+                touched[1] = *reinterpret_cast<const int*>(reinterpret_cast<const char*>((tid < kLines ? k : q) + copy) + tid % kLines * 128);
         }
     }
 
@@ -678,6 +707,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
             }
         }
     }
+    asm volatile("" ::"v"(touched[0]), "v"(touched[1]));  // (keeps the two loads in the program)
     whole_term = tile0 == 0 ? whole_term * gate[kSince * kBlock + kBlock - 1] : 0.0f;  // a cell counts once
     whole_term = sum16(whole_term + carried);
     whole_term += __shfl_xor(whole_term, 16);
