@@ -512,7 +512,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
         if (tid < kGateFloats) gate[tid] = gate_raw;
     }
 
-    fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B: own tokens, own features
+    fx4 x[kTok], a[kTok], b[kTok];  // dQ, A and B: own features (rows), own tokens (columns)
     float value_dot = 0.0f, whole_term = 0.0f;
 #pragma unroll
     for (int t = 0; t < kTok; ++t) x[t] = a[t] = b[t] = fx4{0, 0, 0, 0};
@@ -541,9 +541,9 @@ __global__ __launch_bounds__(512) void delta_gradients(
 #pragma unroll
             for (int t = 0; t < kTok; ++t) {
                 const int row = 16 * (tile0 + t) + c;
-                x[t] = mma<NI, NS>(ot_of(group).along(row, 32 * i, g), so[i], x[t]);
-                a[t] = mma<NS, NS>(rt_of(group).along(row, 32 * i, g), so[i], a[t]);
-                b[t] = mma<NS, NS>(ut_of(group).along(row, 32 * i, g), dd[i], b[t]);
+                x[t] = mma<NS, NI>(so[i], ot_of(group).along(row, 32 * i, g), x[t]);
+                a[t] = mma<NS, NS>(so[i], rt_of(group).along(row, 32 * i, g), a[t]);
+                b[t] = mma<NS, NS>(dd[i], ut_of(group).along(row, 32 * i, g), b[t]);
             }
     }
     // Tokens against tokens, from the last group of columns back: tile `own` against all in dO U^T (waves 0 to 3) or
@@ -654,57 +654,56 @@ __global__ __launch_bounds__(512) void delta_gradients(
         ko[p] = kt.down(32 * p, feature0, lane);
         qo[p] = qt.down(32 * p, feature0, lane);
     }
-    const uint32_t to0 = feature0 + c < s.dk ? (16 * tile0 + 4 * g) * k_step + (feature0 + c) * kSize : kOutside;
+    const uint32_t to0 = feature0 + 4 * g < s.dk ? (16 * tile0 + c) * k_step + (feature0 + 4 * g) * kSize : kOutside;
     const Buffer qb = rows_of(d_q, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
     const Buffer kb = rows_of(d_k, k_step, (int64_t)key_head * s.dk * kSize, s.dk * kSize);
     float* const mine = sums + ((entry * 16 + wave) * kTok * 64 + lane) * 4;  // dK's half is 8 waves on
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
-        const int tile = tile0 + t;
+        const int tile = tile0 + t, token = 16 * tile + c;
         // factors of the parts that went through the state
-        const fx4 since = *reinterpret_cast<const fx4*>(gate + kSince * kBlock + 16 * tile + 4 * g);
-        const fx4 until = *reinterpret_cast<const fx4*>(gate + kUntil * kBlock + 16 * tile + 4 * g);
-        const fx4 beta = *reinterpret_cast<const fx4*>(gate + kBeta * kBlock + 16 * tile + 4 * g);
-        const fx4 kv = kt.tile(16 * tile, feature0, lane), qv = qt.tile(16 * tile, feature0, lane);
+        const float since = gate[kSince * kBlock + token], until = gate[kUntil * kBlock + token], beta = gate[kBeta * kBlock + token];
+        const fx4 kv = kt.quad(token, feature0 + 4 * g), qv = qt.quad(token, feature0 + 4 * g);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            x[t][r] *= s.scale * since[r];
-            a[t][r] *= -since[r];
-            b[t][r] *= until[r];
+            x[t][r] *= s.scale * since;
+            a[t][r] *= -since;
+            b[t][r] *= until;
             carried += kv[r] * b[t][r];
         }
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             if (p <= (tile >> 1)) {
-                x[t] = mma<NS, NI>(f_rows.get(pair_lower(tile, p), lane), ko[p], x[t]);
-                a[t] = mma<NS, NI>(l_rows.get(pair_lower(tile, p), lane), ko[p], a[t]);
+                x[t] = mma<NI, NS>(ko[p], f_rows.get(pair_lower(tile, p), lane), x[t]);
+                a[t] = mma<NI, NS>(ko[p], l_rows.get(pair_lower(tile, p), lane), a[t]);
             }
             if (p >= (tile >> 1)) {
-                b[t] = mma<NS, NI>(f_cols.get(pair_upper(tile, p), lane), qo[p], b[t]);
-                b[t] = mma<NS, NI>(l_cols.get(pair_upper(tile, p), lane), ko[p], b[t]);
+                b[t] = mma<NI, NS>(qo[p], f_cols.get(pair_upper(tile, p), lane), b[t]);
+                b[t] = mma<NI, NS>(ko[p], l_cols.get(pair_upper(tile, p), lane), b[t]);
             }
         }
-        fx4 dc, da;  // of the own features: q.dQ + beta k.A - k.B and k.A
+        float dc = 0.0f, da = 0.0f;  // of the own features: q.dQ + beta k.A - k.B and k.A
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float ka = kv[r] * a[t][r];
-            dc[r] = sum16(qv[r] * x[t][r] + (beta[r] * ka - kv[r] * b[t][r]));
-            da[r] = sum16(ka);
-            b[t][r] += beta[r] * a[t][r];  // dK
+            dc += qv[r] * x[t][r] + (beta * ka - kv[r] * b[t][r]);
+            da += ka;
+            b[t][r] += beta * a[t][r];  // dK
         }
-        if (c == 0) {
-            *reinterpret_cast<fx4*>(&dots[wave][0][16 * t + 4 * g]) = dc;
-            *reinterpret_cast<fx4*>(&dots[wave][1][16 * t + 4 * g]) = da;
+        dc += __shfl_xor(dc, 16);
+        dc += __shfl_xor(dc, 32);
+        da += __shfl_xor(da, 16);
+        da += __shfl_xor(da, 32);
+        if (g == 0) {
+            dots[wave][0][16 * t + c] = dc;
+            dots[wave][1][16 * t + c] = da;
         }
         if constexpr (SHARED) {
             *reinterpret_cast<fx4*>(mine + t * 256) = x[t];
             *reinterpret_cast<fx4*>(mine + (8 * kTok + t) * 256) = b[t];
         } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                put1<E>(qb, to0 + (16 * t + r) * k_step, x[t][r]);
-                put1<E>(kb, to0 + (16 * t + r) * k_step, b[t][r]);
-            }
+            put4<E>(qb, to0 + 16 * t * k_step, x[t]);
+            put4<E>(kb, to0 + 16 * t * k_step, b[t]);
         }
     }
     asm volatile("" ::"v"(touched[0]), "v"(touched[1]));  // (keeps the two loads in the program)
@@ -759,7 +758,7 @@ __global__ __launch_bounds__(512) void delta_fold(DeltaShape s, const float* __r
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
     const BlockAt found = block_at(s, block);
     if (found.length <= 0) return;
-    const int feature = 16 * (wave & (kFeatures - 1)) + c, tile0 = kFeatures == 8 ? 0 : (wave >> 2) * kTok;
+    const int feature = 16 * (wave & (kFeatures - 1)) + 4 * g, tile0 = kFeatures == 8 ? 0 : (wave >> 2) * kTok;
     const float* from = sums + (((block * s.heads + key_head * share) * 16 + wave) * kTok * 64 + lane) * 4;
     fx4 x[kTok], b[kTok];
 #pragma unroll
@@ -772,16 +771,14 @@ __global__ __launch_bounds__(512) void delta_fold(DeltaShape s, const float* __r
         }
     }
 #pragma unroll
-    for (int t = 0; t < kTok; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * (tile0 + t) + 4 * g + r;
-            if (row < found.length && feature < s.dk) {
-                const int64_t to = ((found.row + row) * s.key_heads + key_head) * s.dk + feature;
-                d_q[to] = E::put(x[t][r]);
-                d_k[to] = E::put(b[t][r]);
-            }
+    for (int t = 0; t < kTok; ++t) {
+        const int row = 16 * (tile0 + t) + c;
+        if (row < found.length && feature < s.dk) {
+            const int64_t to = ((found.row + row) * s.key_heads + key_head) * s.dk + feature;
+            store4<E>(d_q + to, x[t]);
+            store4<E>(d_k + to, b[t]);
         }
+    }
 }
 
 }  // namespace

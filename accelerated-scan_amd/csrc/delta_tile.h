@@ -207,7 +207,7 @@ __device__ __forceinline__ Eight<E> fetch8(Buffer b, uint32_t at) {
     }
     return r;
 }
-// Four neighbouring values, and one, to byte `at`.
+// Four neighbouring values to byte `at`.
 template <class E>
 __device__ __forceinline__ void put4(Buffer b, uint32_t at, const fx4& x) {
     typename E::S s[4];
@@ -221,15 +221,6 @@ __device__ __forceinline__ void put4(Buffer b, uint32_t at, const fx4& x) {
         ux2 v;
         __builtin_memcpy(&v, s, 8);
         __builtin_amdgcn_raw_buffer_store_b64(v, b, at, 0, 0);
-    }
-}
-template <class E>
-__device__ __forceinline__ void put1(Buffer b, uint32_t at, float x) {
-    const typename E::S s = E::put(x);
-    if constexpr (E::kWide) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, s), b, at, 0, 0);
-    } else {
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, s), b, at, 0, 0);
     }
 }
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -363,10 +354,19 @@ struct Tile {
     }
     // The 16 x 16 tile at (row0, col0) in the accumulator's layout.
     __device__ __forceinline__ fx4 tile(int row0, int col0, int lane) const {
+        return summed([&](int i) { return __builtin_bit_cast(uint64_t, column4(i, row0, col0, lane)); });
+    }
+    // Columns col .. col+3 (col a multiple of 4) of row `row`.
+    __device__ __forceinline__ fx4 quad(int row, int col) const {
+        return summed([&](int i) { return *reinterpret_cast<const uint64_t*>(base + i * kPlane + place(row, col)); });
+    }
+    // Four values of which part i is four bfloat16 values in a word.
+    template <class F>
+    static __device__ __forceinline__ fx4 summed(F word) {
         fx4 x;
 #pragma unroll
         for (int i = P - 1; i >= 0; --i) {
-            const uint64_t w = __builtin_bit_cast(uint64_t, column4(i, row0, col0, lane));
+            const uint64_t w = word(i);
             const uint32_t a = (uint32_t)w, b = (uint32_t)(w >> 32);
             const fx4 part = {__builtin_bit_cast(float, a << 16), __builtin_bit_cast(float, a & 0xffff0000u),
                               __builtin_bit_cast(float, b << 16), __builtin_bit_cast(float, b & 0xffff0000u)};
@@ -397,6 +397,7 @@ struct Tile<0, W> {
         *reinterpret_cast<fx4*>(at) = a;
         *reinterpret_cast<fx4*>(at + 4) = b;
     }
+    __device__ __forceinline__ fx4 quad(int row, int col) const { return *reinterpret_cast<const fx4*>(base + row * kStride + col); }
     __device__ __forceinline__ Operand<0> along(int row, int k0, int g) const {
         const float* at = base + row * kStride + k0 + 8 * g;
         Operand<0> o;
