@@ -277,9 +277,12 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         }
     } else if (seq_length > 0) {
         // Keys, queries, dO, T and gates to LDS.
-        Eight<E> k_raw[2][kCopies], q_raw[2][kCopies], o_raw[2];
-        fx4 t_raw[2][kPieces<NS>];
-        float gate_raw[2];
+        // (in registers for two blocks, or for one where two do not fit: with 114 registers in memory fp32 (2, 2048, 8 heads
+        // of 128 x 128) took 192 us, with one block 132)
+        constexpr int kSets = sizeof(Eight<E>) * kCopies > 64 ? 1 : 2;
+        Eight<E> k_raw[kSets][kCopies], q_raw[kSets][kCopies], o_raw[kSets];
+        fx4 t_raw[kSets][kPieces<NS>];
+        float gate_raw[kSets];
         const int64_t copy0 = ((seq_block + last) * s.key_heads + key_head) * kBlock * DK;
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *q_p = reinterpret_cast<const char*>(q + copy0);
         const char* o_p = start_of(d_out, v_step, (int64_t)head * s.dv * kSize);
@@ -336,20 +339,21 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             }
         };
         load_block(last, 0);
-        load_block(last - 1, 1);
+        if constexpr (kSets == 2) load_block(last - 1, 1);
         stage_block(last, 0);
         stage_queries(0);
-        load_block(last - 2, 0);
+        load_block(last - kSets, 0);
         touch_block(last - 3);
         touch_block(last - 4);
         lds_barrier();
-        const auto block = [&](int64_t now, int other) __attribute__((always_inline)) {
+        const auto block = [&](int64_t now, int next) __attribute__((always_inline)) {
+            const int other = next & (kSets - 1);
             lds_barrier();
             lds_barrier();
             stage_block(now - 1, other);  // the readers of all but the queries are behind the second barrier
             lds_barrier();
             stage_queries(other);
-            load_block(now - 3, other);
+            load_block(now - 1 - kSets, other);
             touch_block(now - 5);
         };
         for (int64_t now = last; now >= 0; now -= 2) {
