@@ -386,9 +386,13 @@ constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS
 
 // A block of one head.  A wave owns 16 features of keys and queries and dk/2 of the tokens, so that each row of the two
 // states is read by one wave only (or two); the 64 x 64 products of tokens with tokens are divided among the waves by
-// tiles and go round through LDS.  A workgroup reads 230 KiB and computes for 3 us; with one resident to a compute unit
-// the two alternate, and a loop over heads or blocks around this body would only lift its address arithmetic in front,
-// where it does not fit the registers (bf16 (2, 4096, 16 heads of 128 x 128): 428 us with one, 218 us without).
+// tiles and go round through LDS.  The products have features as rows, so that a lane holds four of a token's and writes
+// 8 bytes (with tokens as rows 211 us instead of 194, below).
+//
+// What bounds it: a workgroup reads 256 KiB and has a compute unit to itself, for its registers.  bf16 (2, 4096, 16 heads
+// of 128 x 128) takes 194 us; 134 are left when nothing is read, most of them LDS and its latencies, so that loads and
+// products overlap in part only.  A loop over heads or blocks around this body, to load ahead, lifts its address
+// arithmetic in front, where it does not fit the registers (428 us for 218 at the time).
 //
 // SHARED: dQ and dK go to `sums` in fp32, to be added over the heads that share the keys (delta_fold).
 // q and k: the copies that delta_prepare made.  grid (blocks, heads), 512 threads.

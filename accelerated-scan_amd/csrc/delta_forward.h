@@ -6,8 +6,14 @@
 // dk/4 w .. in its accumulators and computes tokens 16w .. 16w+15 of every block.  State, R and U go round through LDS
 // in the order in which the next product reads them, with one barrier each.  What the chain does not wait for
 // is done by waves of their own beside these on the same SIMDs: four compute the outputs, four bring keys, values, T
-// and gates to LDS blocks ahead.  (The loads are 66 KiB a block, which the 64 bytes per clock of a compute unit's
-// cache turn into 1100 clocks of issue: a wave that loads is late for its barrier if it has anything else to do.)
+// and gates to LDS blocks ahead.  (The loads are 60 KiB a block, which the 64 bytes per clock of a compute unit's
+// cache turn into 960 clocks of issue: a wave that loads is late for its barrier if it has anything else to do.)
+//
+// What bounds it: bf16 (1, 16384, 32 heads of 128 x 128) takes 345 to 390 us, 256 blocks of 1.3 to 1.5 us, one chain to
+// a compute unit.  200 KiB a block go through LDS, 1600 clocks at 128 bytes each, beside three round trips (write,
+// barrier, read, product) of 300 to 400 clocks that nothing overlaps but the other waves' work.  More columns to a workgroup
+// would read less per column and leave compute units without one.  The chain that also writes states and U moves 0.5 GB
+// in 135 us (2, 4096, 16 heads).
 #ifndef ASCAN_DELTA_FORWARD_H_
 #define ASCAN_DELTA_FORWARD_H_
 
@@ -30,15 +36,15 @@ __device__ __forceinline__ ChainAt chain_at(const DeltaShape& s) {
 }
 inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads + 7) / 8 * 8 * ((s.dv + 15) / 16); }
 
-// Whether a chain kernel asks for its blocks ahead (touch below).  It gains where a compute unit runs one long chain
-// of large blocks: bf16 (1, 16384, 32 heads of 128 x 128) 379 -> 341 us; and loses where workgroups follow each other, whose
-// starts it delays (fp16, 16 packed sequences, 2048 workgroups: 226 -> 239 us), where blocks are small (key size 64:
-// 51 -> 57 us) and where fp32 products take longer than the loads (69 -> 72 us).
+// Whether a chain kernel asks for its blocks ahead (touch below).  It gains where a compute unit runs one chain of large
+// blocks: bf16 (2, 4096, 16 heads of 128 x 128) forward 155 -> 135 us, backward 201 -> 167, (1, 16384, 32 heads)
+// 394 -> 387; and gives nothing where workgroups follow each other (fp16, 16 packed sequences, 2048 workgroups: 243 us without,
+// 245 with), where blocks are small (key size 64: 58 and 58.5) and where fp32 products take longer than the loads (74 and 74).
 template <int NC, int DK>
 inline bool chain_touches(const DeltaShape& s) { return NC > 0 && DK == 128 && chain_grid(s) <= 512; }
 
 // A chain's workgroup may have as many lines of 128 bytes on their way as its compute unit's cache holds, 256.  At the
-// latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 66 (and nobody else uses the
+// latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 60 (and nobody else uses the
 // bandwidth); at that of the die's second cache it is three times as much.  So every line is asked for blocks ahead by
 // one of the workgroups that will read it: line `id` of up to five pieces of memory, one after the other.
 struct Lines {

@@ -7,7 +7,8 @@
 //   dx = (e - h mean(e h)) / r,   dz = dy w h s (1 + z (1 - s)),   dw = sum over rows of dy h silu(z)
 //
 // A pass over memory: a row's values stay in the registers of the lanes that share it while their sums go
-// round.  Sums and all arithmetic are fp32.
+// round.  Sums and all arithmetic are fp32.  Memory bounds it: bf16, 524288 rows of 128, forward 403 MB in 77.5 us
+// (5.2 TB/s, what a large copy reaches), backward 671 MB in 126 us (5.3 TB/s) and 6 us for the sums over its workgroups.
 #ifndef ASCAN_NORM_KERNEL_H_
 #define ASCAN_NORM_KERNEL_H_
 
