@@ -120,7 +120,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
 // P leaves from the accumulators: the tile K_j Q_i^T has token i in a lane's column and its rows j along the depth, as
 // the operand wants it (Q_i K_j^T for the transpose).  The inverse of I + L is made by substitution inside the
 // diagonal's 16 x 16 tiles, which is exact to rounding whatever the keys are (a series in L is not: its
-// grow), and joined from there to 32 and to 64 with fp32 products.
+// terms grow), and joined from there to 32 and to 64 with fp32 products.
 //
 // The block's keys and queries are copied to where they stand without gaps, missing rows and features as zeros: in the
 // tensors the rows of a head are a power of two apart as a rule, so that one channel of the cache holds them all, and the

@@ -12,7 +12,7 @@ int norm_status(hipError_t e) {
     return ASCAN_ERR_LAUNCH;
 }
 
-// Workgroups of the backward kernel: four to a compute unit, so that one's loads cover another's sums.
+// Workgroups of the backward kernel: eight to a compute unit, so that one's loads cover another's sums.
 constexpr int64_t kNormParts = 2048;
 
 template <int L>

@@ -399,6 +399,7 @@ ASCAN_API int ascan_backward_gated_values(const void* gate_inputs, const void* v
  * head h / (heads / key_heads).  dk is a multiple of 8 up to 128, dv a multiple of 8 up to 4096.  dtype is
  * ASCAN_F32, ASCAN_BF16 or ASCAN_F16 and holds for q, k, v, out and their gradients; log_gates, beta and their
  * gradients have it too, or are fp32 with ASCAN_DELTA_GATES_F32.  All buffers start on 16 bytes, except the gates.
+ * A call has up to 65535 sequences, and heads * dv and key_heads * dk are up to 2^22.
  *
  *   - `sequences` sequences of rows / sequences tokens each where `offsets` is NULL; else packed ones, sequence n
  *     being rows offsets[n] .. offsets[n+1]-1 (device memory, sequences + 1 ascending numbers; int32, or int64 with
