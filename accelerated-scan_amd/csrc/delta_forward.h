@@ -10,7 +10,7 @@
 // cache turn into 960 clocks of issue: a wave that loads is late for its barrier if it has anything else to do.)
 //
 // What bounds it: bf16 (1, 16384, 32 heads of 128 x 128) takes 345 to 390 us, 256 blocks of 1.3 to 1.5 us, one chain to
-// a compute unit.  200 KiB a block go through LDS, 1600 clocks at 128 bytes each, beside three round trips (write,
+// a compute unit.  LDS is at work half of the time (200 KiB a block, 1600 clocks), the matrix units a fifth, beside three round trips (write,
 // barrier, read, product) of 300 to 400 clocks that nothing overlaps but the other waves' work.  More columns to a workgroup
 // would read less per column and leave compute units without one.  The chain that also writes states and U moves 0.5 GB
 // in 135 us (2, 4096, 16 heads).
