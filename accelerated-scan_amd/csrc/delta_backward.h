@@ -390,7 +390,7 @@ constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS
 // 8 bytes (with tokens as rows 211 us instead of 194, below).
 //
 // What bounds it: a workgroup reads 256 KiB and has a compute unit to itself, for its registers.  bf16 (2, 4096, 16 heads
-// of 128 x 128) takes 194 us for 0.7 GB, 3.6 TB/s; 134 us are left when nothing is read, a quarter of them LDS at work and
+// of 128 x 128) takes 194 us for 0.7 GB, 3.6 TB/s; 134 us are left when nothing is read, a third of them LDS at work and
 // the rest latencies, so that loads and products overlap in part only.  A loop over heads or blocks around this body, to load ahead, lifts its address
 // arithmetic in front, where it does not fit the registers (428 us for 218 at the time).
 //
