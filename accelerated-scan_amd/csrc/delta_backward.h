@@ -8,8 +8,13 @@
 //   B  = diag(e^(c[63]-c)) U D1^T + (F . dO U^T)^T Q - (diag(beta) G . dR U^T)^T K
 //   dK = diag(beta) A + B
 //   dbeta[i] = dR[i].v[i] + k[i].A[i]
-//   dc[i] = q[i].dQ[i] + beta[i] k[i].A[i] - k[i].B[i],  and c[63] also gets e^c[63] S0.D1 + sum over i of
-//           k[i].(diag(e^(c[63]-c)) U D1^T)[i];  the gradient of a log gate sums dc from its token on
+//   The log gate of token t lies on the way from S0 to t and later tokens, from earlier tokens to the state behind the block,
+//   from earlier tokens to t and later ones, and from S0 to the state behind the block:
+//     sum over i >= t of (q.dQ + beta k.A)[i], their parts from S0,   sum over j < t of k[j].(diag(e^(c[63]-c)) U D1^T)[j],
+//     sum over pairs j < t <= i,   e^c[63] S0.D1
+//   Of the pairs only the sums over earlier and over later partners of a token are known: the sum over j < t <= i is the
+//   difference of the two summed from t on, or up to t.  Taken from the nearer end, and without the pairs of a token
+//   with itself, it has the fewest terms that cancel (none for the first and the last token).
 #ifndef ASCAN_DELTA_BACKWARD_H_
 #define ASCAN_DELTA_BACKWARD_H_
 
@@ -19,6 +24,8 @@ namespace ascan {
 namespace {
 
 constexpr int kAhead = 256;   // workgroups from one to that which takes its place: one to a compute unit
+// Sums over the features of a token: its partners S0, the state behind the block, earlier and later tokens; k.A.
+enum { kFromState, kToState, kEarlier, kLater, kBetas, kSums };
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
 template <int NI, int NS, int NC, int DK>
@@ -371,12 +378,14 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     }
 }
 
+constexpr int kGradientStatic = 13 * 1024;  // what delta_gradients has in LDS beside the arrays below, at most
+
 // dO, U and dR of kColumns columns in LDS.  The second pass over the columns goes back: with room for two such sets it finds
 // the last two where the first pass has left them.
 template <int NI, int NS>
 constexpr int kRowsBytes = Tile<NI, kColumns>::kBytes + 2 * Tile<NS, kColumns>::kBytes;
 template <int NI, int NS, int DK>
-constexpr int kRowSets = 2 * Tile<NI, DK>::kBytes + 2 * kRowsBytes<NI, NS> + 8 * 1024 <= 160 * 1024 ? 2 : 1;
+constexpr int kRowSets = 2 * Tile<NI, DK>::kBytes + 2 * kRowsBytes<NI, NS> + kGradientStatic <= 160 * 1024 ? 2 : 1;
 template <int NI, int NS, int DK>
 constexpr int kGradientShared = kRowSets<NI, NS, DK> * kRowsBytes<NI, NS> > 4 * Exchange<NS, kPairs>::kBytes
                                     ? kRowSets<NI, NS, DK> * kRowsBytes<NI, NS>
@@ -407,8 +416,8 @@ __global__ __launch_bounds__(512) void delta_gradients(
     constexpr int kFeatures = DK / 16, kTok = DK / 32;  // tiles of features, and of tokens that a wave owns
     extern __shared__ __align__(16) char smem[];
     __shared__ __align__(16) float gate[kGateFloats];
-    __shared__ __align__(16) float dots[8][2][16 * kTok];
-    __shared__ float value_dots[kBlock], whole_terms[8];
+    __shared__ float dots[8][kSums][16 * kTok];
+    __shared__ float value_dots[kBlock], diagonal[kBlock], whole_terms[8];
     const int64_t block = blockIdx.x;
     const int head = blockIdx.y, share = s.heads / s.key_heads, key_head = head / share;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, c = lane & 15;
@@ -635,7 +644,8 @@ __global__ __launch_bounds__(512) void delta_gradients(
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float w = factor * exp_of((high - h[r]) + (low - l[r]));
-                        e[r] = there0 + r < here + (second ? 0 : 1) ? w * early[t][r] : 0.0f;
+                        e[r] = there0 + r < here ? w * early[t][r] : 0.0f;
+                        if (!second && there0 + r == here) diagonal[here] = w * early[t][r];
                     }
                 }
                 rows.put(2 * pair_lower(own, t >> 1) + (t & 1), lane, e);
@@ -647,7 +657,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float w = factor * (second ? beta[r] : 1.0f) * exp_of((h[r] - high) + (l[r] - low));
-                        e[r] = there0 + r > here - (second ? 0 : 1) ? w * late[t][r] : 0.0f;
+                        e[r] = there0 + r > here ? w * late[t][r] : 0.0f;
                     }
                 }
                 cols.put(2 * pair_upper(own, t >> 1) + (t & 1), lane, e);
@@ -655,7 +665,6 @@ __global__ __launch_bounds__(512) void delta_gradients(
         }
     }
     lds_barrier();
-    float carried = 0.0f;
     Operand<NI> ko[2], qo[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
@@ -672,39 +681,42 @@ __global__ __launch_bounds__(512) void delta_gradients(
         // factors of the parts that went through the state
         const float since = gate[kSince * kBlock + token], until = gate[kUntil * kBlock + token], beta = gate[kBeta * kBlock + token];
         const fx4 kv = kt.quad(token, feature0 + 4 * g), qv = qt.quad(token, feature0 + 4 * g);
+        float sums_of[kSums] = {0, 0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             x[t][r] *= s.scale * since;
             a[t][r] *= -since;
             b[t][r] *= until;
-            carried += kv[r] * b[t][r];
+            sums_of[kFromState] += qv[r] * x[t][r] + beta * (kv[r] * a[t][r]);
+            sums_of[kToState] += kv[r] * b[t][r];
         }
+        fx4 xi = {0, 0, 0, 0}, ai = {0, 0, 0, 0}, bi = {0, 0, 0, 0};
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             if (p <= (tile >> 1)) {
-                x[t] = mma<NI, NS>(ko[p], f_rows.get(pair_lower(tile, p), lane), x[t]);
-                a[t] = mma<NI, NS>(ko[p], l_rows.get(pair_lower(tile, p), lane), a[t]);
+                xi = mma<NI, NS>(ko[p], f_rows.get(pair_lower(tile, p), lane), xi);
+                ai = mma<NI, NS>(ko[p], l_rows.get(pair_lower(tile, p), lane), ai);
             }
             if (p >= (tile >> 1)) {
-                b[t] = mma<NI, NS>(qo[p], f_cols.get(pair_upper(tile, p), lane), b[t]);
-                b[t] = mma<NI, NS>(ko[p], l_cols.get(pair_upper(tile, p), lane), b[t]);
+                bi = mma<NI, NS>(qo[p], f_cols.get(pair_upper(tile, p), lane), bi);
+                bi = mma<NI, NS>(ko[p], l_cols.get(pair_upper(tile, p), lane), bi);
             }
         }
-        float dc = 0.0f, da = 0.0f;  // of the own features: q.dQ + beta k.A - k.B and k.A
+        const float with_itself = diagonal[token];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float ka = kv[r] * a[t][r];
-            dc += qv[r] * x[t][r] + (beta * ka - kv[r] * b[t][r]);
-            da += ka;
-            b[t][r] += beta * a[t][r];  // dK
+            sums_of[kEarlier] += qv[r] * xi[r] + beta * (kv[r] * ai[r]);
+            sums_of[kLater] += kv[r] * bi[r];
+            a[t][r] += ai[r];
+            sums_of[kBetas] += kv[r] * a[t][r];
+            x[t][r] += xi[r] + with_itself * kv[r];
+            b[t][r] += bi[r] + with_itself * qv[r] + beta * a[t][r];  // dK
         }
-        dc += __shfl_xor(dc, 16);
-        dc += __shfl_xor(dc, 32);
-        da += __shfl_xor(da, 16);
-        da += __shfl_xor(da, 32);
-        if (g == 0) {
-            dots[wave][0][16 * t + c] = dc;
-            dots[wave][1][16 * t + c] = da;
+#pragma unroll
+        for (int i = 0; i < kSums; ++i) {
+            sums_of[i] += __shfl_xor(sums_of[i], 16);
+            sums_of[i] += __shfl_xor(sums_of[i], 32);
+            if (g == 0) dots[wave][i][16 * t + c] = sums_of[i];
         }
         if constexpr (SHARED) {
             *reinterpret_cast<fx4*>(mine + t * 256) = x[t];
@@ -716,7 +728,7 @@ __global__ __launch_bounds__(512) void delta_gradients(
     }
     asm volatile("" ::"v"(touched[0]), "v"(touched[1]));  // (keeps the two loads in the program)
     whole_term = tile0 == 0 ? whole_term * gate[kSince * kBlock + kBlock - 1] : 0.0f;  // a cell counts once
-    whole_term = sum16(whole_term + carried);
+    whole_term = sum16(whole_term);
     whole_term += __shfl_xor(whole_term, 16);
     whole_term += __shfl_xor(whole_term, 32);
     if (lane == 0) whole_terms[wave] = whole_term;
@@ -726,22 +738,29 @@ __global__ __launch_bounds__(512) void delta_gradients(
     if ((tid & 7) == 0) value_dots[tid >> 3] = value_dot;
     lds_barrier();
     if (wave == 0) {
-        // token `lane`: over the tiles of features, then the sums from it on
-        float dc = 0.0f, da = 0.0f, whole = 0.0f;
+        // token `lane`: over the tiles of features, then over tokens
+        float sum[kSums] = {0, 0, 0, 0, 0}, whole = 0.0f;
 #pragma unroll
         for (int i = 0; i < kFeatures; ++i) {
             const int w = lane / (16 * kTok) * kFeatures + i;
-            dc += dots[w][0][lane % (16 * kTok)];
-            da += dots[w][1][lane % (16 * kTok)];
+#pragma unroll
+            for (int n = 0; n < kSums; ++n) sum[n] += dots[w][n][lane % (16 * kTok)];
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) whole += whole_terms[i];
+        const bool front = lane < (length + 1) / 2;
+        float from = sum[kFromState], to_state = sum[kToState], pairs = front ? sum[kLater] - sum[kEarlier] : sum[kEarlier] - sum[kLater];
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-            const float y = __shfl_down(dc, d);
-            if (lane + d < 64) dc += y;
+            const float x1 = __shfl_down(from, d), x2 = __shfl_up(to_state, d), x3 = __shfl(pairs, (front ? lane - d : lane + d) & 63);
+            if (lane + d < 64) from += x1;
+            if (lane >= d) to_state += x2;
+            if (front ? lane >= d : lane + d < 64) pairs += x3;
         }
-        dc += whole;
+        to_state = __shfl_up(to_state, 1);
+        const float before = __shfl_up(pairs, 1);
+        if (front) pairs = lane > 0 ? before : 0.0f;
+        const float dc = from + pairs + whole + (lane > 0 ? to_state : 0.0f), da = sum[kBetas];
         if (lane < length) {
             const int64_t to = (row0 + lane) * s.heads + head;
             if (s.wide_gates) {

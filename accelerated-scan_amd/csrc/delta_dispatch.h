@@ -77,7 +77,7 @@ int delta_forward_dk(const DeltaForward& f) {
 
 template <class E, int NI, int NS, int NC, int DK>
 int delta_backward_dk(const DeltaBackward& f) {
-    static_assert(kReverseBytes<NI, NS, NC, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + 8 * 1024 <= kLdsBytes, "fits a compute unit");
+    static_assert(kReverseBytes<NI, NS, NC, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + kGradientStatic <= kLdsBytes, "fits a compute unit");
     using S = typename E::S;
     const DeltaShape& s = f.shape;
     const DeltaParts<NS, NC> at(s, true, sizeof(S));

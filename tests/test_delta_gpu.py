@@ -669,3 +669,22 @@ def test_captured_training_step():
         gradients()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), turn
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("tokens", [1, 2, 3, 70])
+def test_gate_gradients_without_a_state(tokens, dtype):
+    """A first token's gate scales nothing, and closed gates leave little: no rest of terms that cancel."""
+    from accelerated_scan import delta
+
+    data = ref.inputs(2, tokens, 1, 2, 64, 48, dtype, seed=50 + tokens, gates=torch.float32, decay=30.0 if tokens < 70 else 6.0)[:5]
+    exact = as_exact(data, grad=True)
+    out, final = ref.delta_scan(*exact)
+    gen = torch.Generator().manual_seed(51)
+    d_out, d_final = torch.randn(out.shape, generator=gen).to(dtype), torch.randn(final.shape, generator=gen)
+    want = torch.autograd.grad([out, final], exact, [d_out.double(), d_final.double()])
+    leaves = on_gpu(data, grad=True)
+    got = torch.autograd.grad(delta.gated_delta_scan(*leaves), leaves, on_gpu([d_out, d_final]))
+    assert not got[3][:, 0].any()
+    for name, a, b in zip(NAMES, got, want):
+        ref.close(a, b, dtype, backward=True, what=name)
