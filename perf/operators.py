@@ -19,11 +19,6 @@ import torch
 
 own = False
 
-# this repository's package lies in a folder of its own beside this one
-_PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "accelerated-scan_amd")
-if _PACKAGE not in sys.path:
-    sys.path.insert(0, _PACKAGE)
-
 DTYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 BLOCK = 64     # tokens the plain form takes at a time
 EPS = 1e-6
@@ -236,20 +231,28 @@ def _longest(case):
     return max(int(n) for n in case["lengths"].split(",")) if case["lengths"] else case["tokens"]
 
 
+def _package():
+    """This repository's package, which lies in a folder of its own beside this one."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "accelerated-scan_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from accelerated_scan import delta, norm
+
+    return delta, norm
+
+
 def run(state):
     case = state["case"]
     dtype = DTYPES[case["dtype"]]
     if case["kind"] == "norm":
         if own:
-            from accelerated_scan import norm
-
+            _, norm = _package()
             return norm.gated_norm(state["x"], state["gate"], state["weight"], eps=EPS)
         return _plain_norm(state["x"], state["gate"], state["weight"]).to(dtype)
     if case["kind"] == "norm_train":
         leaves = [state[name].detach().requires_grad_() for name in ("x", "gate", "weight")]
         if own:
-            from accelerated_scan import norm
-
+            _, norm = _package()
             out = norm.gated_norm(*leaves, eps=EPS)
         else:
             out = _plain_norm(*leaves).to(dtype)
@@ -259,8 +262,7 @@ def run(state):
     if case["kind"] == "step":
         inputs = [state[name] for name in ("q", "k", "v", "log_gates", "beta")]
         if own:
-            from accelerated_scan import delta
-
+            delta, _ = _package()
             out = delta.gated_delta_step(*inputs, state["states"], slots=state["slots"], scale=scale)
             return {"out": out, "states": state["states"]}
         shared = case["heads"] // case["key_heads"]
@@ -278,8 +280,7 @@ def run(state):
     leaves = [state[name].detach().requires_grad_(train) for name in names]
     initial = leaves[5] if len(leaves) > 5 else None
     if own:
-        from accelerated_scan import delta
-
+        delta, _ = _package()
         out, final = delta.gated_delta_scan(*leaves[:5], initial=initial, scale=scale, offsets=state["offsets"])
     else:
         out, final = _plain_sequences(*leaves[:5], initial, scale, state["offsets"], _longest(case))
