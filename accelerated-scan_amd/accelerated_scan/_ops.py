@@ -18,6 +18,7 @@ are public as ``torch.ops.accelerated_scan.*``.
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi
 
@@ -291,6 +292,19 @@ torch.library.register_autograd(
 # Gated delta rule and gated norm (modules ``delta`` and ``norm``).  The ``*_run`` functions choose between the
 # custom operator, while a graph is being captured, and the direct call.
 # ---------------------------------------------------------------------------
+def no_tangents(*tensors) -> None:
+    """Refuse tensors that carry a forward-mode tangent: these operators have none to hand on, and results without one
+    read as a derivative of zero.  (Outside a dual level, where no tensor has one, this is one comparison.)"""
+    if forward_ad._current_level < 0:
+        return
+    # (the body of an operator that changes an argument runs behind the dispatch key that takes a dual tensor apart)
+    hidden = torch._C._dispatch_tls_local_exclude_set().remove(torch._C.DispatchKey.ADInplaceOrView)
+    with torch._C._ForceDispatchKeyGuard(torch._C._dispatch_tls_local_include_set(), hidden):
+        duals = any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if duals:
+        raise NotImplementedError("accelerated_scan: the gated delta rule and the gated norm have no forward-mode derivatives")
+
+
 def _delta_outputs(queries, values, initial, offsets, keep):
     """Empty (out, final, states, updates) of a delta rule call."""
     batch, tokens, _, key_dim = queries.shape
@@ -358,6 +372,7 @@ def _on_16_bytes(t):
 
 
 def _delta_backward(queries, keys, values, log_gates, beta, states, updates, offsets, scale, d_out, d_final, started):
+    no_tangents(states, updates, d_out, d_final)
     grads = _delta_gradients(queries, keys, values, log_gates, beta, states, started, offsets)
     if offsets is not None and offsets.shape[0] == 1:
         for g in grads:
@@ -461,6 +476,7 @@ def _(x, gate, weight, eps):
 
 
 def _gated_norm_backward(x, gate, weight, d_out, eps):
+    no_tangents(d_out)
     d_x, d_gate = torch.empty_like(x), torch.empty_like(gate)
     if x.numel() == 0:
         return d_x, d_gate, torch.zeros_like(weight)

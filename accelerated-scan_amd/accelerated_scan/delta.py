@@ -85,6 +85,7 @@ def _plainly_right(queries, keys, values, log_gates, beta):
 
 
 def _check_scan(queries, keys, values, log_gates, beta, initial, offsets):
+    _ops.no_tangents(queries, keys, values, log_gates, beta, initial)
     if (initial is None and offsets is None and queries.dim() == 4 and values.dim() == 4
             and _plainly_right(queries, keys, values, log_gates, beta)):
         return queries.shape[0]
@@ -163,8 +164,8 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
     Returns:
         (torch.Tensor, torch.Tensor): the outputs, shape (B, T, heads, value_dim), and the states behind the last
         tokens, fp32, as ``initial`` has them: hand them to the next chunk or to ``gated_delta_step``.
-        Differentiable once in all tensors but ``offsets``.  A token that is not finite leaves the outputs of the
-        tokens before it as they are.
+        Differentiable once, in reverse mode, in all tensors but ``offsets``.  A token that is not finite leaves the
+        outputs of the tokens before it as they are.
     """
     _check_scan(queries, keys, values, log_gates, beta, initial, offsets)
     scale = float(scale) if scale is not None else queries.shape[-1] ** -0.5
@@ -178,6 +179,7 @@ def gated_delta_scan(queries, keys, values, log_gates, beta, initial=None, scale
 
 
 def _check_step(queries, keys, values, log_gates, beta, states, slots):
+    _ops.no_tangents(queries, keys, values, log_gates, beta, states)
     if (queries.dim() == 3 and values.dim() == 3 and states.dtype == torch.float32 and states.dim() == 4
             and states.shape[1:] == (values.shape[1], queries.shape[2], values.shape[2]) and states.device == queries.device
             and states.is_contiguous()
@@ -205,7 +207,7 @@ def _check_step(queries, keys, values, log_gates, beta, states, slots):
 
 
 def gated_delta_step(queries, keys, values, log_gates, beta, states, slots=None, scale=None):
-    """Advance states by one token each, in place (no autograd: for generation).
+    """Advance states by one token each, in place (no autograd, in either mode: for generation).
 
     Arguments:
         queries, keys (torch.Tensor): shape (B, key_heads, key_dim), contiguous; fp32, bf16 or fp16.

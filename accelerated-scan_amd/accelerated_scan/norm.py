@@ -17,6 +17,7 @@ _REAL_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 def _check(x, gate, weight):
     """The passing case builds no message."""
+    _ops.no_tangents(x, gate, weight)
     dtype, device, shape = x.dtype, x.device, x.shape
     if (dtype in _REAL_DTYPES and gate.dtype == dtype and weight.dtype == dtype and gate.shape == shape
             and weight.shape == shape[-1:] and len(shape) > 0 and x.is_cuda and gate.device == device
@@ -79,7 +80,7 @@ def gated_norm(x, gate, weight, eps=1e-6):
         eps (float): added to the mean of the squares.
 
     Returns:
-        (torch.Tensor): the shape of x; differentiable once in x, gate and weight.
+        (torch.Tensor): the shape of x; differentiable once, in reverse mode, in x, gate and weight.
     """
     _check(x, gate, weight)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or weight.requires_grad):

@@ -243,3 +243,29 @@ def test_launches_beyond_the_hardware_are_refused(room):
     assert forward(room, rows=1 << 30, sequences=1, **many) == SHAPE  # 2^24 blocks
     assert step(room, batch=1 << 24, count=1 << 24, **many) == SHAPE
     assert step(room, count=1 << 62) == SHAPE
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent would get lost, and a result without one reads as a derivative of zero."""
+    from torch.autograd import forward_ad
+
+    *t, states = tensors(B=3, T=1)
+    token = [x[:, 0] for x in t]
+    rows = [torch.randn(3, 8), torch.randn(3, 8), torch.ones(8)]
+    ops = torch.ops.accelerated_scan
+    calls = [(lambda *a: delta.gated_delta_scan(*a), [*t, states]),
+             (lambda *a: ops.delta_forward(*a, None, 1.0, False), [*t, states]),
+             (lambda *a: delta.gated_delta_step(*a), [*token, states]),
+             (lambda *a: ops.delta_step(*a, None, 1.0), [*token, states]),
+             (lambda *a: norm.gated_norm(*a), rows),
+             (lambda *a: ops.gated_norm(*a, 1e-6), rows)]
+    for call, args in calls:
+        for i in range(len(args)):
+            with forward_ad.dual_level():
+                some = list(args)
+                some[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+                for grad in (True, False):
+                    with pytest.raises(NotImplementedError, match="forward-mode"), torch.set_grad_enabled(grad):
+                        call(*some)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="device tensor"):
+            call(*args)  # no tangent: the next check's turn

@@ -688,3 +688,39 @@ def test_gate_gradients_without_a_state(tokens, dtype):
     assert not got[3][:, 0].any()
     for name, a, b in zip(NAMES, got, want):
         ref.close(a, b, dtype, backward=True, what=name)
+
+
+def test_forward_mode_is_refused_and_leaves_the_rest_alone():
+    """Tangents of inputs and of incoming gradients; calls without one inside a dual level go on as they do outside."""
+    from torch.autograd import forward_ad
+
+    from accelerated_scan import delta, norm
+
+    data = on_gpu(ref.inputs(1, 70, 1, 2, 16, 16, torch.float32, seed=41))
+    weight = torch.ones(16, device=DEVICE)
+    dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+    want = delta.gated_delta_scan(*data)
+    with forward_ad.dual_level():
+        assert all(torch.equal(a, b) for a, b in zip(delta.gated_delta_scan(*data), want))
+        for i in range(6):
+            some = [dual(t) if i == j else t for j, t in enumerate(data)]
+            with pytest.raises(NotImplementedError):
+                delta.gated_delta_scan(*some)
+        with pytest.raises(NotImplementedError):
+            norm.gated_norm(dual(data[2]), data[2], weight)
+        leaves = [t.clone().requires_grad_() for t in data]
+        out, final = delta.gated_delta_scan(*leaves)
+        for d in ((dual(want[0]), want[1]), (want[0], dual(want[1]))):
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad([out, final], leaves, d, retain_graph=True)
+        normed = norm.gated_norm(leaves[2], data[2], weight)
+        with pytest.raises(NotImplementedError):
+            torch.autograd.grad(normed, leaves[2], dual(data[2]), retain_graph=True)
+        torch.autograd.grad([out, final], leaves, want)
+        token, states = [t[:, 0].contiguous() for t in data[:5]], data[5].clone()
+        for step in (delta.gated_delta_step, lambda *a: torch.ops.accelerated_scan.delta_step(*a, None, 0.25)):
+            with pytest.raises(NotImplementedError):
+                step(*token[:4], dual(token[4]), states)
+            assert torch.equal(states, data[5])
+        first = delta.gated_delta_step(*token, states)
+        assert torch.equal(first, torch.ops.accelerated_scan.delta_step(*token, data[5], None, 0.25)) and torch.equal(states, data[5])
