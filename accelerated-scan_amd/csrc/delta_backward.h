@@ -28,16 +28,15 @@ constexpr int kAhead = 256;   // workgroups from one to that which takes its pla
 enum { kFromState, kToState, kEarlier, kLater, kBetas, kSums };
 constexpr int kColumns = 64;  // value columns that a workgroup of delta_gradients takes at a time
 
-template <int NI, int NS, int NC, int DK>
+template <int NI, int NS, int DK>
 constexpr int kReverseBytes = 3 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                              Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + (4 + DK / 16) * 1024 + kMatrixBytes<NS> + 4 * kBlock * 4;
+                              2 * Exchange<NS, 2>::kBytes + (4 + DK / 16) * 1024 + Exchange<NS, kPairs>::kBytes + 4 * kBlock * 4;
 
 // The chain, last block first, divided like the forward one: 16 columns of D to a workgroup; state wave w keeps rows
 // dk/4 w .. of them and computes tokens 16w .. 16w+15; D, dU and -diag(beta e^c) dR go round through LDS.  Four waves
 // compute what does not wait for D (P^T dO and Q^T diag(scale e^c) dO) and write what leaves the chain, four load.
-// What enters D for good (P^T dO, W and the rows from dR) is in NC parts, the rest in NS, as in the forward chain.
 // q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.
-template <class E, int NI, int NS, int NC, int DK>
+template <class E, int NI, int NS, int DK>
 __global__ __launch_bounds__(768) void delta_reverse_chain(
     DeltaShape s, const typename E::S* __restrict__ q, const typename E::S* __restrict__ k,
     const typename E::S* __restrict__ d_out, const float* __restrict__ gates, const char* __restrict__ t_in,
@@ -65,16 +64,14 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
     m += 2 * Tile<NI, 16>::kBytes;
     Exchange<NS, kDepths> xs(m);
     m += Exchange<NS, kDepths>::kBytes;
-    Exchange<NS, 2> xr(m);
-    m += Exchange<NS, 2>::kBytes;
-    Exchange<NC, 2> xu(m);
-    m += Exchange<NC, 2>::kBytes;
+    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes);
+    m += 2 * Exchange<NS, 2>::kBytes;
     fx4* const po_at = reinterpret_cast<fx4*>(m) + lane;  // accumulator tiles from wave to wave, a KiB each
     fx4* const dr_at = po_at;  // (P^T dO is read in front of the second barrier, dR written behind it)
     fx4* const qw_at = po_at + 4 * 64;
     m += (4 + DK / 16) * 1024;
-    char* const matrix_at = m;
-    float* const gate = reinterpret_cast<float*>(m + kMatrixBytes<NS>);
+    Exchange<NS, kPairs> matrix(m);
+    float* const gate = reinterpret_cast<float*>(m + Exchange<NS, kPairs>::kBytes);
 
     constexpr uint32_t kSize = sizeof(ES);
     constexpr int kKeyBytes = kBlock * DK * kSize;
@@ -90,7 +87,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         return static_cast<const char*>(p) + (seq_row + last * kBlock) * step + at_head;
     };
     const int64_t entry0 = (seq_block + last) * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, t_move = (int64_t)s.heads * kMatrixBytes<NS>, p_move = (int64_t)s.heads * kMatrixBytes<NC>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes;
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
     const auto keys_at = [&](int64_t n_block) { return Tile<NI, DK>(smem + (n_block & 1) * Tile<NI, DK>::kBytes); };
@@ -133,8 +130,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
                 const fx4 po = po_at[wave * 64], until = gate_rows(kUntil);
-                tm[0] = matrix_operand<NS>(matrix_at, pair_upper(wave, wave >> 1), lane);
-                tm[1] = matrix_operand<NS>(matrix_at, pair_upper(wave, 1), lane);
+                tm[0] = matrix.get(pair_upper(wave, wave >> 1), lane);
+                tm[1] = matrix.get(pair_upper(wave, 1), lane);
                 beta_since = gate_rows(kBetaSince);
                 whole = gate[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
@@ -160,12 +157,12 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 if (wave < 2) {
-                    u2 = mma_all<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
-                    u = mma_all<NS, NS>(tm[1], high, u);
+                    u2 = mma<NS, NS>(tm[0], low, fx4{0, 0, 0, 0});
+                    u = mma<NS, NS>(tm[1], high, u);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 } else {
-                    u = mma_all<NS, NS>(tm[1], high, u);
+                    u = mma<NS, NS>(tm[1], high, u);
                 }
             }
             {
@@ -179,7 +176,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 
             // D0 = e^c[63] D1 + Q^T diag(scale e^c) dO - K^T diag(beta e^c) dR
             {
-                const Operand<NC> low = xu.get(0, lane), high = xu.get(1, lane);
+                const Operand<NS> low = xu.get(0, lane), high = xu.get(1, lane);
                 fx4 qw[kOwn], D2[kOwn];
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) qw[t] = qw_at[(kOwn * wave + t) * 64];
@@ -188,8 +185,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) D[t][r] *= whole;
-                    D[t] = mma<NI, NC>(k_low[t], low, D[t]);
-                    D2[t] = mma<NI, NC>(k_high[t], high, qw[t]);
+                    D[t] = mma<NI, NS>(k_low[t], low, D[t]);
+                    D2[t] = mma<NI, NS>(k_high[t], high, qw[t]);
                 }
                 read_block(now > 0 ? now - 1 : now);
 #pragma unroll
@@ -214,23 +211,23 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         }
     } else if (role == 1 && seq_length > 0) {
         // In front of the first block loads repeat it or give zero and stores are dropped: no condition stands around them.
-        Operand<NC> pm[2][2];
-        const char* p_p = p_in + entry0 * kMatrixBytes<NC>;
+        fx4 p_raw[2][2][2];
+        const char* p_p = p_in + entry0 * kMatrixBytes;
         char* state_p = reinterpret_cast<char*>(d_states + entry0 * s.dk * s.dv);
         const int quad = col0 + 4 * g;
         char *v_p = const_cast<char*>(start_of(d_v, v_step, (int64_t)head * s.dv * kSize));
         char *r_p = const_cast<char*>(start_of(d_rows, r_step, (int64_t)head * s.dv * 4));
         const auto load_p = [&](int64_t n_block, int set) __attribute__((always_inline)) {
-            const Buffer b = buffer_of(p_p, kMatrixBytes<NC>);
-            pm[set][0] = matrix_operand<NC>(b, wave < 2 ? pair_upper(wave, 0) : (int)(kOutside >> 12), lane);
-            pm[set][1] = matrix_operand<NC>(b, pair_upper(wave, 1), lane);
-            if (n_block > 0) p_p -= p_move;
+            const Buffer b = buffer_of(p_p, kMatrixBytes);
+            fetch_matrix(b, wave < 2, pair_upper(wave, 0), lane, p_raw[set][0]);
+            fetch_matrix(b, true, pair_upper(wave, 1), lane, p_raw[set][1]);
+            if (n_block > 0) p_p -= matrix_move;
         };
         const auto outputs = [&](int64_t n_block, int set) __attribute__((always_inline)) {  // P^T dO
             const Tile<NI, 16> ot = outs_at(n_block);
             fx4 po = {0, 0, 0, 0};
-            if (wave < 2) po = mma<NC, NI>(pm[set][0], ot.down(0, 0, lane), po);
-            po_at[wave * 64] = mma<NC, NI>(pm[set][1], ot.down(32, 0, lane), po);
+            if (wave < 2) po = mma<NS, NI>(operand_of<NS>(p_raw[set][0][0], p_raw[set][0][1]), ot.down(0, 0, lane), po);
+            po_at[wave * 64] = mma<NS, NI>(operand_of<NS>(p_raw[set][1][0], p_raw[set][1][1]), ot.down(32, 0, lane), po);
         };
         load_p(last, 0);
         load_p(last - 1, 1);
@@ -250,7 +247,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 for (int r = 0; r < 4; ++r) w[t][r] *= s.scale * f[r];
             }
             const float beta = gate[kBeta * kBlock + token];
-            const Operand<NC> w_low = operand_of<NC>(w[0], w[1]), w_high = operand_of<NC>(w[2], w[3]);
+            const Operand<NS> w_low = operand_of<NS>(w[0], w[1]), w_high = operand_of<NS>(w[2], w[3]);
             {
                 const Buffer to = buffer_of(state_p, now >= 0 ? (int64_t)s.dk * s.dv * 4 : 0);
 #pragma unroll
@@ -261,8 +258,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < kOwn; ++t) {
-                fx4 qw = mma<NI, NC>(qt.down_features(0, kOwn * wave + t, lane), w_low, fx4{0, 0, 0, 0});
-                qw = mma<NI, NC>(qt.down_features(32, kOwn * wave + t, lane), w_high, qw);
+                fx4 qw = mma<NI, NS>(qt.down_features(0, kOwn * wave + t, lane), w_low, fx4{0, 0, 0, 0});
+                qw = mma<NI, NS>(qt.down_features(32, kOwn * wave + t, lane), w_high, qw);
                 qw_at[(kOwn * wave + t) * 64] = qw;
             }
             lds_barrier();
@@ -288,14 +285,14 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
         // of 128 x 128) took 192 us, with one block 132)
         constexpr int kSets = sizeof(Eight<E>) * kCopies > 64 ? 1 : 2;
         Eight<E> k_raw[kSets][kCopies], q_raw[kSets][kCopies], o_raw[kSets];
-        fx4 t_raw[kSets][kPieces<NS>];
+        fx4 t_raw[kSets][kPieces];
         float gate_raw[kSets];
         const int64_t copy0 = ((seq_block + last) * s.key_heads + key_head) * kBlock * DK;
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *q_p = reinterpret_cast<const char*>(q + copy0);
         const char* o_p = start_of(d_out, v_step, (int64_t)head * s.dv * kSize);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const char* t_p = t_in + entry0 * kMatrixBytes;
         const auto load_block = [&](int64_t n_block, int set) __attribute__((always_inline)) {
-            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes<NS>);
+            const Buffer kb = buffer_of(k_p, kKeyBytes), qb = buffer_of(q_p, kKeyBytes), tb = buffer_of(t_p, kMatrixBytes);
             const Buffer ob = d_out != nullptr ? rows_of(o_p, n_block, v_step, s.dv * kSize) : buffer_of(k_p, 0);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) {
@@ -305,13 +302,13 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             o_raw[set] = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
 #pragma unroll
-            for (int i = 0; i < kPieces<NS>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(buffer_of(gate_p, kGateFloats * 4), tid * 4);
             o_p -= v_move;
             if (n_block > 0) {
                 k_p -= k_move;
                 q_p -= k_move;
-                t_p -= t_move;
+                t_p -= matrix_move;
                 gate_p -= gate_move;
             }
         };
@@ -321,8 +318,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             outs_at(n_block).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces<NS>; ++i)
-                if ((tid + 256 * i) * 16 < kMatrixBytes<NS>) *reinterpret_cast<fx4*>(matrix_at + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces; ++i) matrix.put(4 * i + wave, lane, t_raw[set][i]);
             gate[tid] = gate_raw[set];
         };
         const auto stage_queries = [&](int set) __attribute__((always_inline)) {
@@ -337,9 +333,9 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
                 const int64_t back = last - n_block, rows = seq_length - n_block * kBlock < kBlock ? seq_length - n_block * kBlock : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) - back * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) - back * k_move;
-                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NS> - back * t_move, p_in + entry0 * kMatrixBytes<NC> - back * p_move,
+                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes - back * matrix_move, p_in + entry0 * kMatrixBytes - back * matrix_move,
                                    start_of(d_out, v_step, (int64_t)head * s.dv * kSize) - back * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NC> / 128,
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes / 128, kMatrixBytes / 128,
                                    d_out != nullptr ? (int)rows * ((row_bytes + 127) / 128) : 0},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);

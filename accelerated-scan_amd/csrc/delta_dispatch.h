@@ -20,7 +20,6 @@ inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 
 // The workspace's parts: table of the blocks' gates, T, P, copies of keys and queries, and for the backward
 // pass the state gradients behind every block, the rows dR and sums over heads that share their keys.
-template <int NS, int NC>
 struct DeltaParts {
     size_t gates, t, p, k, q, d_states, d_rows, sums, end;
     DeltaParts(const DeltaShape& s, bool backward, size_t element) {
@@ -28,8 +27,8 @@ struct DeltaParts {
         const size_t copy = (size_t)s.blocks * s.key_heads * kBlock * (s.dk <= 64 ? 64 : 128) * element;
         gates = 0;
         t = round_up(gates + entries * kGateFloats * 4);
-        p = round_up(t + entries * kMatrixBytes<NS>);
-        k = round_up(p + entries * (backward ? kMatrixBytes<NC> : kMatrixBytes<NS>));
+        p = round_up(t + entries * kMatrixBytes);
+        k = round_up(p + entries * kMatrixBytes);
         q = round_up(k + copy);
         d_states = round_up(q + copy);
         d_rows = round_up(d_states + (backward ? entries * s.dk * s.dv * 4 : 0));
@@ -44,11 +43,11 @@ hipError_t delta_launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_
     return hipGetLastError();
 }
 
-template <class E, int NI, int NS, int NC, int DK>
+template <class E, int NI, int DK>
 hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void* log_gates, const void* beta,
-                   char* ws, const DeltaParts<NS, NC>& at, bool upper, hipStream_t stream) {
+                   char* ws, const DeltaParts& at, bool upper, hipStream_t stream) {
     using S = typename E::S;
-    const auto kernel = upper ? delta_prepare<E, NI, NC, NS, DK, true> : delta_prepare<E, NI, NS, NS, DK, false>;
+    const auto kernel = upper ? delta_prepare<E, NI, DK, true> : delta_prepare<E, NI, DK, false>;
     return delta_launch(kernel, dim3((unsigned)s.blocks, (unsigned)s.heads), 256,
                         kPrepareBytes<NI, DK>, stream, s, static_cast<const S*>(q), static_cast<const S*>(k),
                         log_gates, beta, reinterpret_cast<float*>(ws + at.gates), ws + at.t, ws + at.p,
@@ -57,40 +56,40 @@ hipError_t prepare(const DeltaShape& s, const void* q, const void* k, const void
 
 constexpr int kLdsBytes = 160 * 1024;  // of a compute unit
 
-template <class E, int NI, int NS, int NC, int DK>
+template <class E, int NI, int NS, int DK>
 int delta_forward_dk(const DeltaForward& f) {
-    static_assert(kChainBytes<NI, NS, NC, DK> <= kLdsBytes && kPrepareBytes<NI, DK> <= kLdsBytes, "fits a compute unit");
+    static_assert(kChainBytes<NI, NS, DK> <= kLdsBytes && kPrepareBytes<NI, DK> <= kLdsBytes, "fits a compute unit");
     using S = typename E::S;
     const DeltaShape& s = f.shape;
-    const DeltaParts<NS, NC> at(s, false, sizeof(S));
+    const DeltaParts at(s, false, sizeof(S));
     if (s.blocks > 0) {
-        const hipError_t e = prepare<E, NI, NS, NC, DK>(s, f.q, f.k, f.log_gates, f.beta, f.workspace, at, false, f.stream);
+        const hipError_t e = prepare<E, NI, DK>(s, f.q, f.k, f.log_gates, f.beta, f.workspace, at, false, f.stream);
         if (e != hipSuccess) return delta_status(e);
     }
-    const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, NC, DK, true> : delta_chain<E, NI, NS, NC, DK, false>;
+    const auto chain = f.states != nullptr ? delta_chain<E, NI, NS, DK, true> : delta_chain<E, NI, NS, DK, false>;
     return delta_status(delta_launch(
-        chain, dim3((unsigned)chain_grid(s)), 768, kChainBytes<NI, NS, NC, DK>, f.stream,
+        chain, dim3((unsigned)chain_grid(s)), 768, kChainBytes<NI, NS, DK>, f.stream,
         s, reinterpret_cast<const S*>(f.workspace + at.q), reinterpret_cast<const S*>(f.workspace + at.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
-        static_cast<S*>(f.out), f.final, f.states, f.updates, chain_touches<NC, DK>(s)));
+        static_cast<S*>(f.out), f.final, f.states, f.updates, chain_touches<NS, DK>(s)));
 }
 
-template <class E, int NI, int NS, int NC, int DK>
+template <class E, int NI, int NS, int DK>
 int delta_backward_dk(const DeltaBackward& f) {
-    static_assert(kReverseBytes<NI, NS, NC, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + kGradientStatic <= kLdsBytes, "fits a compute unit");
+    static_assert(kReverseBytes<NI, NS, DK> <= kLdsBytes && kGradientBytes<NI, NS, DK> + kGradientStatic <= kLdsBytes, "fits a compute unit");
     using S = typename E::S;
     const DeltaShape& s = f.shape;
-    const DeltaParts<NS, NC> at(s, true, sizeof(S));
+    const DeltaParts at(s, true, sizeof(S));
     char* ws = f.workspace;
     hipError_t e = hipSuccess;
-    if (s.blocks > 0) e = prepare<E, NI, NS, NC, DK>(s, f.q, f.k, f.log_gates, f.beta, ws, at, true, f.stream);
+    if (s.blocks > 0) e = prepare<E, NI, DK>(s, f.q, f.k, f.log_gates, f.beta, ws, at, true, f.stream);
     if (e != hipSuccess) return delta_status(e);
     const float* gates = reinterpret_cast<const float*>(ws + at.gates);
     float* d_states = reinterpret_cast<float*>(ws + at.d_states);
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
-    e = delta_launch(delta_reverse_chain<E, NI, NS, NC, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NS, NC, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
+    e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NS, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
-                     f.d_initial, d_states, d_rows, chain_touches<NC, DK>(s));
+                     f.d_initial, d_states, d_rows, chain_touches<NS, DK>(s));
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
     const bool shared = s.heads > s.key_heads;
     const auto kernel = shared ? delta_gradients<E, NI, NS, DK, true> : delta_gradients<E, NI, NS, DK, false>;
@@ -123,16 +122,16 @@ int delta_step_any(const DeltaStep& p) {
 
 }  // namespace
 
-#define ASCAN_DEFINE_DELTA(suffix, E, NI, NS, NC)                                                                   \
+#define ASCAN_DEFINE_DELTA(suffix, E, NI, NS)                                                                       \
     namespace ascan {                                                                                           \
     int delta_forward_##suffix(const DeltaForward& f) {                                                         \
-        return f.shape.dk <= 64 ? delta_forward_dk<E, NI, NS, NC, 64>(f) : delta_forward_dk<E, NI, NS, NC, 128>(f);     \
+        return f.shape.dk <= 64 ? delta_forward_dk<E, NI, NS, 64>(f) : delta_forward_dk<E, NI, NS, 128>(f);     \
     }                                                                                                           \
     int delta_backward_##suffix(const DeltaBackward& f) {                                                       \
-        return f.shape.dk <= 64 ? delta_backward_dk<E, NI, NS, NC, 64>(f) : delta_backward_dk<E, NI, NS, NC, 128>(f);   \
+        return f.shape.dk <= 64 ? delta_backward_dk<E, NI, NS, 64>(f) : delta_backward_dk<E, NI, NS, 128>(f);   \
     }                                                                                                           \
     int delta_step_##suffix(const DeltaStep& p) { return delta_step_any<E>(p); }                                \
-    size_t delta_workspace_##suffix(const DeltaShape& s, bool backward) { return DeltaParts<NS, NC>(s, backward, sizeof(E::S)).end; } \
+    size_t delta_workspace_##suffix(const DeltaShape& s, bool backward) { return DeltaParts(s, backward, sizeof(E::S)).end; } \
     }
 
 }  // namespace ascan

@@ -40,8 +40,8 @@ inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads +
 // blocks: bf16 (2, 4096, 16 heads of 128 x 128) forward 155 -> 135 us, backward 201 -> 167, (1, 16384, 32 heads)
 // 394 -> 387; and gives nothing where workgroups follow each other (fp16, 16 packed sequences, 2048 workgroups: 243 us without,
 // 245 with), where blocks are small (key size 64: 58 and 58.5) and where fp32 products take longer than the loads (74 and 74).
-template <int NC, int DK>
-inline bool chain_touches(const DeltaShape& s) { return NC > 0 && DK == 128 && chain_grid(s) <= 512; }
+template <int NS, int DK>
+inline bool chain_touches(const DeltaShape& s) { return NS > 0 && DK == 128 && chain_grid(s) <= 512; }
 
 // A chain's workgroup may have as many lines of 128 bytes on their way as its compute unit's cache holds, 256.  At the
 // latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 60 (and nobody else uses the
@@ -64,13 +64,11 @@ __device__ __forceinline__ int touch(const Lines& l, int id) {
     return p != nullptr ? *reinterpret_cast<const int*>(p) : 0;
 }
 
-template <int NI, int NS, int NC, int DK>
+template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
-                            2 * Exchange<NS, 2>::kBytes + Exchange<NC, 2>::kBytes + 2 * kMatrixBytes<NS> + 2 * 4 * kBlock * 4 + 64;
+                            3 * Exchange<NS, 2>::kBytes + 2 * Exchange<NS, kPairs>::kBytes + 2 * 4 * kBlock * 4 + 64;
 
-// Pieces of 16 bytes of T that each of 256 threads carries to LDS.
-template <int NC>
-constexpr int kPieces = (kMatrixBytes<NC> / 16 + 255) / 256;
+constexpr int kPieces = kMatrixTiles / 4;  // tiles of T that a wave of four carries to LDS
 
 // Zeros for what is not finite in an operand of tokens; the first such token, where its first four are row0 ..
 template <int P>
@@ -95,11 +93,10 @@ __device__ __forceinline__ int zero_odd(Operand<P>& o, int row0) {
 
 // q and k: the copies that delta_prepare made.  grid chain_grid(), 768 threads.  KEEP: write the states in front
 // of the blocks and the rows U.
-// U goes into the state in NC parts, all else is in NS: the rounding of U stays in a state for good, where the
-// delta rule corrects in the next block what it read and solved inexactly.  With NS = 2 and bf16 a state after 16384 tokens is
-// off by 2.8e-6 of its norm with NC = 2 (341 us), by 7.0e-7 with NC = 3 and all pairs of parts in T R (348 us),
-// by 1.4e-7 with three parts throughout, where the longer exchanges and matrices cost 478 us.
-template <class E, int NI, int NS, int NC, int DK, bool KEEP>
+// States, R, U, T and P are in NS parts.  T and P come from memory in fp32 and their parts are made by the waves with time for it:
+// as parts they are half as large again (bf16, 16384 tokens, 32 heads, with delta_prepare: 537 us so, 547 from fp32; packed
+// fp16 400 and 389, training 619 and 603).
+template <class E, int NI, int NS, int DK, bool KEEP>
 __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename E::S* __restrict__ q,
                                                    const typename E::S* __restrict__ k,
                                                    const typename E::S* __restrict__ v,
@@ -127,12 +124,10 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     m += 2 * Tile<NI, 16>::kBytes;
     Exchange<NS, kDepths> xs(m);
     m += Exchange<NS, kDepths>::kBytes;
-    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes);
-    m += 2 * Exchange<NS, 2>::kBytes;
-    Exchange<NC, 2> xd(m);
-    m += Exchange<NC, 2>::kBytes;
+    Exchange<NS, 2> xr(m), xu(m + Exchange<NS, 2>::kBytes), xd(m + 2 * Exchange<NS, 2>::kBytes);
+    m += 3 * Exchange<NS, 2>::kBytes;
     char* const matrix_at = m;
-    float* const gate_at = reinterpret_cast<float*>(m + 2 * kMatrixBytes<NS>);
+    float* const gate_at = reinterpret_cast<float*>(m + 2 * Exchange<NS, kPairs>::kBytes);
     // Per column the first token of the block at hand from which its state is not finite.  A NaN in R meets the zeros of T
     // and would meet those of P and reach earlier tokens: U, which shows it, is computed again with a zero in its place,
     // and state and outputs get the NaN by this number.  (A test of R itself stands on every block's way.)
@@ -149,19 +144,15 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     };
     const auto start_of = [&](const void* p, uint32_t step, int64_t at_head) { return static_cast<const char*>(p) + seq_row * step + at_head; };
     const int64_t entry0 = seq_block * s.heads + head;
-    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes<NS>;
+    const int64_t gate_move = (int64_t)s.heads * kGateFloats * 4, matrix_move = (int64_t)s.heads * kMatrixBytes;
     constexpr int kKeyBytes = kBlock * DK * kSize;  // of a block, in the copies
     const int64_t k_move = (int64_t)s.key_heads * kKeyBytes, v_move = (int64_t)v_step * kBlock;
     const char* gate_p = reinterpret_cast<const char*>(gates + entry0 * kGateFloats);
     const auto gates_here = [&]() { return buffer_of(gate_p, kGateFloats * 4); };
-    // (waves 0 and 1 have one operand to a row of tiles: their second load lies outside and gives zero)
-    const auto load_matrix = [&](const char* from, Operand<NS>(&o)[2]) {
-        const Buffer b = buffer_of(from, kMatrixBytes<NS>);
-        o[0] = matrix_operand<NS>(b, pair_lower(wave, 0), lane);
-        o[1] = matrix_operand<NS>(b, wave >= 2 ? pair_lower(wave, 1) : (int)(kOutside >> 12), lane);
-    };
     const auto keys_at = [&](int64_t first) { return Tile<NI, DK>(smem + ((first / kBlock) & 1) * Tile<NI, DK>::kBytes); };
-    const auto matrix_of = [&](int64_t first) { return matrix_at + ((first / kBlock) & 1) * kMatrixBytes<NS>; };
+    const auto matrix_of = [&](int64_t first) {
+        return Exchange<NS, kPairs>(matrix_at + ((first / kBlock) & 1) * Exchange<NS, kPairs>::kBytes);
+    };
     const auto gate_of = [&](int64_t first) { return gate_at + ((first / kBlock) & 1) * 4 * kBlock; };
     const auto values_at = [&](int64_t first) { return Tile<NI, 16>(vt_at + ((first / kBlock) & 1) * Tile<NI, 16>::kBytes); };
 
@@ -210,8 +201,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 Operand<NS> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
-                tm[0] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane);
-                tm[1] = matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane);
+                tm[0] = matrix_of(first).get(pair_lower(wave, 0), lane);
+                tm[1] = matrix_of(first).get(pair_lower(wave, wave >> 1), lane);
                 until = gate_rows(first, kUntil);
                 whole = gate_of(first)[kSince * kBlock + kBlock - 1];
                 __builtin_amdgcn_sched_barrier(0);  // all reads on their way before the first product waits for one
@@ -241,12 +232,12 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 // (one branch around all of it: where a branch stands between a matrix instruction and the first use of its
                 // result, the compiler has left out the wait)
                 if (wave >= 2) {
-                    u2 = mma_all<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
-                    u = mma_all<NS, NS>(tm[0], low, u);
+                    u2 = mma<NS, NS>(tm[1], high, fx4{0, 0, 0, 0});
+                    u = mma<NS, NS>(tm[0], low, u);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] += u2[r];
                 } else {
-                    u = mma_all<NS, NS>(tm[0], low, u);
+                    u = mma<NS, NS>(tm[0], low, u);
                 }
             }
             {
@@ -263,8 +254,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 odd = min(odd, zero_odd(low, 4 * g));
                 odd = min(odd, __shfl_xor(odd, 16));
                 odd = min(odd, __shfl_xor(odd, 32));
-                u = mma_all<NS, NS>(matrix_operand<NS>(matrix_of(first), pair_lower(wave, 0), lane), low, fx4{0, 0, 0, 0});
-                u2 = mma_all<NS, NS>(matrix_operand<NS>(matrix_of(first), pair_lower(wave, wave >> 1), lane), high, fx4{0, 0, 0, 0});
+                u = mma<NS, NS>(matrix_of(first).get(pair_lower(wave, 0), lane), low, fx4{0, 0, 0, 0});
+                u2 = mma<NS, NS>(matrix_of(first).get(pair_lower(wave, wave >> 1), lane), high, fx4{0, 0, 0, 0});
                 fx4 y;
 #pragma unroll
                 for (int r = 3; r >= 0; --r) {
@@ -285,15 +276,15 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 
             // S1 = e^c[63] S0 + K^T diag(e^(c[63]-c)) U
             {
-                const Operand<NC> low = xd.get(0, lane), high = xd.get(1, lane);
+                const Operand<NS> low = xd.get(0, lane), high = xd.get(1, lane);
                 __builtin_amdgcn_sched_barrier(0);
                 fx4 S2[kOwn];
 #pragma unroll
                 for (int t = 0; t < kOwn; ++t) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) S[t][r] *= whole;
-                    S[t] = mma<NI, NC>(k_low[t], low, S[t]);
-                    S2[t] = mma<NI, NC>(k_high[t], high, fx4{0, 0, 0, 0});
+                    S[t] = mma<NI, NS>(k_low[t], low, S[t]);
+                    S2[t] = mma<NI, NS>(k_high[t], high, fx4{0, 0, 0, 0});
                 }
                 read_block(more ? first + kBlock : first);
 #pragma unroll
@@ -321,11 +312,11 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         // did not would make its wait one for all before it.  Behind the last block loads repeat it or give zero and
         // stores are dropped, so that no condition stands around them.
         Eight<E> q_raw[2][kDepths];
-        Operand<NS> pm[2][2];
+        fx4 p_raw[2][2][2];
         float since[2];
-        const char *q_p = reinterpret_cast<const char*>(q + copy0), *p_p = p_in + entry0 * kMatrixBytes<NS>;
+        const char *q_p = reinterpret_cast<const char*>(q + copy0), *p_p = p_in + entry0 * kMatrixBytes;
         const char* out_p = start_of(out, v_step, v_head);
-        // KEEP: state and updates leave from their parts in LDS, to 2^-16 like all that is computed from them (fp32: exact)
+        // KEEP: state and updates leave from their parts in LDS, to 2^-24
         const uint32_t u_step = s.heads * s.dv * 4;
         [[maybe_unused]] char* state_p = reinterpret_cast<char*>(states + entry0 * s.dk * s.dv);
         [[maybe_unused]] char* update_p = reinterpret_cast<char*>(updates + (seq_row * s.heads + head) * s.dv);
@@ -337,7 +328,9 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             if (first + kBlock < seq_length) q_p += k_move;
         };
         const auto load_p = [&](int64_t first, int set) __attribute__((always_inline)) {
-            load_matrix(p_p, pm[set]);
+            const Buffer b = buffer_of(p_p, kMatrixBytes);
+            fetch_matrix(b, true, pair_lower(wave, 0), lane, p_raw[set][0]);
+            fetch_matrix(b, wave >= 2, pair_lower(wave, 1), lane, p_raw[set][1]);  // (one product to a row of tiles in waves 0, 1)
             since[set] = fetch4(gates_here(), kSince * 256 + token * 4);
             if (first + kBlock < seq_length) {
                 p_p += matrix_move;
@@ -352,11 +345,15 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             lds_barrier();
             // (Q S0)^T (rows: state columns, columns: tokens)
             fx4 o = {0, 0, 0, 0}, o2 = {0, 0, 0, 0};
+            Operand<NS> p_low, p_high;
             {
                 Operand<NS> so[kDepths];
 #pragma unroll
                 for (int d = 0; d < kDepths; ++d) so[d] = xs.get(d, lane);
                 __builtin_amdgcn_sched_barrier(0);
+                // P's parts while the reads are under way: later they are on the chain's way
+                p_low = operand_of<NS>(p_raw[own][0][0], p_raw[own][0][1]);
+                p_high = operand_of<NS>(p_raw[own][1][0], p_raw[own][1][1]);
 #pragma unroll
                 for (int d = 0; d < kDepths; d += 2) {
                     o = mma<NS, NI>(so[d], operand_from<NI, E>(q_raw[own][d]), o);
@@ -381,12 +378,12 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             int odd[4];
             __builtin_memcpy(odd, odd_at + 4 * g, 16);
             if (wave >= 2) {
-                o2 = mma<NS, NS>(xu.get(1, lane), pm[own][1], fx4{0, 0, 0, 0});
-                o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
+                o2 = mma<NS, NS>(xu.get(1, lane), p_high, fx4{0, 0, 0, 0});
+                o = mma<NS, NS>(xu.get(0, lane), p_low, o);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) o[r] += o2[r];
             } else {
-                o = mma<NS, NS>(xu.get(0, lane), pm[own][0], o);
+                o = mma<NS, NS>(xu.get(0, lane), p_low, o);
             }
             if (__any(odd[0] < kBlock || odd[1] < kBlock || odd[2] < kBlock || odd[3] < kBlock)) {
 #pragma unroll
@@ -407,19 +404,19 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
     } else if (seq_length > 0) {
         // Keys, values, T and gates to LDS, three blocks ahead.
         Eight<E> k_raw[2][kCopies], v_raw[2];
-        fx4 t_raw[2][kPieces<NS>];
+        fx4 t_raw[2][kPieces];
         float gate_raw[2];
         const char *k_p = reinterpret_cast<const char*>(k + copy0), *v_p = start_of(v, v_step, v_head);
-        const char* t_p = t_in + entry0 * kMatrixBytes<NS>;
+        const char* t_p = t_in + entry0 * kMatrixBytes;
         const auto load_block = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Buffer kb = buffer_of(k_p, kKeyBytes), vb = rows_of(v_p, first, v_step, s.dv * kSize);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) k_raw[set][i] = fetch8<E>(kb, (tid + 256 * i) * 8 * kSize);
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
-            const Buffer tb = buffer_of(t_p, kMatrixBytes<NS>);
+            const Buffer tb = buffer_of(t_p, kMatrixBytes);
 #pragma unroll
-            for (int i = 0; i < kPieces<NS>; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(gates_here(), tid * 4);
             v_p += v_move;
             if (first + kBlock < seq_length) {
@@ -428,14 +425,18 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 gate_p += gate_move;
             }
         };
+        typename Exchange<NS, kPairs>::Kept t_kept[kPieces];
+        const auto make_parts = [&](int set) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) t_kept[i] = Exchange<NS, kPairs>::kept(t_raw[set][i]);
+        };
         const auto stage_block = [&](int64_t first, int set) __attribute__((always_inline)) {
             const Tile<NI, DK> kb = keys_at(first);
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
 #pragma unroll
-            for (int i = 0; i < kPieces<NS>; ++i)
-                if ((tid + 256 * i) * 16 < kMatrixBytes<NS>) *reinterpret_cast<fx4*>(matrix_of(first) + (tid + 256 * i) * 16) = t_raw[set][i];
+            for (int i = 0; i < kPieces; ++i) matrix_of(first).put(4 * i + wave, lane, t_kept[i]);
             gate_of(first)[tid] = gate_raw[set];
         };
         const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
@@ -446,9 +447,9 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
                 const int64_t n_block = first / kBlock, rows = seq_length - first < kBlock ? seq_length - first : kBlock;
                 const char* at_k = reinterpret_cast<const char*>(k + copy0) + n_block * k_move;
                 const char* at_q = reinterpret_cast<const char*>(q + copy0) + n_block * k_move;
-                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes<NS> + n_block * matrix_move,
-                                   p_in + entry0 * kMatrixBytes<NS> + n_block * matrix_move, start_of(v, v_step, v_head) + n_block * v_move},
-                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes<NS> / 128, kMatrixBytes<NS> / 128,
+                const Lines lines{{at_k, at_q, t_in + entry0 * kMatrixBytes + n_block * matrix_move,
+                                   p_in + entry0 * kMatrixBytes + n_block * matrix_move, start_of(v, v_step, v_head) + n_block * v_move},
+                                  {kKeyBytes / 128, kKeyBytes / 128, kMatrixBytes / 128, kMatrixBytes / 128,
                                    (int)rows * ((row_bytes + 127) / 128)},
                                   (row_bytes + 127) / 128, (int64_t)v_step};
                 touched = touch(lines, tid * groups + col0 / 16);
@@ -456,6 +457,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         };
         load_block(0, 0);
         load_block(kBlock, 1);
+        make_parts(0);
         stage_block(0, 0);
         load_block(2 * kBlock, 0);
         touch_block(3 * kBlock);
@@ -463,6 +465,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
         lds_barrier();
         const auto block = [&](int64_t first, int other) __attribute__((always_inline)) {
             lds_barrier();
+            make_parts(other);
             lds_barrier();
             stage_block(first + kBlock, other);  // the tiles' last readers are behind the first barrier
             lds_barrier();

@@ -13,12 +13,15 @@ namespace {
 enum { kBeta, kBetaSince, kSince, kUntil, kSumHigh, kSumLow, kGateRows };
 constexpr int kGateFloats = kGateRows * kBlock;
 
-template <int P>
-constexpr int kMatrixBytes = P == 0 ? kPairs * 64 * 8 * 4 : P * kPairs * 64 * 8 * 2;
+constexpr int kMatrixTiles = 2 * kPairs;                // of a triangular matrix in memory, fp32
+constexpr int kMatrixBytes = kMatrixTiles * 64 * 4 * 4;
 
 // Where products of depth 32 stand in a triangular matrix: row tile m, depths 32 s .. 32 s + 31.
 __device__ __forceinline__ constexpr int pair_lower(int m, int s) { return m < 2 ? m : 2 * m - 2 + s; }
 __device__ __forceinline__ constexpr int pair_upper(int m, int s) { return m < 2 ? 2 * m + s : m + 2; }
+
+// Where in memory lane `lane` has its four values of tile n of a product.
+__device__ __forceinline__ constexpr int matrix_place(int pair, int n, int lane) { return ((2 * pair + n) * 64 + lane) * 16; }
 
 struct BlockAt {
     int64_t row;  // first row of the block
@@ -114,8 +117,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
     return (((row >> 4) * (DK / 32) + (d >> 5)) * 64 + ((d >> 3) & 3) * 16 + (row & 15)) * 8;
 }
 
-// grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.  T is written in NT
-// parts, P in NP.
+// grid (blocks, heads), 256 threads.  `upper`: the transposes of T and P, for the backward pass.
 //
 // P leaves from the accumulators: the tile K_j Q_i^T has token i in a lane's column and its rows j along the depth, as
 // the operand wants it (Q_i K_j^T for the transpose).  The inverse of I + L is made by substitution inside the
@@ -128,7 +130,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
 // the chain 463 us without copies, 439 with; they cost this kernel 14).
 //
 // What bounds it: there it reads 130 MB and writes 350 MB in 107 us, 4.5 TB/s.
-template <class E, int NI, int NP, int NT, int DK, bool upper>
+template <class E, int NI, int DK, bool upper>
 __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
                                                      const typename E::S* __restrict__ k,
                                                      const void* __restrict__ log_gates, const void* __restrict__ beta,
@@ -214,10 +216,10 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
         for (int j = 0; j < kTiles; ++j) {
             if (j <= wave) {
                 const Operand<NI> o = kt.along(16 * j + c, d, g);
-                kk[j] = mma<NI, NI>(o, mine, kk[j]);
-                if (!upper) pq[j] = mma<NI, NI>(o, theirs, pq[j]);
+                kk[j] = mma_all<NI, NI>(o, mine, kk[j]);
+                if (!upper) pq[j] = mma_all<NI, NI>(o, theirs, pq[j]);
             }
-            if (upper && j >= wave) pq[j] = mma<NI, NI>(qt.along(16 * j + c, d, g), theirs, pq[j]);
+            if (upper && j >= wave) pq[j] = mma_all<NI, NI>(qt.along(16 * j + c, d, g), theirs, pq[j]);
         }
     }
     const int here = 16 * wave + c;
@@ -260,20 +262,14 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
             pq[j][r] = (upper ? row0 + r >= here && row0 + r < odd : row0 + r <= here_up_to) ? s.scale * e[r] * pq[j][r] : 0.0f;
     }
     {
-        char* to = p_out + (block * s.heads + head) * kMatrixBytes<NP>;
+        char* to = p_out + (block * s.heads + head) * kMatrixBytes;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const bool there = upper ? h >= (wave >> 1) : h <= (wave >> 1);
             if (there) {
-                const int i = (upper ? pair_upper(wave, h) : pair_lower(wave, h)) * 64 + lane;
-                const Operand<NP> o = operand_of<NP>(pq[2 * h], pq[2 * h + 1]);
-                if constexpr (NP == 0) {
-                    reinterpret_cast<fx4*>(to + i * 32)[0] = o.t[0];
-                    reinterpret_cast<fx4*>(to + i * 32)[1] = o.t[1];
-                } else {
+                const int pair = upper ? pair_upper(wave, h) : pair_lower(wave, h);
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
-                }
+                for (int n = 0; n < 2; ++n) *reinterpret_cast<fx4*>(to + matrix_place(pair, n, lane)) = pq[2 * h + n];
             }
         }
     }
@@ -343,7 +339,7 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
     }
     __syncthreads();
 
-    char* to = t_out + (block * s.heads + head) * kMatrixBytes<NT>;
+    char* to = t_out + (block * s.heads + head) * kMatrixBytes;
     for (int i = tid; i < kPairs * 64; i += 256) {
         const int pair = i >> 6;
         const int m = upper ? (pair < 4 ? pair >> 1 : pair - 2) : (pair < 2 ? pair : (pair + 2) >> 1);
@@ -362,43 +358,15 @@ __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const type
             a[r] -= row == col + r ? 1.0f : 0.0f;
             b[r] -= row == col + 16 + r ? 1.0f : 0.0f;
         }
-        const Operand<NT> o = operand_of<NT>(a, b);
-        if constexpr (NT == 0) {
-            reinterpret_cast<fx4*>(to + i * 32)[0] = o.t[0];
-            reinterpret_cast<fx4*>(to + i * 32)[1] = o.t[1];
-        } else {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) *reinterpret_cast<bx8*>(to + (n * kPairs * 64 + i) * 16) = o.p[n];
-        }
+        *reinterpret_cast<fx4*>(to + matrix_place(pair, 0, lane)) = a;
+        *reinterpret_cast<fx4*>(to + matrix_place(pair, 1, lane)) = b;
     }
 }
 
-// Operand `pair` of a matrix that delta_prepare wrote.
-template <int P>
-__device__ __forceinline__ Operand<P> matrix_operand(Buffer m, int pair, int lane) {
-    Operand<P> o;
-    if constexpr (P == 0) {
-        o.t[0] = fetch16(m, (pair * 64 + lane) * 32);
-        o.t[1] = fetch16(m, (pair * 64 + lane) * 32 + 16);
-    } else {
+// The tiles of product `pair` of a matrix that delta_prepare wrote, or zeros where it is not `there`.
+__device__ __forceinline__ void fetch_matrix(Buffer m, bool there, int pair, int lane, fx4 (&x)[2]) {
 #pragma unroll
-        for (int n = 0; n < P; ++n) o.p[n] = __builtin_bit_cast(bx8, fetch16(m, ((n * kPairs + pair) * 64 + lane) * 16));
-    }
-    return o;
-}
-
-// The same from a copy in LDS.
-template <int P>
-__device__ __forceinline__ Operand<P> matrix_operand(const char* m, int pair, int lane) {
-    Operand<P> o;
-    if constexpr (P == 0) {
-        o.t[0] = *reinterpret_cast<const fx4*>(m + (pair * 64 + lane) * 32);
-        o.t[1] = *reinterpret_cast<const fx4*>(m + (pair * 64 + lane) * 32 + 16);
-    } else {
-#pragma unroll
-        for (int n = 0; n < P; ++n) o.p[n] = *reinterpret_cast<const bx8*>(m + ((n * kPairs + pair) * 64 + lane) * 16);
-    }
-    return o;
+    for (int n = 0; n < 2; ++n) x[n] = fetch16(m, there ? matrix_place(pair, n, lane) : kOutside);
 }
 
 }  // namespace

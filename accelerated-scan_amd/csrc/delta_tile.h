@@ -15,8 +15,13 @@
 // Arithmetic (parameter P of an operand, its number of parts):
 //   P = 0   fp32 values and fp32 matrix instructions, 256 operations per clock and compute unit;
 //   P >= 1  a value is the sum of P bfloat16 parts (8 bits each: one part holds a bfloat16 value, two a
-//           half value without loss, or an fp32 value to 2^-16, three hold it to 2^-24), products are
+//           half value without loss, three an fp32 value to 2^-24), products are
 //           summed over the pairs of parts that count, at 4096 operations per clock and pair.
+// Tensors of 16 bits are taken in the parts that hold them, everything computed in three: states, their gradients and those
+// of fp32 gates leave in 32 bits, and in two parts they were off by 0.7 to 6e-6 (with equal keys, whose U is a small difference
+// of large terms, a state by 6e-5) where fp32 arithmetic gives 1 to 3e-7, and 16-bit outputs by a last bit ten times as often.
+// Three parts throughout cost a bf16 prompt (1, 16384, 32 heads of 128 x 128) 430 -> 520 to 545 us, packed fp16 sequences 295 -> 388,
+// a training step (bf16, 2 x 4096, 16 heads) 567 -> 593.
 #ifndef ASCAN_DELTA_TILE_H_
 #define ASCAN_DELTA_TILE_H_
 
@@ -113,7 +118,7 @@ __device__ __forceinline__ fx4 mma(const Operand<PA>& a, const Operand<PB>& b, f
     return c;
 }
 
-// The same over all pairs of parts, for a product in which the last ones are as large as the parts' own rounding.
+// The same over all pairs of parts: for two half values, whose second parts' product is as large as 2^-18.
 template <int PA, int PB>
 __device__ __forceinline__ fx4 mma_all(const Operand<PA>& a, const Operand<PB>& b, fx4 c) {
     if constexpr (PA == 0) {
@@ -438,18 +443,34 @@ struct Exchange {
 
     __device__ __forceinline__ explicit Exchange(char* p) : base(p) {}
 
-    __device__ __forceinline__ void put(int tile, int lane, const fx4& x) {
+    // A lane's four values as they are kept here.
+    struct Kept {
+        ux2 w[P == 0 ? 2 : P];
+    };
+    static __device__ __forceinline__ Kept kept(const fx4& x) {
+        Kept k;
         if constexpr (P == 0) {
-            *reinterpret_cast<fx4*>(base + (tile * 64 + lane) * 16) = x;
+            __builtin_memcpy(k.w, &x, 16);
         } else {
             uint32_t low[P], high[P];
             pair_parts<P>(x[0], x[1], low);
             pair_parts<P>(x[2], x[3], high);
 #pragma unroll
-            for (int i = 0; i < P; ++i)
-                *reinterpret_cast<ux2*>(base + ((i * N + (tile >> 1)) * 64 + lane) * 16 + (tile & 1) * 8) = ux2{low[i], high[i]};
+            for (int i = 0; i < P; ++i) k.w[i] = ux2{low[i], high[i]};
+        }
+        return k;
+    }
+    __device__ __forceinline__ void put(int tile, int lane, const Kept& k) {
+        if constexpr (P == 0) {
+            fx4 x;
+            __builtin_memcpy(&x, k.w, 16);
+            *reinterpret_cast<fx4*>(base + (tile * 64 + lane) * 16) = x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) *reinterpret_cast<ux2*>(base + ((i * N + (tile >> 1)) * 64 + lane) * 16 + (tile & 1) * 8) = k.w[i];
         }
     }
+    __device__ __forceinline__ void put(int tile, int lane, const fx4& x) { put(tile, lane, kept(x)); }
     __device__ __forceinline__ Operand<P> get(int n, int lane) const {
         Operand<P> o;
         if constexpr (P == 0) {

@@ -71,3 +71,19 @@ def close(got, want, like, backward=False, what="", grow=1.0):
     most = want.abs().max().item()
     over = (off.abs() - (u * want.abs() + 12 * stages * e * most)).max().item()
     assert over <= 0, f"{what}: a value is {over:.3g} beyond its bound"
+
+
+def close_in_32_bits(got, want, backward=False, what=""):
+    """A float32 result against float64, whatever the inputs' type, in the root mean square.
+
+    An operand lacks at most 2^-25 of itself (three bfloat16 parts hold a float32 value), the pairs of parts that are left
+    out come to 3 * 2^-25, and a sum of up to 128 products is made in at most 24 steps, each rounded to 2^-24 of a partial
+    sum.  Roundings are independent, so they add in squares: a product is off by at most sqrt((24 + 6) / 3) < 3.2 times
+    2^-24 of its size.  The six of the forward pass come to sqrt(6) 3.2 < 8, the twelve of a gradient to 11, and the condition
+    of I + L, below 4 for the largest error, takes a random one to twice its size at most: 16 and, with
+    the states' own error that the gradients are formed with, 32 times 2^-24."""
+    assert got.dtype == torch.float32
+    got, want = got.detach().cpu().double(), want.detach()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    rel, most = (got - want).norm().item() / want.norm().item(), (32 if backward else 16) * 2.0 ** -24
+    assert rel <= most, f"{what}: relative error {rel:.3g} over {most:.3g}"

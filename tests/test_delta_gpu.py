@@ -724,3 +724,48 @@ def test_forward_mode_is_refused_and_leaves_the_rest_alone():
             assert torch.equal(states, data[5])
         first = delta.gated_delta_step(*token, states)
         assert torch.equal(first, torch.ops.accelerated_scan.delta_step(*token, data[5], None, 0.25)) and torch.equal(states, data[5])
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(4, 50, 2, 2, 64, 64), (1, 700, 2, 2, 64, 64), (1, 500, 1, 2, 128, 128), (2, 90, 1, 3, 40, 72)], ids=str)
+def test_results_in_32_bits(shape, dtype):
+    """States and their gradients, and the gradients of gates in 32 bits, are as exact from 16-bit tensors as from others."""
+    from accelerated_scan import delta
+
+    data = ref.inputs(*shape, dtype, seed=42, gates=torch.float32, decay=0.2)
+    exact, leaves = as_exact(data, grad=True), on_gpu(data, grad=True)
+    results, got = ref.delta_scan(*exact), delta.gated_delta_scan(*leaves)
+    ref.close_in_32_bits(got[1], results[1], what="final")
+    gen = torch.Generator().manual_seed(43)
+    d_out, d_final = torch.randn(got[0].shape, generator=gen).to(dtype), torch.randn(got[1].shape, generator=gen)
+    want = torch.autograd.grad(results, exact[3:], [d_out.double(), d_final.double()])
+    for name, a, b in zip(NAMES[3:], torch.autograd.grad(got, leaves[3:], on_gpu([d_out, d_final])), want):
+        ref.close_in_32_bits(a, b, backward=True, what=name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_states_after_many_tokens(dtype):
+    from accelerated_scan import delta
+
+    data = ref.inputs(1, 4000, 1, 1, 128, 32, dtype, seed=44, gates=torch.float32, decay=0.02)
+    with torch.no_grad():
+        _, want = ref.delta_scan(*as_exact(data))
+        _, got = delta.gated_delta_scan(*on_gpu(data))
+    ref.close_in_32_bits(got, want, what="final")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("tokens, key_dim", [(64, 64), (640, 128)])
+def test_equal_keys_of_16_bits(tokens, key_dim, dtype):
+    """The matrix to invert at its worst: what a token adds to the state is a small difference of large terms, so that
+    fewer bits in them would show at once.  The state is held to the bound of 32-bit calls."""
+    from accelerated_scan import delta
+
+    data = ref.inputs(1, tokens, 1, 2, key_dim, 64, dtype, seed=45, gates=torch.float32)
+    data[1][:] = data[1][:, :1]
+    data[3].zero_()
+    data[4].fill_(0.99)
+    want, final = ref.delta_scan(*as_exact(data))
+    got, state = delta.gated_delta_scan(*on_gpu(data))
+    ref.close(got, want, dtype)
+    ref.close(state, final, torch.float32)
