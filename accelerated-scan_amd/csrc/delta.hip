@@ -121,6 +121,7 @@ int ascan_delta_forward(const void* q, const void* k, const void* v, const void*
     const int status = check_scan(needed, 6, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
     if (sequences == 0 || (rows == 0 && final == nullptr)) return ASCAN_OK;
+    if (rows > 0 && (states == nullptr) != (updates == nullptr)) return ASCAN_ERR_NULL_POINTER;
     for (const void* p : {static_cast<const void*>(initial), static_cast<const void*>(final),
                           static_cast<const void*>(states), static_cast<const void*>(updates)})
         if (misaligned(p, 16)) return ASCAN_ERR_MISALIGNED;

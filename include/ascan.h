@@ -408,7 +408,7 @@ ASCAN_API int ascan_backward_gated_values(const void* gate_inputs, const void* v
  *     no access outside the buffers;
  *   - initial (or NULL for zeros) and final (or NULL) hold one state per sequence;
  *   - states (ascan_delta_blocks() x heads x dk x dv) and updates (rows x heads x dv) are what the backward pass
- *     needs of the forward pass; NULL where there will be none;
+ *     needs of the forward pass; both NULL where there will be none, and one alone is refused;
  *   - d_out and d_final may be NULL (zeros), d_initial may be NULL (not wanted);
  *   - the workspace has the size that ascan_delta_workspace_bytes gives, and belongs to the call until it has run.
  *     Its contents on entry do not matter;

@@ -269,3 +269,12 @@ def test_forward_mode_tangents_are_refused():
                         call(*some)
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="device tensor"):
             call(*args)  # no tangent: the next check's turn
+
+
+def test_states_and_updates_come_together(room):
+    """What a backward pass needs is both or none: the kernel that keeps one writes the other too."""
+    kept = dict(states=room + 0x50000, updates=room + 0x58000)
+    for name in kept:
+        assert forward(room, **{name: kept[name]}) == NULL, name
+    assert forward(room, **kept, out=room) == OVERLAP  # a pair gets past that check
+    assert forward(room, states=room + 0x50000, rows=0, sequences=0) == OK
