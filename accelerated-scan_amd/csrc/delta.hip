@@ -121,7 +121,6 @@ int ascan_delta_forward(const void* q, const void* k, const void* v, const void*
     const int status = check_scan(needed, 6, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
     if (sequences == 0 || (rows == 0 && final == nullptr)) return ASCAN_OK;
-    if (rows > 0 && (states == nullptr) != (updates == nullptr)) return ASCAN_ERR_NULL_POINTER;
     for (const void* p : {static_cast<const void*>(initial), static_cast<const void*>(final),
                           static_cast<const void*>(states), static_cast<const void*>(updates)})
         if (misaligned(p, 16)) return ASCAN_ERR_MISALIGNED;
@@ -137,6 +136,7 @@ int ascan_delta_forward(const void* q, const void* k, const void* v, const void*
     const Range to[] = {{out, rows * heads * dv * es}, {final, state}, {states, s.blocks * heads * dk * dv * 4},
                         {updates, rows * heads * dv * 4}, {workspace, need}};
     if (outputs_meet(in, to)) return ASCAN_ERR_OVERLAP;
+    if (rows > 0 && (states == nullptr) != (updates == nullptr)) return ASCAN_ERR_NULL_POINTER;
     const DeltaForward f{s, q, k, v, log_gates, beta, initial, out, final, states, updates,
                          static_cast<char*>(workspace), static_cast<hipStream_t>(stream)};
     switch (dtype) {
