@@ -94,6 +94,31 @@ int check_scan(const void* const* inputs, size_t count, int64_t rows, int64_t se
     return ASCAN_OK;
 }
 
+// Two bytes to a thread: every output is a whole number of them.
+__global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t n) {
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += gridDim.x * (int64_t)256) p[i] = 0;
+}
+
+// A call whose offsets hold no sequence: all rows are outside, outputs are zero.  (A kernel, so that a graph can have it.)
+template <size_t N>
+int zero_outputs(const Range (&out)[N], size_t alignment, void* stream) {
+    for (const Range& o : out) {
+        if (o.p == nullptr) return ASCAN_ERR_NULL_POINTER;
+        if (misaligned(o.p, alignment)) return ASCAN_ERR_MISALIGNED;
+    }
+    for (const Range& o : out) {
+        const int64_t groups = (o.bytes / 2 + 255) / 256;
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                           static_cast<uint16_t*>(const_cast<void*>(o.p)), o.bytes / 2);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            g_last_hip_error = (int)e;
+            return ASCAN_ERR_LAUNCH;
+        }
+    }
+    return ASCAN_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -120,6 +145,10 @@ int ascan_delta_forward(const void* q, const void* k, const void* v, const void*
     const void* needed[] = {log_gates, beta, q, k, v, out};
     const int status = check_scan(needed, 6, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
+    if (sequences == 0 && rows > 0) {  // (packed: others have no rows then)
+        const Range to[] = {{out, rows * heads * dv * es}};
+        return zero_outputs(to, es, stream);
+    }
     if (sequences == 0 || (rows == 0 && final == nullptr)) return ASCAN_OK;
     for (const void* p : {static_cast<const void*>(initial), static_cast<const void*>(final),
                           static_cast<const void*>(states), static_cast<const void*>(updates)})
@@ -156,6 +185,11 @@ int ascan_delta_backward(const void* q, const void* k, const void* v, const void
     const void* needed[] = {log_gates, beta, q, k, v, states, updates, d_q, d_k, d_v};
     const int status = check_scan(needed, 10, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
+    if (sequences == 0 && rows > 0) {
+        const Range to[] = {{d_q, rows * key_heads * dk * es}, {d_k, rows * key_heads * dk * es}, {d_v, rows * heads * dv * es},
+                            {d_log_gates, rows * heads * gs}, {d_beta, rows * heads * gs}};
+        return zero_outputs(to, es, stream);
+    }
     if (sequences == 0 || (rows == 0 && d_initial == nullptr)) return ASCAN_OK;
     if (rows > 0 && (d_log_gates == nullptr || d_beta == nullptr)) return ASCAN_ERR_NULL_POINTER;
     if (misaligned(d_log_gates, gs) || misaligned(d_beta, gs)) return ASCAN_ERR_MISALIGNED;

@@ -278,3 +278,10 @@ def test_states_and_updates_come_together(room):
         assert forward(room, **{name: kept[name]}) == NULL, name
     assert forward(room, **kept, out=room) == OVERLAP  # a pair gets past that check
     assert forward(room, states=room + 0x50000, rows=0, sequences=0) == OK
+
+
+@pytest.mark.parametrize("call, outputs", [(forward, ["out"]), (backward, ["d_q", "d_k", "d_v", "d_log_gates", "d_beta"])])
+def test_outputs_of_packed_rows_without_a_sequence_are_wanted(room, call, outputs):
+    for name in outputs:
+        assert call(room, sequences=0, offsets=room + 0xf0000, **{name: None}) == NULL, name
+        assert call(room, sequences=0, offsets=room + 0xf0000, **{name: room + 0x40001}) == MISALIGNED, name

@@ -769,3 +769,21 @@ def test_equal_keys_of_16_bits(tokens, key_dim, dtype):
     got, state = delta.gated_delta_scan(*on_gpu(data))
     ref.close(got, want, dtype)
     ref.close(state, final, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_packed_rows_without_a_sequence(dtype):
+    """The C entry points by themselves: all rows are outside of the sequences, outputs and gradients are zero."""
+    from accelerated_scan import _abi
+
+    for rows in (1, 70, 5000):
+        q, k, v, g, b, _ = on_gpu(ref.inputs(1, rows, 1, 3, 40, 24, dtype, seed=46))
+        offsets = torch.zeros(1, dtype=torch.int32, device=DEVICE)
+        new = lambda t: torch.full_like(t, float("nan"))  # noqa: E731
+        nothing = torch.empty(0, device=DEVICE)
+        out, final = new(v), torch.empty(0, 3, 40, 24, device=DEVICE)
+        _abi.delta_forward(q, k, v, g, b, None, offsets, 1.0, out, final)
+        grads = [new(t) for t in (q, k, v, g, b)]
+        _abi.delta_backward(q, k, v, g, b, nothing, nothing, offsets, 1.0, v, None, *grads, None)
+        for t in (out, *grads):
+            assert torch.equal(t, torch.zeros_like(t))
