@@ -76,7 +76,9 @@ int norm_backward_any(const void* x, const void* gate, const void* weight, const
         return norm_status(hipGetLastError());
     });
     if (status != ASCAN_OK) return status;
-    hipLaunchKernelGGL((norm_fold<E>), dim3((unsigned)((width + 15) / 16)), dim3(1024), 0, stream, partial,
+    // (up to 2^20 workgroups, which walk over the columns: an axis of a launch holds 2^32 threads, 2^26 columns)
+    const int64_t columns = (width + 15) / 16;
+    hipLaunchKernelGGL((norm_fold<E>), dim3((unsigned)(columns < (1 << 20) ? columns : (1 << 20))), dim3(1024), 0, stream, partial,
                        static_cast<S*>(d_weight), (int)parts, (int)width);
     return norm_status(hipGetLastError());
 }

@@ -238,19 +238,22 @@ __global__ __launch_bounds__(1024) void norm_fold(const float* __restrict__ part
                                                   int parts, int width) {
     __shared__ float sums[64][17];
     const int lane = threadIdx.x & 15, strip = threadIdx.x >> 4;
-    const int col = blockIdx.x * 16 + lane;
-    float sum = 0.0f;
-    if (col < width) {
+    for (int first = blockIdx.x * 16; first < width; first += gridDim.x * 16) {
+        const int col = first + lane;
+        float sum = 0.0f;
+        if (col < width) {
 #pragma unroll 4
-        for (int i = strip; i < parts; i += 64) sum += partial[(int64_t)i * width + col];
-    }
-    sums[strip][lane] = sum;
-    __syncthreads();
-    if (threadIdx.x < 256) {  // 16 threads to a column, four strips each, then across
-        const int at = threadIdx.x & 15, c = threadIdx.x >> 4;
-        float all = (sums[at][c] + sums[at + 16][c]) + (sums[at + 32][c] + sums[at + 48][c]);
-        all = sum16(all);
-        if (at == 0 && blockIdx.x * 16 + c < width) d_weight[blockIdx.x * 16 + c] = E::put(all);
+            for (int i = strip; i < parts; i += 64) sum += partial[(int64_t)i * width + col];
+        }
+        sums[strip][lane] = sum;
+        __syncthreads();
+        if (threadIdx.x < 256) {  // 16 threads to a column, four strips each, then across
+            const int at = threadIdx.x & 15, c = threadIdx.x >> 4;
+            float all = (sums[at][c] + sums[at + 16][c]) + (sums[at + 32][c] + sums[at + 48][c]);
+            all = sum16(all);
+            if (at == 0 && first + c < width) d_weight[first + c] = E::put(all);
+        }
+        __syncthreads();
     }
 }
 

@@ -145,3 +145,26 @@ def test_captured_backward_and_empty_rows():
     out = norm.gated_norm(empty, empty, weight)
     assert out.shape == (0, 8)
     assert not torch.autograd.grad(out.sum(), weight)[0].any()
+
+
+def test_rows_wider_than_a_launch_has_threads_for():
+    """The weight's gradient of 2^26 columns and more.  Elements of +-1 make the row's sum of squares exact; the mean over the
+    row that dx subtracts is a sum of 2^18 terms to a lane, each rounded to 2^-24 of it: 2^-6 of the terms' mean size."""
+    from accelerated_scan import norm
+
+    width = 2 ** 26 + 24
+    gen = torch.Generator(device=DEVICE).manual_seed(7)
+    x = torch.randn(1, width, generator=gen, device=DEVICE).sign().add(0.5).sign().to(torch.bfloat16)
+    z, d = (torch.randn(1, width, generator=gen, device=DEVICE).to(torch.bfloat16) for _ in range(2))
+    w = torch.ones(width, device=DEVICE, dtype=torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, z, w)]
+    dx, _, dw = torch.autograd.grad(norm.gated_norm(*leaves), leaves, d)
+    with torch.no_grad():
+        inverse = (1 + 1e-6) ** -0.5
+        e = d.double() * z.double() * torch.sigmoid(z.double())
+        want = (e * x.double()).squeeze(0) * inverse
+        u = 2.0 ** -8
+        assert ((dw.double() - want).abs() <= (u + 2.0 ** -17) * want.abs() + 2.0 ** -40).all()
+        mean = want.mean()
+        off = (dx.double() - (e - x.double() * inverse * mean) * inverse).abs()
+        assert (off <= (u + 2.0 ** -17) * e.abs() + 2 * 2.0 ** -6 * want.abs().mean()).all()
