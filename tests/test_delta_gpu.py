@@ -787,3 +787,57 @@ def test_packed_rows_without_a_sequence(dtype):
         _abi.delta_backward(q, k, v, g, b, nothing, nothing, offsets, 1.0, v, None, *grads, None)
         for t in (out, *grads):
             assert torch.equal(t, torch.zeros_like(t))
+
+
+MANY = [(64, 4, 8, 128, 128), (40, 8, 16, 96, 200), (90, 2, 6, 40, 256), (128, 2, 4, 64, 128), (35, 2, 8, 128, 136)]  # as in test_step
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", MANY, ids=str)
+def test_step_of_many_conversations(shape, dtype):
+    """512 workgroups of 128 columns and more: the wide variants, with states that leave a part of the rows or columns over."""
+    from accelerated_scan import delta
+
+    B, key_heads, heads, dk, dv = shape
+    assert B * heads * -(-dv // 128) >= 512
+    data = ref.inputs(B, 1, key_heads, heads, dk, dv, dtype, seed=47)
+    want, final = ref.delta_scan(*as_exact(data))
+    *inputs, state = on_gpu(data)
+    token = [t[:, 0].contiguous() for t in inputs]
+    got = delta.gated_delta_step(*token, state)
+    ref.close(got, want[:, 0], dtype)
+    ref.close(state, final, torch.float32)
+    # in the slots of a pool, in another order: the same states
+    gen = torch.Generator().manual_seed(48)
+    slots = torch.randperm(B + 5, generator=gen)[:B].to(DEVICE)
+    pool = torch.full((B + 5, heads, dk, dv), 7.0, device=DEVICE)
+    pool[slots] = data[5].to(DEVICE)
+    assert torch.equal(delta.gated_delta_step(*token, pool, slots=slots), got) and torch.equal(pool[slots], state)
+    rest = torch.ones(B + 5, dtype=torch.bool, device=DEVICE)
+    rest[slots] = False
+    assert (pool[rest] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", MANY[:3], ids=str)
+def test_slots_of_many_conversations(shape, dtype):
+    """Rows that share a slot, and rows without a state, among many."""
+    from accelerated_scan import delta
+
+    B, key_heads, heads, dk, dv = shape
+    count = B // 3
+    slots = torch.randint(-2, count + 2, (B,), generator=torch.Generator().manual_seed(49))
+    data = ref.inputs(B, 1, key_heads, heads, dk, dv, dtype, seed=50, sequences=count)
+    q, k, v, g, b, pool = as_exact(data)
+    want, want_pool = torch.zeros_like(v[:, 0]), pool.clone()
+    for row, slot in enumerate(slots.tolist()):
+        if 0 <= slot < count:
+            o, want_pool[slot:slot + 1] = ref.delta_scan(*(t[row:row + 1] for t in (q, k, v, g, b)), want_pool[slot:slot + 1].clone())
+            want[row] = o[0, 0]
+    *inputs, states = on_gpu(data)
+    got = delta.gated_delta_step(*[t[:, 0].contiguous() for t in inputs], states, slots=slots.to(torch.int32).to(DEVICE))
+    ref.close(got, want, dtype)
+    ref.close(states, want_pool, torch.float32)
+    for row, slot in enumerate(slots.tolist()):
+        if not 0 <= slot < count:
+            assert not got[row].any()

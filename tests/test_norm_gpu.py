@@ -168,3 +168,68 @@ def test_rows_wider_than_a_launch_has_threads_for():
         mean = want.mean()
         off = (dx.double() - (e - x.double() * inverse * mean) * inverse).abs()
         assert (off <= (u + 2.0 ** -17) * e.abs() + 2 * 2.0 ** -6 * want.abs().mean()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(33000, 96), (40001, 64), (8300, 257), (8203, 512), (2100, 1000), (2500, 1025), (2049, 2052),
+                                   (2100, 8200), (2050, 5001)], ids=str)
+def test_more_rows_than_workgroups(shape, dtype):
+    """The backward kernel's workgroups, 2048 at most, take several rows (of 16, 64 or 256 lanes) after one another, in every
+    variant: the bounds are those of test_norm_and_gradients."""
+    from accelerated_scan import norm
+
+    x, z, w, d = (t.to(DEVICE) for t in make(shape, dtype, 8))
+    leaves = [t.clone().requires_grad_() for t in (x, z, w)]
+    got = norm.gated_norm(*leaves)
+    dx, dz, dw = torch.autograd.grad(got, leaves, d)
+    u, e17 = torch.finfo(dtype).eps / 2, 2.0 ** -17
+    tiny = torch.finfo(dtype).smallest_normal * u * 2 + 2.0 ** -40
+    x, z, w, d = (t.double() for t in (x, z, w, d))
+    inverse = (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    s, h = torch.sigmoid(z), x * inverse
+    want = h * w * z * s
+    assert ((got.double() - want).abs() <= (u + e17) * want.abs() + tiny).all()
+    e = d * w * z * s
+    want_x = (e - h * (e * h).mean(-1, keepdim=True)) * inverse
+    assert ((dx.double() - want_x).abs() <= (u + e17) * want_x.abs() + 8 * e17 * want_x.abs().amax(-1, keepdim=True) + tiny).all()
+    want_z = d * w * h * s * (1 + z * (1 - s))
+    assert ((dz.double() - want_z).abs() <= (u + e17) * want_z.abs() + e17 * (d * w * h * s * (1 + z.abs())).abs() + tiny).all()
+    terms = d * h * z * s
+    # in fp32: rows / 2048 at most in a workgroup's chain, 32 shares in a thread's, then a tree
+    assert ((dw.double() - terms.sum(0)).abs() <= u * terms.sum(0).abs() + 2.0 ** -15 * terms.abs().sum(0) + tiny).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_more_rows_than_workgroups_start_anywhere(dtype):
+    """The same rows in tensors that do not start on 16 bytes, which take the element-wise variant."""
+    from accelerated_scan import norm
+
+    for shape in ((33000, 96), (2100, 1000), (2050, 5000)):
+        plain = [t.to(DEVICE) for t in make(shape, dtype, 9)]
+        odd = []
+        for t in plain:
+            odd.append(torch.empty(t.numel() + 1, dtype=dtype, device=DEVICE)[1:].view(t.shape).copy_(t))
+        assert odd[0].data_ptr() % 16
+        results = []
+        for x, z, w, d in (plain, odd):
+            leaves = [t.detach().requires_grad_() for t in (x, z, w)]
+            out = norm.gated_norm(*leaves)
+            results.append([out.detach(), *torch.autograd.grad(out, leaves, d)])
+        for a, b in zip(*results):  # sums in another order: 2^-15 of a sum's terms, whose size is at most its largest times 8
+            most = b.float().abs().max().item()
+            torch.testing.assert_close(a, b, rtol=2 * torch.finfo(dtype).eps, atol=8 * 2.0 ** -15 * most)
+
+
+@pytest.mark.parametrize("rows, width", [(2 ** 24 + 17, 8), (2 ** 22 + 3, 130), (2 ** 20 + 5, 520)])
+def test_more_rows_than_forward_workgroups(rows, width):
+    """The forward kernel's workgroups, 2^20 at most, take several rows after one another."""
+    from accelerated_scan import norm
+
+    gen = torch.Generator(device=DEVICE).manual_seed(10)
+    x, z = (torch.randn(rows, width, generator=gen, device=DEVICE, dtype=torch.bfloat16) for _ in range(2))
+    w = torch.randn(width, generator=gen, device=DEVICE, dtype=torch.bfloat16)
+    got = norm.gated_norm(x, z, w)
+    first = 2 ** 20 * (16 if width <= 128 else 4 if width <= 512 else 1)  # the second turn's first row
+    for some in (slice(0, 50), slice(first - 20, rows)):
+        want = ref.gated_norm(x[some].double(), z[some].double(), w.double())
+        assert ((got[some].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs() + 2.0 ** -40).all()
