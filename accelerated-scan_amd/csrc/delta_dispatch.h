@@ -71,7 +71,7 @@ int delta_forward_dk(const DeltaForward& f) {
         chain, dim3((unsigned)chain_grid(s)), 768, kChainBytes<NI, NS, DK>, f.stream,
         s, reinterpret_cast<const S*>(f.workspace + at.q), reinterpret_cast<const S*>(f.workspace + at.k), static_cast<const S*>(f.v),
         reinterpret_cast<const float*>(f.workspace + at.gates), f.workspace + at.t, f.workspace + at.p, f.initial,
-        static_cast<S*>(f.out), f.final, f.states, f.updates, chain_touches<NS, DK>(s)));
+        static_cast<S*>(f.out), f.final, f.states, f.updates, chain_touches<NI, NS, DK>(f.states != nullptr)));
 }
 
 template <class E, int NI, int NS, int DK>
@@ -89,7 +89,7 @@ int delta_backward_dk(const DeltaBackward& f) {
     float* d_rows = reinterpret_cast<float*>(ws + at.d_rows);
     e = delta_launch(delta_reverse_chain<E, NI, NS, DK>, dim3((unsigned)chain_grid(s)), 768, kReverseBytes<NI, NS, DK>, f.stream, s, reinterpret_cast<const S*>(ws + at.q), reinterpret_cast<const S*>(ws + at.k),
                      static_cast<const S*>(f.d_out), gates, ws + at.t, ws + at.p, f.d_final, static_cast<S*>(f.d_v),
-                     f.d_initial, d_states, d_rows, chain_touches<NS, DK>(s));
+                     f.d_initial, d_states, d_rows, chain_touches<NI, NS, DK>(true));
     if (e != hipSuccess || s.blocks == 0) return delta_status(e);
     const bool shared = s.heads > s.key_heads;
     const auto kernel = shared ? delta_gradients<E, NI, NS, DK, true> : delta_gradients<E, NI, NS, DK, false>;

@@ -36,12 +36,13 @@ __device__ __forceinline__ ChainAt chain_at(const DeltaShape& s) {
 }
 inline int64_t chain_grid(const DeltaShape& s) { return (s.sequences * s.heads + 7) / 8 * 8 * ((s.dv + 15) / 16); }
 
-// Whether a chain kernel asks for its blocks ahead (touch below).  It gains where a compute unit runs one chain of large
-// blocks: bf16 (2, 4096, 16 heads of 128 x 128) forward 155 -> 135 us, backward 201 -> 167, (1, 16384, 32 heads)
-// 394 -> 387; and gives nothing where workgroups follow each other (fp16, 16 packed sequences, 2048 workgroups: 243 us without,
-// 245 with), where blocks are small (key size 64: 58 and 58.5) and where fp32 products take longer than the loads (74 and 74).
-template <int NS, int DK>
-inline bool chain_touches(const DeltaShape& s) { return NS > 0 && DK == 128 && chain_grid(s) <= 512; }
+// Whether a chain kernel asks for its blocks ahead (touch below).  It gains where a block's loads are many beside its work:
+// chains that also write states (`keeps`) or run backward, training step bf16 (2, 4096, 16 heads of 128 x 128) 654 -> 599 us,
+// (4, 2048, 32 heads) 1336 -> 1210, and half values, whose keys take twice the room in LDS, (1, 16384, 32 heads) 822 -> 750 us,
+// (16, 512, 32 heads) 482 -> 469; it costs bf16 prompts 1 to 3 % (526 -> 530, 332 -> 343), and gives nothing where blocks are
+// small (key size 64: chains of 71 and 89 us 71 and 92) and where fp32 products take longer than the loads (73 and 73).
+template <int NI, int NS, int DK>
+constexpr bool chain_touches(bool keeps) { return NS > 0 && DK == 128 && (NI > 1 || keeps); }
 
 // A chain's workgroup may have as many lines of 128 bytes on their way as its compute unit's cache holds, 256.  At the
 // latency of memory, a microsecond, that is 32 KiB per microsecond where a block wants 60 (and nobody else uses the
@@ -68,7 +69,8 @@ template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
                             3 * Exchange<NS, 2>::kBytes + 2 * Exchange<NS, kPairs>::kBytes + 2 * 4 * kBlock * 4 + 64;
 
-constexpr int kPieces = kMatrixTiles / 4;  // tiles of T that a wave of four carries to LDS
+constexpr int kPieces = kMatrixTiles / 4;  // tiles of T that a wave of four carries to LDS: two that stand together, and one
+__device__ __forceinline__ constexpr int piece_tile(int wave, int i) { return i < 2 ? 2 * wave + i : 8 + wave; }
 
 // Zeros for what is not finite in an operand of tokens; the first such token, where its first four are row0 ..
 template <int P>
@@ -416,7 +418,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
             const Buffer tb = buffer_of(t_p, kMatrixBytes);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, matrix_place(0, piece_tile(wave, i), lane));
             gate_raw[set] = fetch4(gates_here(), tid * 4);
             v_p += v_move;
             if (first + kBlock < seq_length) {
@@ -435,8 +437,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) matrix_of(first).put(4 * i + wave, lane, t_kept[i]);
+            matrix_of(first).put_two(wave, lane, t_kept[0], t_kept[1]);
+            matrix_of(first).put(piece_tile(wave, 2), lane, t_kept[2]);
             gate_of(first)[tid] = gate_raw[set];
         };
         const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;
