@@ -302,7 +302,7 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
             const int d = col0 + (tid & 1) * 8;  // (the upper two waves repeat what the lower two do)
             o_raw[set] = fetch8<E>(ob, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, matrix_place(0, piece_tile(wave, i), lane));
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(buffer_of(gate_p, kGateFloats * 4), tid * 4);
             o_p -= v_move;
             if (n_block > 0) {
@@ -317,8 +317,8 @@ __global__ __launch_bounds__(768) void delta_reverse_chain(
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             outs_at(n_block).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, o_raw[set]);
-            matrix.put_two(wave, lane, matrix.kept(t_raw[set][0]), matrix.kept(t_raw[set][1]));
-            matrix.put(piece_tile(wave, 2), lane, t_raw[set][2]);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) matrix.put(4 * i + wave, lane, t_raw[set][i]);
             gate[tid] = gate_raw[set];
         };
         const auto stage_queries = [&](int set) __attribute__((always_inline)) {

@@ -69,8 +69,7 @@ template <int NI, int NS, int DK>
 constexpr int kChainBytes = 2 * Tile<NI, DK>::kBytes + 2 * Tile<NI, 16>::kBytes + Exchange<NS, DK / 32>::kBytes +
                             3 * Exchange<NS, 2>::kBytes + 2 * Exchange<NS, kPairs>::kBytes + 2 * 4 * kBlock * 4 + 64;
 
-constexpr int kPieces = kMatrixTiles / 4;  // tiles of T that a wave of four carries to LDS: two that stand together, and one
-__device__ __forceinline__ constexpr int piece_tile(int wave, int i) { return i < 2 ? 2 * wave + i : 8 + wave; }
+constexpr int kPieces = kMatrixTiles / 4;  // tiles of T that a wave of four carries to LDS
 
 // Zeros for what is not finite in an operand of tokens; the first such token, where its first four are row0 ..
 template <int P>
@@ -418,7 +417,7 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
             v_raw[set] = fetch8<E>(vb, d < s.dv ? ((tid & 127) >> 1) * v_step + d * kSize : kOutside);
             const Buffer tb = buffer_of(t_p, kMatrixBytes);
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, matrix_place(0, piece_tile(wave, i), lane));
+            for (int i = 0; i < kPieces; ++i) t_raw[set][i] = fetch16(tb, (tid + 256 * i) * 16);
             gate_raw[set] = fetch4(gates_here(), tid * 4);
             v_p += v_move;
             if (first + kBlock < seq_length) {
@@ -437,8 +436,8 @@ __global__ __launch_bounds__(768) void delta_chain(DeltaShape s, const typename 
 #pragma unroll
             for (int i = 0; i < kCopies; ++i) kb.template put8<E>((tid + 256 * i) / (DK / 8), (tid + 256 * i) % (DK / 8) * 8, k_raw[set][i]);
             values_at(first).template put8<E>((tid & 127) >> 1, (tid & 1) * 8, v_raw[set]);
-            matrix_of(first).put_two(wave, lane, t_kept[0], t_kept[1]);
-            matrix_of(first).put(piece_tile(wave, 2), lane, t_kept[2]);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) matrix_of(first).put(4 * i + wave, lane, t_kept[i]);
             gate_of(first)[tid] = gate_raw[set];
         };
         const int groups = (s.dv + 15) / 16, row_bytes = s.dv * (int)kSize;

@@ -471,17 +471,6 @@ struct Exchange {
         }
     }
     __device__ __forceinline__ void put(int tile, int lane, const fx4& x) { put(tile, lane, kept(x)); }
-    // Tiles 2n and 2n + 1: 16 bytes to a lane, where one tile's eight leave gaps that cost as much time again.
-    __device__ __forceinline__ void put_two(int n, int lane, const Kept& a, const Kept& b) {
-        if constexpr (P == 0) {
-            put(2 * n, lane, a);
-            put(2 * n + 1, lane, b);
-        } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-                *reinterpret_cast<ux4*>(base + ((i * N + n) * 64 + lane) * 16) = ux4{a.w[i][0], a.w[i][1], b.w[i][0], b.w[i][1]};
-        }
-    }
     __device__ __forceinline__ Operand<P> get(int n, int lane) const {
         Operand<P> o;
         if constexpr (P == 0) {
