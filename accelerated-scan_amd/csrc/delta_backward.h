@@ -392,12 +392,13 @@ constexpr int kGradientBytes = 2 * Tile<NI, DK>::kBytes + kGradientShared<NI, NS
 // A block of one head.  A wave owns 16 features of keys and queries and dk/2 of the tokens, so that each row of the two
 // states is read by one wave only (or two); the 64 x 64 products of tokens with tokens are divided among the waves by
 // tiles and go round through LDS.  The products have features as rows, so that a lane holds four of a token's and writes
-// 8 bytes (with tokens as rows 211 us instead of 194 for the case below; the five sums of a token that the gates'
-// gradients are made of, where two with terms that cancel would do, cost 15 again).
+// 8 bytes (with tokens as rows 211 us instead of 194 for the case below, when values were in two parts; the five sums of a token
+// that the gates' gradients are made of, where two with terms that cancel would do, cost 15 again).
 //
-// What bounds it: a workgroup reads 256 KiB and has a compute unit to itself, for its registers.  bf16 (2, 4096, 16 heads
-// of 128 x 128) takes 209 us for 0.7 GB, 3.4 TB/s; two thirds are left when nothing is read, a third of them LDS at work and
-// the rest latencies, so that loads and products overlap in part only.  A loop over heads or blocks around this body, to load ahead, lifts its address
+// What bounds it: a workgroup reads 256 KiB and has a compute unit to itself, for its registers (250).  bf16 (2, 4096, 16 heads
+// of 128 x 128) takes 229 to 246 us for 0.72 GB, 2.9 to 3.1 TB/s, with LDS at work a third of the time, vector instructions
+// 37 % and the matrix units 22 %; of 195 us in two parts 134 were left when nothing was read, so that loads and products overlap
+// in part only.  A loop over heads or blocks around this body, to load ahead, lifts its address
 // arithmetic in front, where it does not fit the registers (428 us for 218 at the time).
 //
 // SHARED: dQ and dK go to `sums` in fp32, to be added over the heads that share the keys (delta_fold).

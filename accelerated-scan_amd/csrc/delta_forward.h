@@ -9,11 +9,14 @@
 // and gates to LDS blocks ahead.  (The loads are 60 KiB a block, which the 64 bytes per clock of a compute unit's
 // cache turn into 960 clocks of issue: a wave that loads is late for its barrier if it has anything else to do.)
 //
-// What bounds it: bf16 (1, 16384, 32 heads of 128 x 128) takes 345 to 390 us, 256 blocks of 1.3 to 1.5 us, one chain to
-// a compute unit.  LDS is at work half of the time (200 KiB a block, 1600 clocks), the matrix units a fifth, beside three round trips (write,
-// barrier, read, product) of 300 to 400 clocks that nothing overlaps but the other waves' work.  More columns to a workgroup
-// would read less per column and leave compute units without one.  The chain that also writes states and U moves 0.5 GB
-// in 135 us (2, 4096, 16 heads).
+// What bounds it: bf16 (1, 16384, 32 heads of 128 x 128) takes 455 to 540 us, 256 blocks of 1.8 to 2.1 us, one chain to
+// a compute unit.  LDS is at work 54 % of the time (240 KiB a block, 1900 clocks), vector instructions 46 % (most of them splitting
+// values into parts), the matrix units 24 %, beside three round trips (write, barrier, read, product) of 300 to 400 clocks that
+// nothing overlaps but the other waves' work.  More columns to a workgroup
+// would read less per column and leave compute units without one.  The chain that also writes states and U moves 0.41 GB
+// in 141 to 155 us (2, 4096, 16 heads).
+// Registers, at 12 waves to a compute unit and a key size above 64: two of the bf16 chain are kept in memory, 14 of the
+// fp16 one and one of the fp32 one, nearly all of them addresses that the loop does not touch.
 #ifndef ASCAN_DELTA_FORWARD_H_
 #define ASCAN_DELTA_FORWARD_H_
 

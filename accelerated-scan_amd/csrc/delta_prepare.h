@@ -129,7 +129,7 @@ __device__ __forceinline__ constexpr int query_place(int row, int d) {
 // chain's workgroups, which all want the same rows at the same time, waited for it (bf16 (1, 16384, 32 heads of 128 x 128):
 // the chain 463 us without copies, 439 with; they cost this kernel 14).
 //
-// What bounds it: there it reads 130 MB and writes 350 MB in 107 us, 4.5 TB/s.
+// What bounds it: there it reads 130 MB and writes 350 MB in 104 to 112 us, 4.3 to 4.6 TB/s.
 template <class E, int NI, int DK, bool upper>
 __global__ __launch_bounds__(256, 4) void delta_prepare(DeltaShape s, const typename E::S* __restrict__ q,
                                                      const typename E::S* __restrict__ k,

@@ -20,8 +20,8 @@
 // Tensors of 16 bits are taken in the parts that hold them, everything computed in three: states, their gradients and those
 // of fp32 gates leave in 32 bits, and in two parts they were off by 0.7 to 6e-6 (with equal keys, whose U is a small difference
 // of large terms, a state by 6e-5) where fp32 arithmetic gives 1 to 3e-7, and 16-bit outputs by a last bit ten times as often.
-// Three parts throughout cost a bf16 prompt (1, 16384, 32 heads of 128 x 128) 430 -> 520 to 545 us, packed fp16 sequences 295 -> 388,
-// a training step (bf16, 2 x 4096, 16 heads) 567 -> 593.
+// Three parts throughout cost a bf16 prompt (1, 16384, 32 heads of 128 x 128) 430 -> 515 us, 16 packed fp16 sequences (12291
+// tokens, 16 heads) 295 -> 365, a training step (bf16, 2 x 4096, 16 heads) 567 -> 594.
 #ifndef ASCAN_DELTA_TILE_H_
 #define ASCAN_DELTA_TILE_H_
 

@@ -12,7 +12,11 @@ int norm_status(hipError_t e) {
     return ASCAN_ERR_LAUNCH;
 }
 
-// Workgroups of the backward kernel: eight to a compute unit, so that one's loads cover another's sums.
+// Workgroups of the backward kernel: eight to a compute unit, so that one's loads cover another's sums, where its registers let
+// as many in.  With the sum over their shares, for 512, 1024, 2048 and 4096 of them (us): bf16 rows of 128 (524288) 152, 140, 139, 141;
+// of 1024 (65536) 309, 226, 215, 211; of 2048 (16384) 94, 80, 79, 83; fp32 of 1000 (5001) 29, 26, 27, 31.  Rows above 2048 elements, whose
+// variant leaves room for one workgroup to a compute unit, would rather have fewer, since each costs a row of the shares: bf16 of
+// 4096, 16384 rows 278, 284, 294, 313 and 2048 rows 42, 47, 58, 58 (39 with 256 workgroups); of 8192 (16384) 365, 374, 397, 437.
 constexpr int64_t kNormParts = 2048;
 
 template <int L>
