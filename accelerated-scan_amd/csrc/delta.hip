@@ -100,12 +100,13 @@ __global__ __launch_bounds__(256) void zero_kernel(uint16_t* p, int64_t n) {
 }
 
 // A call whose offsets hold no sequence: all rows are outside, outputs are zero.  (A kernel, so that a graph can have it.)
-template <size_t N>
-int zero_outputs(const Range (&out)[N], size_t alignment, void* stream) {
+template <size_t NI, size_t NO>
+int zero_outputs(const Range (&in)[NI], const Range (&out)[NO], size_t alignment, void* stream) {
     for (const Range& o : out) {
         if (o.p == nullptr) return ASCAN_ERR_NULL_POINTER;
         if (misaligned(o.p, alignment)) return ASCAN_ERR_MISALIGNED;
     }
+    if (outputs_meet(in, out)) return ASCAN_ERR_OVERLAP;
     for (const Range& o : out) {
         const int64_t groups = (o.bytes / 2 + 255) / 256;
         hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, static_cast<hipStream_t>(stream),
@@ -146,8 +147,10 @@ int ascan_delta_forward(const void* q, const void* k, const void* v, const void*
     const int status = check_scan(needed, 6, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
     if (sequences == 0 && rows > 0) {  // (packed: others have no rows then)
+        const Range in[] = {{q, rows * key_heads * dk * es}, {k, rows * key_heads * dk * es}, {v, rows * heads * dv * es},
+                            {log_gates, rows * heads * gs}, {beta, rows * heads * gs}};
         const Range to[] = {{out, rows * heads * dv * es}};
-        return zero_outputs(to, es, stream);
+        return zero_outputs(in, to, es, stream);
     }
     if (sequences == 0 || (rows == 0 && final == nullptr)) return ASCAN_OK;
     for (const void* p : {static_cast<const void*>(initial), static_cast<const void*>(final),
@@ -186,9 +189,11 @@ int ascan_delta_backward(const void* q, const void* k, const void* v, const void
     const int status = check_scan(needed, 10, rows, sequences, heads, key_heads, dk, dv, dtype, flags, offsets, gs);
     if (status != ASCAN_OK) return status;
     if (sequences == 0 && rows > 0) {
+        const Range in[] = {{q, rows * key_heads * dk * es}, {k, rows * key_heads * dk * es}, {v, rows * heads * dv * es},
+                            {log_gates, rows * heads * gs}, {beta, rows * heads * gs}, {d_out, rows * heads * dv * es}};
         const Range to[] = {{d_q, rows * key_heads * dk * es}, {d_k, rows * key_heads * dk * es}, {d_v, rows * heads * dv * es},
                             {d_log_gates, rows * heads * gs}, {d_beta, rows * heads * gs}};
-        return zero_outputs(to, es, stream);
+        return zero_outputs(in, to, es, stream);
     }
     if (sequences == 0 || (rows == 0 && d_initial == nullptr)) return ASCAN_OK;
     if (rows > 0 && (d_log_gates == nullptr || d_beta == nullptr)) return ASCAN_ERR_NULL_POINTER;

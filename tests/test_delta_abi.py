@@ -285,3 +285,9 @@ def test_outputs_of_packed_rows_without_a_sequence_are_wanted(room, call, output
     for name in outputs:
         assert call(room, sequences=0, offsets=room + 0xf0000, **{name: None}) == NULL, name
         assert call(room, sequences=0, offsets=room + 0xf0000, **{name: room + 0x40001}) == MISALIGNED, name
+
+
+@pytest.mark.parametrize("call, outputs", [(forward, ["out"]), (backward, ["d_q", "d_v", "d_beta"])])
+def test_overlaps_of_packed_rows_without_a_sequence(room, call, outputs):
+    for name in outputs:
+        assert call(room, sequences=0, offsets=room + 0xf0000, **{name: room}) == OVERLAP, name
